@@ -8,4 +8,7 @@
 #include "gemm_glu_dw_sm100.cu"
 #include "attention_sm100.cu"
 #include "ctc_head.cu"
+#include "train_rows.cu"
+#include "ctc_loss.cu"
 #include "capi.cu"
+#include "capi_train.cu"

@@ -142,6 +142,67 @@ int launch_bpe_pool(const __nv_bfloat16* h, const float* blank, __nv_bfloat16* p
 int launch_ctc_collapse(const unsigned long long* keys, const int* plen, int* ids, int* tokens, int* counts, int B,
                         int Pp, int blank_id, cudaStream_t stream);
 
+// ---- row operators of fine-tuning (train_rows.cu) --------------------------------------------------------------
+// Rows of D elements (type: dtype 0 bf16, 1 fp16, 2 fp32), M = B * T of them; inputs have row strides, outputs are
+// dense.  Which fields an operation reads:
+//   kRowNorm          x, weight, bias -> y
+//   kRowDropout       x, residual (or null) -> y
+//   kRowDropNorm      x, residual, weight, bias -> y, h_out
+//   kRowNormGrad      x, dy, weight -> dx, dweight, dbias
+//   kRowDropNormGrad  x (the stored h), dy, dh (or null), weight -> dx, dres, dweight, dbias
+enum RowOp { kRowNorm = 0, kRowDropout = 1, kRowDropNorm = 2, kRowNormGrad = 3, kRowDropNormGrad = 4 };
+constexpr int kMaxRowWidth = 8192;
+struct RowArgs {
+  const void* x = nullptr;
+  const void* dy = nullptr;
+  const void* dh = nullptr;
+  const void* residual = nullptr;
+  int64_t ld_x = 0, ld_dy = 0, ld_dh = 0, ld_res = 0;
+  const void* weight = nullptr;
+  const void* bias = nullptr;
+  int param_fp32 = 0;            // weight, bias, dweight, dbias are fp32 (else of the rows' type)
+  void* y = nullptr;
+  void* h_out = nullptr;
+  void* dx = nullptr;
+  void* dres = nullptr;
+  void* dweight = nullptr;
+  void* dbias = nullptr;
+  float* partials = nullptr;     // [partial_rows][2][D]
+  int64_t partial_rows = 0;      // row_partial_rows(M, D)
+  const int64_t* rng = nullptr;  // device (seed, offset)
+  uint32_t site = 0, threshold = 0;   // an element is dropped where its 16-bit number is below the threshold
+  float factor = 1.f;            // a kept element is multiplied by it
+  const int* lengths = nullptr;  // [M / T] or null
+  int64_t M = 0;
+  int D = 0, T = 0, groups = 0;  // groups = ceil(D / 8)
+  float eps = 0.f;
+  int W = 1;                     // set by the launcher
+};
+int row_partial_rows(int64_t M, int D);
+int launch_row_op(const RowArgs& args, int op, int dtype, cudaStream_t stream);
+
+// ---- CTC loss and its gradient (ctc_loss.cu) ---------------------------------------------------------------------
+constexpr int kMaxCtcLabels = 2000;
+constexpr int kMaxCtcFrames = 32768;
+struct CtcArgs {
+  const void* logits = nullptr;  // [B, T, V], strides ld_b, ld_t, 1
+  int64_t ld_b = 0, ld_t = 0;
+  const int* targets = nullptr;  // [B, S]
+  const int* input_lengths = nullptr;
+  const int* target_lengths = nullptr;
+  int B = 0, T = 0, V = 0, S = 0, blank = 0;
+  int zero_infinity = 0;
+  float2* stats = nullptr;       // [B, T] (largest logit, log of the sum of exp(logit - largest))
+  float* post = nullptr;         // [B, T, S + 1]: logit - largest of blank and labels, then their posteriors
+  float* raw_loss = nullptr;     // [B] loss, inf where no path exists, NaN for bad input
+  float* loss = nullptr;         // [B] loss with zero_infinity applied
+  float2* alpha = nullptr;       // workspace [B, T, 2 S + 1], or null: no posteriors wanted
+  const float* dloss = nullptr;  // [B]
+  void* dlogits = nullptr;       // [B, T, V] dense
+};
+int launch_ctc_loss(const CtcArgs& args, int dtype, cudaStream_t stream);
+int launch_ctc_grad(const CtcArgs& args, int dtype, cudaStream_t stream);
+
 // ---- self-test of the bounded wait (capi.cu) ----------------------------------------------------------------
 int launch_wait_selftest(uint64_t limit_ns, cudaStream_t stream);
 

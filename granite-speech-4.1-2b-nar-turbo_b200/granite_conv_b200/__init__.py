@@ -5,7 +5,7 @@ rest of the Conformer block (feed-forward halves, block-local attention, post no
 Importing the package registers the ops; the CUDA library itself is loaded on the first call and its absence is
 an error, never a fallback.
 """
-from . import ops  # noqa: F401  registers the granite:: custom ops
+from . import ops, training  # noqa: F401  registers the granite:: custom ops
 from .conv_kernel import enable_dwconv_silu  # noqa: F401
 from .dispatch import Chunk, bucket_frames, plan_chunks, shard_chunks  # noqa: F401
 from .block import (ConformerEncoderStack, PreparedConformerBlock, prepare_block_from_params,  # noqa: F401

@@ -17,6 +17,8 @@ _vp = ctypes.c_void_p
 _i32 = ctypes.c_int
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
+_u32 = ctypes.c_uint32
 _u64 = ctypes.c_uint64
 _sz = ctypes.c_size_t
 _fp = ctypes.c_void_p     # float* passed as an address
@@ -85,6 +87,20 @@ SIGNATURES = {
     "gsn_quant_rows_bf16": (_i32, [_vp, _i64, _vp, _fp, _i32, _i32, _vp, _i32, _vp]),
     "gsn_conv_module_bf16_noalloc": (_i32, [_vp, _vp, _vp, _vp, _fp, _vp, _vp, _vp, _fp, _vp, _i32, _vp, _i32,
                                             _i32, _i32, _i32, _f32, _vp]),
+    "gsn_layer_norm_fwd": (_i32, [_vp, _i64, _vp, _vp, _vp, _i64, _i32, _f32, _i32, _i32, _vp, _i32, _vp]),
+    "gsn_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i32]),
+    "gsn_layer_norm_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _f32, _i32, _i32, _vp, _i32,
+                                  _vp, _sz, _vp]),
+    "gsn_dropout_add": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _u32, _f64, _f64, _vp, _i32, _vp]),
+    "gsn_dropout_add_layer_norm_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _f32, _i32, _i32,
+                                              _vp, _u32, _f64, _f64, _vp, _i32, _vp]),
+    "gsn_dropout_add_layer_norm_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i32,
+                                              _f32, _i32, _i32, _vp, _u32, _f64, _f64, _vp, _i32, _vp, _sz, _vp]),
+    "gsn_ctc_loss_workspace_bytes": (_sz, [_i32, _i32, _i32]),
+    "gsn_ctc_loss_fwd": (_i32, [_vp, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _fp, _fp, _fp,
+                                _fp, _vp, _sz, _vp]),
+    "gsn_ctc_loss_bwd": (_i32, [_fp, _vp, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _fp, _fp,
+                                _fp, _vp, _vp]),
     "gsn_interleave_glu_rows": (_i32, [_vp, _vp, _i32, _i64, _vp]),
     "gsn_device_status": (_i32, [ctypes.POINTER(_i32), _i32, _vp]),
     "gsn_selftest_bounded_wait": (_i32, [_u64, _vp]),

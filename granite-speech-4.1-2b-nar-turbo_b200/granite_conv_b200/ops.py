@@ -14,7 +14,8 @@ plus the ops of the whole module (new):
 * ``granite::conv_module_lnfold(x, w1g_glu, b1g_glu, c1_glu, dw_w, dw_b, w2, b2, lengths?, ln_eps, add_residual)``
   (the LayerNorm folded into the up_conv GEMM; T % 128 == 0)
 * ``granite::feed_forward_half(x, ln_w, ln_b, w_up, b_up, w_down, b_down, lengths?, ln_eps)`` (x + 0.5 FF(x))
-* ``granite::layer_norm(x, weight, bias, eps)`` (the block's post LayerNorm)
+* ``granite::layer_norm(x, weight, bias, eps, lengths?)`` (the block's post LayerNorm; differentiable, see
+  ``training`` for the operators of fine-tuning)
 * ``granite::attention_block(x, ln_w, ln_b, w_qkv, b_qkv, w_out, b_out, rel, lengths?, heads, context, max_pos,
   ln_eps)`` (x + ConformerAttention(x), block-local with Shaw relative positions)
 * ``granite::ctc_selfcond(x, w_out, b_out, w_mid, b_mid, lengths?, n_cls)`` -> (x', blank) (the middle CTC head)
@@ -33,9 +34,10 @@ from typing import Optional
 
 import torch
 
-from . import _lib
+from . import _lib, training
 
 KERNEL_SIZE = 15
+LAYERNORM_WIDTHS = (256, 512, 1024, 2048)     # of the inference kernel (gsn_layernorm_bf16)
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -279,17 +281,37 @@ def _(x, ln_w, ln_b, w_up, b_up, w_down, b_down, lengths, ln_eps):
 
 
 @torch.library.custom_op("granite::layer_norm", mutates_args=(), device_types="cuda")
-def layer_norm_op(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, eps: float) -> torch.Tensor:
-    """nn.LayerNorm over the last dim of bf16 x [..., D] (the block's post_norm, conformer.py:199, :209)."""
+def layer_norm_op(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, eps: float,
+                  lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """nn.LayerNorm over the last dim of x [..., D] (the block's post_norm, conformer.py:199, :209), differentiable; x
+    bf16, fp16 or fp32, weight and bias fp32 or of x's type, D <= 8192.  lengths (int [B] beside x [B, T, D]): padding
+    frames are not read and give 0."""
     _require_cuda("granite::layer_norm", x, weight, bias)
     D = x.shape[-1]
-    x2 = x.contiguous().view(-1, D)
-    return layernorm(x2, weight, bias, eps).view(x.shape)
+    if (lengths is None and x.dtype == weight.dtype == bias.dtype == torch.bfloat16 and D in LAYERNORM_WIDTHS
+            and weight.is_contiguous() and bias.is_contiguous()
+            and not (weight.data_ptr() | bias.data_ptr() | x.data_ptr()) & 15):
+        x2 = x.contiguous().view(-1, D)
+        return layernorm(x2, weight, bias, eps).view(x.shape)
+    return training._layer_norm(x, weight, bias, eps, lengths)
 
 
 @layer_norm_op.register_fake
-def _(x, weight, bias, eps):
+def _(x, weight, bias, eps, lengths=None):
     return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def _layer_norm_setup(ctx, inputs, output):
+    x, weight, _, ctx.eps, lengths = inputs
+    ctx.save_for_backward(x, weight, lengths)
+
+
+def _layer_norm_grad(ctx, dy):
+    x, weight, lengths = ctx.saved_tensors
+    return (*torch.ops.granite.layer_norm_backward(dy, x, weight, ctx.eps, lengths), None, None)
+
+
+layer_norm_op.register_autograd(_layer_norm_grad, setup_context=_layer_norm_setup)
 
 
 # ---- block-local attention with Shaw relative positions -----------------------------------------------------------

@@ -1,0 +1,501 @@
+"""Operators for fine-tuning the encoder: the layer norm with its backward pass, dropout with a residual (the mask
+regenerated from a counter, never stored), the residual step fused with the norm behind it (a Conformer block's tail,
+``models/granite_speech_nar/conformer.py:208-209``), and the CTC loss of the heads (``:240-252``) with its gradient.
+
+The functions here take plain tensors and are differentiable; without a gradient to record they launch the kernel
+directly.  Each is also a ``torch.library`` op, so ``torch.compile(fullgraph=True)`` sees one node:
+
+* ``granite::layer_norm(x, weight, bias, eps, lengths?)``, ``granite::layer_norm_backward``
+* ``granite::dropout_add(x, residual?, rng, p, scale, site, lengths?)``
+* ``granite::dropout_add_layer_norm(x, residual, weight, bias, rng, p, scale, site, eps, lengths?) -> (y, h)``,
+  ``granite::dropout_add_layer_norm_backward``
+* ``granite::ctc_loss(logits, targets, input_lengths, target_lengths, blank, zero_infinity)``,
+  ``granite::ctc_loss_backward``
+
+Tensors are bf16, fp16 or fp32 on one CUDA device, parameters fp32 or of the activations' type; work runs on that
+device's current stream.  Results repeat bit for bit.  ``lengths`` (int [B], with x [B, T, D]) marks the frames
+t >= lengths[b] as padding: nothing of them is read, normed outputs and gradients there are zero, they join no weight
+gradient, and a residual passes through.
+
+``rng`` is an int64 tensor of two on the device, (seed, offset), which the kernels read when they run: a captured graph
+draws new masks when it holds ``rng[1] += 1`` after its backward pass.  ``site`` tells apart the dropouts of one step.
+"""
+from __future__ import annotations
+
+import contextlib
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_HERE = contextlib.nullcontext()
+MAX_NORM_WIDTH = 8192
+MAX_CTC_LABELS = 2000
+MAX_CTC_FRAMES = 32768
+
+
+def _on(device: torch.device):
+    """The launches go to the current device: make the tensors' device that."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _check_device(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    if not first.is_cuda:
+        raise RuntimeError(f"{name}: every tensor must be on a CUDA device (got {first.device}); the kernels have no "
+                           "CPU path")
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f"{name}: tensors on {first.device} and {t.device}")
+
+
+def _check_rows(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    if first.dim() < 1 or first.shape[-1] == 0:
+        raise RuntimeError(f"{name}: rows of at least one element expected, got {tuple(first.shape)}")
+    if first.dtype not in _TYPES:
+        raise RuntimeError(f"{name}: bf16, fp16 or fp32 tensors expected, got {first.dtype}")
+    for t in others:
+        if t is not None and (t.dtype != first.dtype or t.shape != first.shape):
+            raise RuntimeError(f"{name}: {first.dtype} {tuple(first.shape)} against {t.dtype} {tuple(t.shape)}")
+
+
+def _check_params(name: str, x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor]) -> None:
+    D = x.shape[-1]
+    if D > MAX_NORM_WIDTH:
+        raise RuntimeError(f"{name}: width {D}, at most {MAX_NORM_WIDTH}")
+    if weight.shape != (D,) or (bias is not None and bias.shape != (D,)):
+        raise RuntimeError(f"{name}: weight and bias must be [{D}]")
+    if weight.dtype not in (torch.float32, x.dtype) or (bias is not None and bias.dtype != weight.dtype):
+        raise RuntimeError(f"{name}: weight and bias must both be fp32 or {x.dtype}")
+
+
+def _check_dropout(name: str, rng: torch.Tensor, p: float, site: int) -> None:
+    if rng.dtype != torch.int64 or rng.shape != (2,):
+        raise RuntimeError(f"{name}: rng must be int64 [2] (seed, offset), got {rng.dtype} {tuple(rng.shape)}")
+    if not 0.0 <= p <= 1.0:
+        raise RuntimeError(f"{name}: p={p} is not a probability")
+    if not 0 <= site < 2 ** 32:
+        raise RuntimeError(f"{name}: site={site} outside [0, 2^32)")
+
+
+def _check_lengths(name: str, x: torch.Tensor, lengths: Optional[torch.Tensor]) -> Tuple[Optional[torch.Tensor], int]:
+    if lengths is None:
+        return None, 0
+    if x.dim() != 3 or lengths.shape != x.shape[:1] or lengths.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"{name}: lengths must be int [B] beside [B, T, D], got {lengths.dtype} "
+                           f"{tuple(lengths.shape)} beside {tuple(x.shape)}")
+    return lengths.to(torch.int32).contiguous(), x.shape[1]
+
+
+def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """(tensor, row stride): t itself where its rows are dense and evenly spaced, else a copy."""
+    D = t.shape[-1]
+    if t.is_contiguous():
+        return t, D
+    if t.stride(-1) == 1 or D == 1:
+        try:
+            r = t.view(-1, D)
+        except RuntimeError:
+            return t.contiguous(), D
+        if r.shape[0] <= 1:
+            return t, D
+        if r.stride(0) >= D:
+            return t, r.stride(0)
+    return t.contiguous(), D
+
+
+# ---- layer norm ------------------------------------------------------------------------------------------------------
+def _layer_norm(x, weight, bias, eps, lengths):
+    name = "granite::layer_norm"
+    _check_device(name, x, weight, bias, lengths)
+    _check_rows(name, x)
+    _check_params(name, x, weight, bias)
+    lens, T = _check_lengths(name, x, lengths)
+    D = x.shape[-1]
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with _on(x.device):
+        xr, ld = _rows(x)
+        w, b = weight.contiguous(), bias.contiguous()
+        _lib.call("gsn_layer_norm_fwd", xr.data_ptr(), ld, w.data_ptr(), b.data_ptr(), y.data_ptr(), y.numel() // D, D,
+                  eps, _TYPES[x.dtype], _TYPES[w.dtype], _ptr(lens), T, _stream(x.device))
+    return y
+
+
+def _layer_norm_backward(dy, x, weight, eps, lengths):
+    name = "granite::layer_norm_backward"
+    _check_device(name, x, dy, weight, lengths)
+    _check_rows(name, x, dy)
+    _check_params(name, x, weight, None)
+    lens, T = _check_lengths(name, x, lengths)
+    D = x.shape[-1]
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    M = dx.numel() // D
+    dw = torch.empty((D,), dtype=weight.dtype, device=x.device)
+    db = torch.empty((D,), dtype=weight.dtype, device=x.device)
+    with _on(x.device):
+        xr, ld_x = _rows(x)
+        gr, ld_g = _rows(dy)
+        w = weight.contiguous()
+        nbytes = _lib.lib().gsn_layer_norm_bwd_workspace_bytes(M, D)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=x.device)
+        _lib.call("gsn_layer_norm_bwd", gr.data_ptr(), ld_g, xr.data_ptr(), ld_x, w.data_ptr(), dx.data_ptr(),
+                  dw.data_ptr(), db.data_ptr(), M, D, eps, _TYPES[x.dtype], _TYPES[w.dtype], _ptr(lens), T,
+                  ws.data_ptr(), nbytes, _stream(x.device))
+    return dx, dw, db
+
+
+@torch.library.custom_op("granite::layer_norm_backward", mutates_args=(), device_types="cuda")
+def layer_norm_backward_op(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: float,
+                           lengths: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dweight, dbias) of granite::layer_norm."""
+    return _layer_norm_backward(dy, x, weight, eps, lengths)
+
+
+@layer_norm_backward_op.register_fake
+def _(dy, x, weight, eps, lengths):
+    return (torch.empty_like(x, memory_format=torch.contiguous_format), weight.new_empty(weight.shape),
+            weight.new_empty(weight.shape))
+
+
+def _recorded(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a call has to go through the dispatcher: a gradient to record, or a graph being compiled."""
+    if torch.compiler.is_compiling():
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, eps: float = 1e-5,
+               lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """nn.LayerNorm over the last dim, differentiable in x, weight and bias."""
+    if _recorded(x, weight, bias):
+        return torch.ops.granite.layer_norm(x, weight, bias, eps, lengths)
+    return _layer_norm(x, weight, bias, eps, lengths)
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5,
+                        lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dweight, dbias) of layer_norm at x for the gradient dy of its output."""
+    if torch.compiler.is_compiling():
+        return torch.ops.granite.layer_norm_backward(dy, x, weight, eps, lengths)
+    return _layer_norm_backward(dy, x, weight, eps, lengths)
+
+
+# ---- dropout with a residual -----------------------------------------------------------------------------------------
+def _dropout_add(x, residual, rng, p, scale, site, lengths):
+    name = "granite::dropout_add"
+    _check_device(name, x, residual, rng, lengths)
+    _check_rows(name, x, residual)
+    _check_dropout(name, rng, p, site)
+    lens, T = _check_lengths(name, x, lengths)
+    D = x.shape[-1]
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with _on(x.device):
+        xr, ld_x = _rows(x)
+        rr, ld_r = (None, 0) if residual is None else _rows(residual)
+        _lib.call("gsn_dropout_add", xr.data_ptr(), ld_x, _ptr(rr), ld_r, out.data_ptr(), out.numel() // D, D,
+                  _TYPES[x.dtype], rng.contiguous().data_ptr(), site, p, scale, _ptr(lens), T, _stream(x.device))
+    return out
+
+
+@torch.library.custom_op("granite::dropout_add", mutates_args=(), device_types="cuda")
+def dropout_add_op(x: torch.Tensor, residual: Optional[torch.Tensor], rng: torch.Tensor, p: float, scale: float,
+                   site: int, lengths: Optional[torch.Tensor]) -> torch.Tensor:
+    """residual + scale * dropout(x) (scale * dropout(x) without a residual)."""
+    return _dropout_add(x, residual, rng, p, scale, site, lengths)
+
+
+@dropout_add_op.register_fake
+def _(x, residual, rng, p, scale, site, lengths):
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def _dropout_add_setup(ctx, inputs, output):
+    _, residual, rng, ctx.p, ctx.scale, ctx.site, lengths = inputs
+    ctx.save_for_backward(rng, lengths)
+    ctx.with_residual = residual is not None
+
+
+def _dropout_add_grad(ctx, dout):
+    rng, lengths = ctx.saved_tensors
+    dx = None
+    if ctx.needs_input_grad[0]:
+        dx = torch.ops.granite.dropout_add(dout, None, rng, ctx.p, ctx.scale, ctx.site, lengths)
+    return dx, dout if ctx.with_residual else None, None, None, None, None, None
+
+
+dropout_add_op.register_autograd(_dropout_add_grad, setup_context=_dropout_add_setup)
+
+
+def dropout_add(x: torch.Tensor, rng: torch.Tensor, p: float, residual: Optional[torch.Tensor] = None,
+                scale: float = 1.0, site: int = 0, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """residual + scale * dropout(x, p), differentiable in x and residual; p to the nearest 1 / 65536."""
+    if _recorded(x, residual):
+        return torch.ops.granite.dropout_add(x, residual, rng, p, scale, site, lengths)
+    return _dropout_add(x, residual, rng, p, scale, site, lengths)
+
+
+def dropout_add_backward(dout: torch.Tensor, rng: torch.Tensor, p: float, scale: float = 1.0, site: int = 0,
+                         lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The gradient of dropout_add's x for the gradient dout of its output (the residual's is dout itself)."""
+    if torch.compiler.is_compiling():
+        return torch.ops.granite.dropout_add(dout, None, rng, p, scale, site, lengths)
+    return _dropout_add(dout, None, rng, p, scale, site, lengths)
+
+
+# ---- dropout, residual and layer norm in one pass --------------------------------------------------------------------
+def _dropout_add_layer_norm(x, residual, weight, bias, rng, p, scale, site, eps, lengths):
+    name = "granite::dropout_add_layer_norm"
+    _check_device(name, x, residual, weight, bias, rng, lengths)
+    _check_rows(name, x, residual)
+    _check_params(name, x, weight, bias)
+    _check_dropout(name, rng, p, site)
+    lens, T = _check_lengths(name, x, lengths)
+    D = x.shape[-1]
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with _on(x.device):
+        xr, ld_x = _rows(x)
+        rr, ld_r = _rows(residual)
+        w, b = weight.contiguous(), bias.contiguous()
+        _lib.call("gsn_dropout_add_layer_norm_fwd", xr.data_ptr(), ld_x, rr.data_ptr(), ld_r, w.data_ptr(),
+                  b.data_ptr(), y.data_ptr(), h.data_ptr(), y.numel() // D, D, eps, _TYPES[x.dtype], _TYPES[w.dtype],
+                  rng.contiguous().data_ptr(), site, p, scale, _ptr(lens), T, _stream(x.device))
+    return y, h
+
+
+def _dropout_add_layer_norm_backward(dy, dh, h, weight, rng, p, scale, site, eps, lengths):
+    name = "granite::dropout_add_layer_norm_backward"
+    _check_device(name, h, dy, dh, weight, rng, lengths)
+    _check_rows(name, h, dy, dh)
+    _check_params(name, h, weight, None)
+    _check_dropout(name, rng, p, site)
+    lens, T = _check_lengths(name, h, lengths)
+    D = h.shape[-1]
+    dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    dres = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    M = dx.numel() // D
+    dw = torch.empty((D,), dtype=weight.dtype, device=h.device)
+    db = torch.empty((D,), dtype=weight.dtype, device=h.device)
+    with _on(h.device):
+        hr, ld_h = _rows(h)
+        gr, ld_g = _rows(dy)
+        sr, ld_s = (None, 0) if dh is None else _rows(dh)
+        w = weight.contiguous()
+        nbytes = _lib.lib().gsn_layer_norm_bwd_workspace_bytes(M, D)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=h.device)
+        _lib.call("gsn_dropout_add_layer_norm_bwd", gr.data_ptr(), ld_g, _ptr(sr), ld_s, hr.data_ptr(), ld_h,
+                  w.data_ptr(), dx.data_ptr(), dres.data_ptr(), dw.data_ptr(), db.data_ptr(), M, D, eps,
+                  _TYPES[h.dtype], _TYPES[w.dtype], rng.contiguous().data_ptr(), site, p, scale, _ptr(lens), T,
+                  ws.data_ptr(), nbytes, _stream(h.device))
+    return dx, dres, dw, db
+
+
+@torch.library.custom_op("granite::dropout_add_layer_norm", mutates_args=(), device_types="cuda")
+def dropout_add_layer_norm_op(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor,
+                              rng: torch.Tensor, p: float, scale: float, site: int, eps: float,
+                              lengths: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(y, h): h = residual + scale * dropout(x), y = layer_norm(h) of the fp32 sum."""
+    return _dropout_add_layer_norm(x, residual, weight, bias, rng, p, scale, site, eps, lengths)
+
+
+@dropout_add_layer_norm_op.register_fake
+def _(x, residual, weight, bias, rng, p, scale, site, eps, lengths):
+    dense = torch.contiguous_format
+    return torch.empty_like(x, memory_format=dense), torch.empty_like(x, memory_format=dense)
+
+
+@torch.library.custom_op("granite::dropout_add_layer_norm_backward", mutates_args=(), device_types="cuda")
+def dropout_add_layer_norm_backward_op(
+        dy: torch.Tensor, dh: Optional[torch.Tensor], h: torch.Tensor, weight: torch.Tensor, rng: torch.Tensor,
+        p: float, scale: float, site: int, eps: float, lengths: Optional[torch.Tensor]
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dresidual, dweight, dbias) of granite::dropout_add_layer_norm from its stored h."""
+    return _dropout_add_layer_norm_backward(dy, dh, h, weight, rng, p, scale, site, eps, lengths)
+
+
+@dropout_add_layer_norm_backward_op.register_fake
+def _(dy, dh, h, weight, rng, p, scale, site, eps, lengths):
+    dense = torch.contiguous_format
+    return (torch.empty_like(h, memory_format=dense), torch.empty_like(h, memory_format=dense),
+            weight.new_empty(weight.shape), weight.new_empty(weight.shape))
+
+
+def _dropout_add_layer_norm_setup(ctx, inputs, output):
+    _, _, weight, _, rng, ctx.p, ctx.scale, ctx.site, ctx.eps, lengths = inputs
+    ctx.save_for_backward(output[1], weight, rng, lengths)
+    ctx.set_materialize_grads(False)               # an unused output sends nothing back, and nothing is read for it
+
+
+def _dropout_add_layer_norm_grad(ctx, dy, dh):
+    h, weight, rng, lengths = ctx.saved_tensors
+    rest = (None,) * 6
+    if dy is None and dh is None:
+        return (None,) * 10
+    if dy is None:
+        dx = torch.ops.granite.dropout_add(dh, None, rng, ctx.p, ctx.scale, ctx.site, lengths)
+        return (dx, dh, None, None, *rest)
+    grads = torch.ops.granite.dropout_add_layer_norm_backward(dy, dh, h, weight, rng, ctx.p, ctx.scale, ctx.site,
+                                                              ctx.eps, lengths)
+    return (*grads, *rest)
+
+
+dropout_add_layer_norm_op.register_autograd(_dropout_add_layer_norm_grad, setup_context=_dropout_add_layer_norm_setup)
+
+
+def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor,
+                           rng: torch.Tensor, p: float, scale: float = 1.0, site: int = 0, eps: float = 1e-5,
+                           lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(y, h): h = residual + scale * dropout(x, p), y = layer_norm(h); differentiable in x, residual, weight, bias."""
+    if _recorded(x, residual, weight, bias):
+        return torch.ops.granite.dropout_add_layer_norm(x, residual, weight, bias, rng, p, scale, site, eps, lengths)
+    return _dropout_add_layer_norm(x, residual, weight, bias, rng, p, scale, site, eps, lengths)
+
+
+def dropout_add_layer_norm_backward(dy: torch.Tensor, dh: Optional[torch.Tensor], h: torch.Tensor,
+                                    weight: torch.Tensor, rng: torch.Tensor, p: float, scale: float = 1.0,
+                                    site: int = 0, eps: float = 1e-5, lengths: Optional[torch.Tensor] = None
+                                    ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dresidual, dweight, dbias) for the gradients dy of y and dh of h (None: nothing comes back to h)."""
+    if torch.compiler.is_compiling():
+        return torch.ops.granite.dropout_add_layer_norm_backward(dy, dh, h, weight, rng, p, scale, site, eps, lengths)
+    return _dropout_add_layer_norm_backward(dy, dh, h, weight, rng, p, scale, site, eps, lengths)
+
+
+# ---- CTC loss --------------------------------------------------------------------------------------------------------
+def _ctc_check(name, logits, targets, input_lengths, target_lengths, blank):
+    _check_device(name, logits, targets, input_lengths, target_lengths)
+    if logits.dim() != 3 or logits.dtype not in _TYPES or logits.shape[2] == 0:
+        raise RuntimeError(f"{name}: logits must be bf16, fp16 or fp32 [B, T, V], got {logits.dtype} "
+                           f"{tuple(logits.shape)}")
+    B, T, V = logits.shape
+    ints = (torch.int32, torch.int64)
+    if targets.dim() != 2 or targets.shape[0] != B or targets.dtype not in ints:
+        raise RuntimeError(f"{name}: targets must be int [{B}, S], got {targets.dtype} {tuple(targets.shape)}")
+    for t in (input_lengths, target_lengths):
+        if t.shape != (B,) or t.dtype not in ints:
+            raise RuntimeError(f"{name}: lengths must be int [{B}], got {t.dtype} {tuple(t.shape)}")
+    if not 0 <= blank < V:
+        raise RuntimeError(f"{name}: blank={blank} outside the {V} classes")
+    if targets.shape[1] > MAX_CTC_LABELS or T > MAX_CTC_FRAMES:
+        raise RuntimeError(f"{name}: {targets.shape[1]} labels and {T} frames, at most {MAX_CTC_LABELS} and "
+                           f"{MAX_CTC_FRAMES}")
+
+
+def _ctc_operands(logits, targets, input_lengths, target_lengths):
+    B, T, V = logits.shape
+    sb, st, sv = logits.stride()
+    if (sv != 1 and V > 1) or (st < V and T > 1):
+        logits = logits.contiguous()
+        sb, st, _ = logits.stride()
+    i32 = [t.to(torch.int32).contiguous() for t in (targets, input_lengths, target_lengths)]
+    return logits, sb, st if T > 1 else V, i32
+
+
+def _ctc_loss(logits, targets, input_lengths, target_lengths, blank, zero_infinity, gradient):
+    name = "granite::ctc_loss"
+    _ctc_check(name, logits, targets, input_lengths, target_lengths, blank)
+    B, T, V = logits.shape
+    S = targets.shape[1]
+    dev = logits.device
+    loss = torch.empty((B,), dtype=torch.float32, device=dev)
+    raw = torch.empty((B,), dtype=torch.float32, device=dev)
+    stats = torch.empty((B, T, 2), dtype=torch.float32, device=dev)
+    post = torch.empty((B, T, S + 1), dtype=torch.float32, device=dev)
+    with _on(dev):
+        x, sb, st, (tg, il, tl) = _ctc_operands(logits, targets, input_lengths, target_lengths)
+        nbytes = _lib.lib().gsn_ctc_loss_workspace_bytes(B, T, S) if gradient else 0
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
+        _lib.call("gsn_ctc_loss_fwd", x.data_ptr(), sb, st, tg.data_ptr(), il.data_ptr(), tl.data_ptr(), B, T, V, S,
+                  blank, int(zero_infinity), _TYPES[x.dtype], loss.data_ptr(), raw.data_ptr(), stats.data_ptr(),
+                  post.data_ptr(), _ptr(ws), nbytes, _stream(dev))
+    return loss, raw, stats, post
+
+
+def _ctc_loss_backward(dloss, logits, targets, input_lengths, target_lengths, raw, stats, post, blank, zero_infinity):
+    name = "granite::ctc_loss_backward"
+    _ctc_check(name, logits, targets, input_lengths, target_lengths, blank)
+    _check_device(name, logits, dloss, raw, stats, post)
+    B, T, V = logits.shape
+    S = targets.shape[1]
+    if dloss.shape != (B,) or raw.shape != (B,) or stats.shape != (B, T, 2) or post.shape != (B, T, S + 1):
+        raise RuntimeError(f"{name}: dloss {tuple(dloss.shape)}, raw_loss {tuple(raw.shape)}, stats "
+                           f"{tuple(stats.shape)}, posteriors {tuple(post.shape)} beside logits {(B, T, V)} and "
+                           f"targets {(B, S)}")
+    if any(t.dtype != torch.float32 or not t.is_contiguous() for t in (raw, stats, post)):
+        raise RuntimeError(f"{name}: raw_loss, stats and posteriors must be the fp32 outputs of granite::ctc_loss")
+    dev = logits.device
+    dx = torch.empty((B, T, V), dtype=logits.dtype, device=dev)
+    with _on(dev):
+        x, sb, st, (tg, il, tl) = _ctc_operands(logits, targets, input_lengths, target_lengths)
+        d = dloss.to(torch.float32).contiguous()
+        _lib.call("gsn_ctc_loss_bwd", d.data_ptr(), x.data_ptr(), sb, st, tg.data_ptr(), il.data_ptr(), tl.data_ptr(),
+                  B, T, V, S, blank, int(zero_infinity), _TYPES[x.dtype], raw.data_ptr(), stats.data_ptr(),
+                  post.data_ptr(), dx.data_ptr(), _stream(dev))
+    return dx
+
+
+@torch.library.custom_op("granite::ctc_loss", mutates_args=(), device_types="cuda")
+def ctc_loss_op(logits: torch.Tensor, targets: torch.Tensor, input_lengths: torch.Tensor,
+                target_lengths: torch.Tensor, blank: int, zero_infinity: bool
+                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(loss [B], and what the gradient needs: raw_loss [B], stats [B, T, 2], posteriors [B, T, S + 1]), all fp32."""
+    return _ctc_loss(logits, targets, input_lengths, target_lengths, blank, zero_infinity, True)
+
+
+@ctc_loss_op.register_fake
+def _(logits, targets, input_lengths, target_lengths, blank, zero_infinity):
+    B, T, _ = logits.shape
+    f = dict(dtype=torch.float32)
+    return (logits.new_empty((B,), **f), logits.new_empty((B,), **f), logits.new_empty((B, T, 2), **f),
+            logits.new_empty((B, T, targets.shape[1] + 1), **f))
+
+
+@torch.library.custom_op("granite::ctc_loss_backward", mutates_args=(), device_types="cuda")
+def ctc_loss_backward_op(dloss: torch.Tensor, logits: torch.Tensor, targets: torch.Tensor,
+                         input_lengths: torch.Tensor, target_lengths: torch.Tensor, raw_loss: torch.Tensor,
+                         stats: torch.Tensor, posteriors: torch.Tensor, blank: int,
+                         zero_infinity: bool) -> torch.Tensor:
+    """The gradient of granite::ctc_loss's logits for the gradient dloss [B] of its loss."""
+    return _ctc_loss_backward(dloss, logits, targets, input_lengths, target_lengths, raw_loss, stats, posteriors,
+                              blank, zero_infinity)
+
+
+@ctc_loss_backward_op.register_fake
+def _(dloss, logits, targets, input_lengths, target_lengths, raw_loss, stats, posteriors, blank, zero_infinity):
+    return torch.empty_like(logits, memory_format=torch.contiguous_format)
+
+
+def _ctc_loss_setup(ctx, inputs, output):
+    logits, targets, input_lengths, target_lengths, ctx.blank, ctx.zero_infinity = inputs
+    _, raw, stats, post = output
+    ctx.save_for_backward(logits, targets, input_lengths, target_lengths, raw, stats, post)
+    ctx.set_materialize_grads(False)
+
+
+def _ctc_loss_grad(ctx, dloss, *_):
+    dx = None
+    if dloss is not None:
+        dx = torch.ops.granite.ctc_loss_backward(dloss, *ctx.saved_tensors, ctx.blank, ctx.zero_infinity)
+    return dx, None, None, None, None, None
+
+
+ctc_loss_op.register_autograd(_ctc_loss_grad, setup_context=_ctc_loss_setup)
+
+
+def ctc_loss(logits: torch.Tensor, targets: torch.Tensor, input_lengths: torch.Tensor, target_lengths: torch.Tensor,
+             blank: int = 0, zero_infinity: bool = False) -> torch.Tensor:
+    """CTC loss [B] (fp32, one value an utterance, no reduction) of logits [B, T, V], any strides with V innermost, for
+    targets int [B, S] with input_lengths and target_lengths int [B]; the softmax is part of it.  Differentiable in the
+    logits.  An utterance without an alignment has the loss inf and a NaN gradient, or 0 and 0 with zero_infinity."""
+    if _recorded(logits):
+        return torch.ops.granite.ctc_loss(logits, targets, input_lengths, target_lengths, blank, zero_infinity)[0]
+    return _ctc_loss(logits, targets, input_lengths, target_lengths, blank, zero_infinity, False)[0]

@@ -346,6 +346,78 @@ int gsn_bpe_head_ctc_bf16(const void* pooled, const int32_t* pooled_lengths, con
                           int V, int blank_id, int32_t* ids, int32_t* tokens, int32_t* counts, int B, int Pp, int D,
                           void* workspace, size_t workspace_bytes, gsn_stream_t stream);
 
+/* ---- fine-tuning: LayerNorm with its backward pass, dropout with a residual ------------------------------------
+ * No counterpart in the reference, which only runs inference; the formulas are those of the block's norms
+ * (models/granite_speech_nar/conformer.py:199, :209) and residual steps (:205-208).  Rows of D elements of `dtype`,
+ * M of them (M < 2^31; with lengths, M / T utterances of T frames); inputs have row strides in elements, outputs are
+ * dense and do not overlap inputs.  Rows aligned to 16 bytes with D % 8 == 0 move in 16-byte words, others element by
+ * element.  weight, bias and their gradients are of `param_dtype`: GSN_FP32 or dtype.  D <= 8192 where a norm is
+ * formed.  All arithmetic is fp32 and no sum depends on the order of arrival: results repeat bit for bit.
+ * Padding frames (t >= lengths[b]): x, h and dy are not read, y and dx are 0, nothing joins dweight and dbias, and
+ * the residual path passes (h = residual, dresidual = dh; without a residual, out = 0).
+ *
+ * gsn_layer_norm_fwd: y = (x - m) / sqrt(v + eps) * weight + bias.
+ * gsn_layer_norm_bwd: dx, dweight, dbias (both written, also for M == 0); the row statistics are formed again from x.
+ * gsn_dropout_add: out = residual + (kept ? factor * x : 0), residual may be NULL (none).  The gradient of x is the
+ *   same call on dout without a residual, the residual's is dout.
+ * gsn_dropout_add_layer_norm_fwd: h as gsn_dropout_add, y = LayerNorm(h) of the fp32 sum before h is rounded.
+ * gsn_dropout_add_layer_norm_bwd: from the stored h; dresidual = dh + LayerNorm's gradient (dh may be NULL: none),
+ *   dx = dropout's gradient of that.
+ * The mask is never stored: group g = row * ceil(D / 8) + column / 8 of eight columns takes the eight 16-bit halves
+ * (low half first) of Philox4x32-10 with the counter (g low, g high, offset low 32 bits, site) and the key seed, where
+ * rng is the device's int64[2] (seed, offset), read when the kernel runs; an element is kept where its number is at
+ * least round(65536 p).  factor = scale * 65536 / (65536 - round(65536 p)), or 0 where everything is dropped.
+ * Workspace: gsn_layer_norm_bwd_workspace_bytes(M, D) bytes on the current device, 16-byte aligned. */
+enum { GSN_BF16 = 0, GSN_FP16 = 1, GSN_FP32 = 2 };
+
+int gsn_layer_norm_fwd(const void* x, int64_t ld_x, const void* weight, const void* bias, void* y, int64_t M, int D,
+                       float eps, int dtype, int param_dtype, const int32_t* lengths, int T, gsn_stream_t stream);
+
+size_t gsn_layer_norm_bwd_workspace_bytes(int64_t M, int D);
+
+int gsn_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const void* weight, void* dx,
+                       void* dweight, void* dbias, int64_t M, int D, float eps, int dtype, int param_dtype,
+                       const int32_t* lengths, int T, void* workspace, size_t workspace_bytes, gsn_stream_t stream);
+
+int gsn_dropout_add(const void* x, int64_t ld_x, const void* residual, int64_t ld_res, void* out, int64_t M, int D,
+                    int dtype, const int64_t* rng, uint32_t site, double p, double scale, const int32_t* lengths, int T,
+                    gsn_stream_t stream);
+
+int gsn_dropout_add_layer_norm_fwd(const void* x, int64_t ld_x, const void* residual, int64_t ld_res,
+                                   const void* weight, const void* bias, void* y, void* h, int64_t M, int D, float eps,
+                                   int dtype, int param_dtype, const int64_t* rng, uint32_t site, double p,
+                                   double scale, const int32_t* lengths, int T, gsn_stream_t stream);
+
+int gsn_dropout_add_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* dh, int64_t ld_dh, const void* h,
+                                   int64_t ld_h, const void* weight, void* dx, void* dresidual, void* dweight,
+                                   void* dbias, int64_t M, int D, float eps, int dtype, int param_dtype,
+                                   const int64_t* rng, uint32_t site, double p, double scale, const int32_t* lengths,
+                                   int T, void* workspace, size_t workspace_bytes, gsn_stream_t stream);
+
+/* ---- CTC loss with its gradient ---------------------------------------------------------------------------------
+ * No counterpart in the reference (inference only): the loss that its CTC heads (conformer.py:240-252) are trained
+ * with, from logits [B, T, V] of `dtype` with strides ld_b, ld_t, 1.  targets int32 [B, S], input_lengths and
+ * target_lengths int32 [B] on the device; S <= 2000, T <= 32768.
+ * gsn_ctc_loss_fwd: loss[b] = -log p(targets[b, :target_lengths[b]] | softmax(logits[b, :input_lengths[b]])), inf where
+ *   no alignment exists (0 with zero_infinity), NaN where a length lies outside [0, T] or [0, S], a label outside
+ *   [0, V), or a valid frame holds NaN or +inf.  raw_loss [B], stats [B, T, 2] and posteriors [B, T, S + 1] are fp32
+ *   buffers that the backward pass reads.  A logit more than 15000 below its frame's largest counts as impossible.
+ *   workspace: NULL for the loss alone (the backward pass then has no posteriors and must not be called), else
+ *   gsn_ctc_loss_workspace_bytes(B, T, S) bytes, 16-byte aligned.
+ * gsn_ctc_loss_bwd: dlogits [B, T, V] dense, dloss[b] * d loss[b] / d logits; 0 in padding frames, for utterances
+ *   without an alignment 0 with zero_infinity and NaN without, NaN for the others whose loss is NaN. */
+size_t gsn_ctc_loss_workspace_bytes(int B, int T, int S);
+
+int gsn_ctc_loss_fwd(const void* logits, int64_t ld_b, int64_t ld_t, const int32_t* targets,
+                     const int32_t* input_lengths, const int32_t* target_lengths, int B, int T, int V, int S, int blank,
+                     int zero_infinity, int dtype, float* loss, float* raw_loss, float* stats, float* posteriors,
+                     void* workspace, size_t workspace_bytes, gsn_stream_t stream);
+
+int gsn_ctc_loss_bwd(const float* dloss, const void* logits, int64_t ld_b, int64_t ld_t, const int32_t* targets,
+                     const int32_t* input_lengths, const int32_t* target_lengths, int B, int T, int V, int S, int blank,
+                     int zero_infinity, int dtype, const float* raw_loss, const float* stats, const float* posteriors,
+                     void* dlogits, gsn_stream_t stream);
+
 /* ---- whole module without any allocation ------------------------------------------------------------------
  * No counterpart in the reference.  For callers that cannot allocate device memory where they run the module —
  * a plugin inside a host application that owns the GPU memory budget and its allocator, or a latency-critical
