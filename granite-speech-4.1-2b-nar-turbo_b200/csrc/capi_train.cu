@@ -220,27 +220,30 @@ int gsn_dropout_add_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* dh
   return finish(launch_row_op(a, kRowDropNormGrad, dtype, (cudaStream_t)stream), name);
 }
 
-size_t gsn_ctc_loss_workspace_bytes(int B, int T, int S) {
-  if (B <= 0 || T <= 0 || S < 0) return 0;
-  return (size_t)B * T * (2 * (size_t)S + 1) * sizeof(float2);
+int gsn_ctc_loss_pitch(int S) { return S < 0 ? 0 : ctc_pitch(S); }
+
+size_t gsn_ctc_loss_workspace_bytes(int B, int T, int S, int gradient) {
+  if (B <= 0 || T < 0 || S < 0 || S > kMaxCtcLabels) return 0;
+  size_t n = align256((size_t)B * sizeof(int)) + align256((size_t)B * 4 * ctc_pitch(S) * sizeof(float2));
+  if (gradient) n += (size_t)B * T * ctc_state_pitch(S) * sizeof(uint32_t);
+  return n;
 }
 
 int gsn_ctc_loss_fwd(const void* logits, int64_t ld_b, int64_t ld_t, const int32_t* targets,
                      const int32_t* input_lengths, const int32_t* target_lengths, int B, int T, int V, int S, int blank,
-                     int zero_infinity, int dtype, float* loss, float* raw_loss, float* stats, float* posteriors,
-                     void* workspace, size_t workspace_bytes, gsn_stream_t stream) {
+                     int zero_infinity, int gradient, int dtype, float* loss, float* raw_loss, float* stats,
+                     float* posteriors, int32_t* order, void* workspace, size_t workspace_bytes, gsn_stream_t stream) {
   const char* name = "gsn_ctc_loss_fwd";
   if (int rc = check_ctc(name, B, T, V, S, ld_b, ld_t, blank, dtype)) return rc < 0 ? ok() : rc;
-  if (!input_lengths || !target_lengths || !loss || !raw_loss || (S > 0 && !targets) ||
+  if (!input_lengths || !target_lengths || !loss || !raw_loss || !order || (S > 0 && !targets) ||
       (T > 0 && (!logits || !stats || !posteriors)))
     return fail(GSN_ERR_INVALID_ARG, "%s: null pointer", name);
-  if (!aligned(logits, type_size(dtype)) || !aligned(stats, 8))
-    return fail(GSN_ERR_UNSUPPORTED, "%s: logits must be aligned to their type, stats to 8 bytes", name);
-  if (workspace) {
-    const size_t need = gsn_ctc_loss_workspace_bytes(B, T, S);
-    if (workspace_bytes < need) return fail(GSN_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", name, workspace_bytes, need);
-    if (!aligned(workspace, 16)) return fail(GSN_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", name);
-  }
+  if (!aligned(logits, type_size(dtype)) || !aligned(stats, 8) || !aligned(posteriors, 16))
+    return fail(GSN_ERR_UNSUPPORTED, "%s: logits must be aligned to their type, stats to 8 and posteriors to 16 bytes",
+                name);
+  const size_t need = gsn_ctc_loss_workspace_bytes(B, T, S, gradient);
+  if (workspace_bytes < need) return fail(GSN_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", name, workspace_bytes, need);
+  if (!workspace || !aligned(workspace, 16)) return fail(GSN_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", name);
   CtcArgs a;
   a.logits = logits;
   a.ld_b = ld_b;
@@ -254,23 +257,30 @@ int gsn_ctc_loss_fwd(const void* logits, int64_t ld_b, int64_t ld_t, const int32
   a.S = S;
   a.blank = blank;
   a.zero_infinity = zero_infinity;
+  a.pitch = ctc_pitch(S);
+  a.state_pitch = ctc_state_pitch(S);
   a.loss = loss;
   a.raw_loss = raw_loss;
   a.stats = (float2*)stats;
   a.post = posteriors;
-  a.alpha = (float2*)workspace;
+  a.order = order;
+  char* ws = static_cast<char*>(workspace);
+  a.bad = (int*)ws;
+  ws += align256((size_t)B * sizeof(int));
+  a.exchange = (float2*)ws;
+  if (gradient) a.states = (uint32_t*)(ws + align256((size_t)B * 4 * a.pitch * sizeof(float2)));
   return finish(launch_ctc_loss(a, dtype, (cudaStream_t)stream), name);
 }
 
 int gsn_ctc_loss_bwd(const float* dloss, const void* logits, int64_t ld_b, int64_t ld_t, const int32_t* targets,
                      const int32_t* input_lengths, const int32_t* target_lengths, int B, int T, int V, int S, int blank,
                      int zero_infinity, int dtype, const float* raw_loss, const float* stats, const float* posteriors,
-                     void* dlogits, gsn_stream_t stream) {
+                     const int32_t* order, void* dlogits, gsn_stream_t stream) {
   const char* name = "gsn_ctc_loss_bwd";
   if (int rc = check_ctc(name, B, T, V, S, ld_b, ld_t, blank, dtype)) return rc < 0 ? ok() : rc;
   if (T == 0) return ok();
   if (!dloss || !logits || !input_lengths || !target_lengths || (S > 0 && !targets) || !raw_loss || !stats ||
-      !posteriors || !dlogits)
+      !posteriors || !order || !dlogits)
     return fail(GSN_ERR_INVALID_ARG, "%s: null pointer", name);
   if (!aligned(logits, type_size(dtype)) || !aligned(dlogits, type_size(dtype)) || !aligned(stats, 8))
     return fail(GSN_ERR_UNSUPPORTED, "%s: logits and dlogits must be aligned to their type, stats to 8 bytes", name);
@@ -287,9 +297,11 @@ int gsn_ctc_loss_bwd(const float* dloss, const void* logits, int64_t ld_b, int64
   a.S = S;
   a.blank = blank;
   a.zero_infinity = zero_infinity;
+  a.pitch = ctc_pitch(S);
   a.raw_loss = const_cast<float*>(raw_loss);
   a.stats = (float2*)const_cast<float*>(stats);
   a.post = const_cast<float*>(posteriors);
+  a.order = const_cast<int*>(order);
   a.dloss = dloss;
   a.dlogits = dlogits;
   return finish(launch_ctc_grad(a, dtype, (cudaStream_t)stream), name);

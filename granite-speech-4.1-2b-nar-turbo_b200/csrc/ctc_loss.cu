@@ -6,270 +6,690 @@
 //   Z = alpha_{n-1}(2S) + alpha_{n-1}(2S-1), loss = -log Z, beta the same from the end (without the emission at t)
 //   dlogits[t, v] = dloss (p_t(v) - sum over s with l'_s = v of alpha_t(s) beta_t(s) / Z), 0 for t >= n
 //
-// Three launches: rows (maximum and sum of exponentials of every frame, the emissions of blank and labels), lattice
-// (both chains, the posteriors), gradient.  The emissions are taken against the frame's largest logit, so the frame's
-// normaliser stays out of the chain: it cancels in the posteriors, and the loss adds the normalisers in 64 bits.
+// Three launches: rows (maximum and sum of exponentials of every frame, the emissions of blank and labels; HBM-bound),
+// lattice (both chains, the posteriors; a chain of n dependent steps), gradient (HBM-bound).  The emissions are taken
+// against the frame's largest logit, so the frame's normaliser stays out of the chain: it cancels in the posteriors,
+// and the loss adds the normalisers in 64 bits.
+#include <type_traits>
+
 #include "gsn_kernels.cuh"
 #include "gsn_ptx.cuh"
 
 namespace gsn {
 
-namespace ctc_impl {
+namespace ctc_loss_impl {
 
 using rows_impl::from_f32;
 using rows_impl::to_f32;
 
+constexpr float kLog2e = 1.4426950408889634f;
+
 // ---- numbers of the lattice ------------------------------------------------------------------------------------------
-// m * 2^e with 1 <= m < 2, or zero: sums over paths leave fp32's range within a few dozen frames, and states thousands
-// of octaves below the frame's largest can still carry the whole posterior (a wrong transcript), so every state has
-// its own exponent.  A product or sum costs a rounding of the 24-bit m only, wherever the logarithm lies; the
-// logarithm itself in fp32 would lose 2^-12 at -4000.
-struct Ext {
-  float m;
-  int e;
-};
-constexpr int kZeroExp = -(1 << 30);
-constexpr float kLowest = -15000.f;   // logits further below the frame's largest count as impossible: the exponents of
-                                      // kMaxCtcFrames frames stay within an int
+// A state is m * 2^e with its own integer exponent.  Sums over paths leave fp32's range within a few dozen frames, and
+// a state thousands of octaves below its frame's largest can still carry the whole posterior (a confident model and
+// another transcript), so neither fp32 with a scale a frame nor fp64 holds them; the logarithm in fp32 would lose
+// 2^-12 at -4000, and costs three exponentials and a logarithm a step where this costs none.  m >= 1 always; a zero
+// has e near kZeroExp, so that its terms vanish in any sum.
+//   bounds: a frame's emission is 2^-15871 at the least (kLowest) or impossible, kMaxCtcFrames of them reach -2^28;
+//   kZeroExp = -2^29, e is held at or above it, and no sum of three exponents leaves an int.
+constexpr int kZeroExp = -(1 << 29);
+constexpr int kZeroBelow = -(3 << 27);        // exponents below it are zeros
+constexpr float kLowest = -15870.f;           // log2 of an emission against the frame's largest; below it: impossible
+constexpr float kImpossible = -1048576.f;     // how an impossible emission is stored (log2)
 
-__device__ __forceinline__ Ext ext_zero() { return Ext{0.f, kZeroExp}; }
+// 2^d for d <= 127 (0 from -127 down)
+__device__ __forceinline__ float pow2i(int d) { return __int_as_float(max(d + 127, 0) << 23); }
 
-// 2^d for d <= 0 (0 below the normal range)
-__device__ __forceinline__ float pow2_nonpos(int d) { return __int_as_float((max(d, -127) + 127) << 23); }
-
-__device__ __forceinline__ Ext ext_norm(float m, int e) {
-  if (m <= 0.f) return ext_zero();
-  const int bits = __float_as_int(m);
-  const int k = (bits >> 23) - 127;
-  return Ext{__int_as_float(bits - (k << 23)), e + k};
+// Stored states: 15 bits of exponent against a reference of the frame's warp, 17 bits of mantissa after the leading
+// one.  Four bytes a state keep half the traffic of a pair; the posterior's rounding of 2^-18 lies below what the
+// chain leaves.  The reference is the largest exponent of the warp's states (its neighbours below included) when its
+// frames of one block began: no state can outgrow it within the block.  A state 2^32600 below it counts as zero.
+constexpr int kPackBias = 32600;
+__device__ __forceinline__ uint32_t pack_state(float m, int e, int ref) {
+  const int t = max(e - ref, -kPackBias - 120);                // m < 2^17: the fields never touch
+  return ((__float_as_uint(m) + 0x20u) >> 6) + ((uint32_t)(t + kPackBias) << 17);
 }
+constexpr uint32_t kPackZero = 64u << 17;                      // below: a zero
 
-__device__ __forceinline__ Ext ext_add3(Ext a, Ext b, Ext c) {
-  const int e = max(a.e, max(b.e, c.e));
-  return ext_norm(fmaf(a.m, pow2_nonpos(a.e - e), fmaf(b.m, pow2_nonpos(b.e - e), c.m * pow2_nonpos(c.e - e))), e);
-}
-
-__device__ __forceinline__ Ext ext_mul(Ext a, Ext b) {
-  return a.m == 0.f || b.m == 0.f ? ext_zero() : ext_norm(a.m * b.m, a.e + b.e);
-}
-
-// exp(a) for a <= 0: 2^k * 2^f with k the nearest integer to a / ln 2
-__device__ __forceinline__ Ext ext_exp(float a) {
-  if (!(a >= kLowest)) return ext_zero();
-  constexpr double kLog2e = 1.4426950408889634;
-  constexpr float hi = (float)kLog2e, lo = (float)(kLog2e - (double)hi);
-  const float k = rintf(a * hi);
-  // the fraction a / ln 2 - k from 1 / ln 2 in two parts: one rounding near zero instead of one near |a|
-  const float f = fmaf(a, lo, fmaf(a, hi, -k));
-  return ext_norm(exp2f(f), (int)k);
+// ---- vectors of eight logits at any alignment ------------------------------------------------------------------------
+// Elements before the first 16-byte boundary of a row, which the vector loops leave to single loads.
+template <typename T>
+__device__ __forceinline__ int head_of(const T* row, int V) {
+  const int h = (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T);
+  return h < V ? h : V;
 }
 
 // ---- rows ------------------------------------------------------------------------------------------------------------
-constexpr int kRowThreads = 256;
+struct Online {                                  // running maximum and sum of exponentials against it
+  float top, sum;
+};
 
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) ctc_rows_kernel(CtcArgs a) {
-  const int t = blockIdx.x, b = blockIdx.y;
-  const int n = __ldg(a.input_lengths + b);
-  if (t >= n) return;
-  __shared__ float red[2][kRowThreads / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const T* x = static_cast<const T*>(a.logits) + b * a.ld_b + t * a.ld_t;
-  float top = -INFINITY;
-  for (int v = threadIdx.x; v < a.V; v += kRowThreads) top = fmaxf(top, to_f32(x[v]));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) red[0][warp] = top;
-  __syncthreads();
-  top = red[0][0];
-#pragma unroll
-  for (int i = 1; i < kRowThreads / 32; ++i) top = fmaxf(top, red[0][i]);
-  float s = 0.f;
-  for (int v = threadIdx.x; v < a.V; v += kRowThreads) s += __expf(to_f32(x[v]) - top);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lane == 0) red[1][warp] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    s = 0.f;
-#pragma unroll
-    for (int i = 0; i < kRowThreads / 32; ++i) s += red[1][i];
-    a.stats[(int64_t)b * a.T + t] = make_float2(top, logf(s));
+__device__ __forceinline__ void online_one(Online& o, float x) {
+  if (x > o.top) {
+    o.sum *= ex2_approx((o.top - x) * kLog2e);
+    o.top = x;
   }
-  float* post = a.post + ((int64_t)b * a.T + t) * (a.S + 1);
+  o.sum += x == -INFINITY ? 0.f : ex2_approx((x - o.top) * kLog2e);
+}
+
+__device__ __forceinline__ void online_eight(Online& o, const float (&f)[8]) {
+  float top = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+  if (top > o.top) {
+    o.sum *= ex2_approx((o.top - top) * kLog2e);
+    o.top = top;
+  }
+  top = o.top == -INFINITY ? 0.f : o.top;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) o.sum += ex2_approx((f[k] - top) * kLog2e);
+}
+
+__device__ __forceinline__ Online online_join(Online a, Online b) {
+  const float top = fmaxf(a.top, b.top);
+  if (top == -INFINITY) return Online{top, a.sum + b.sum};     // nothing seen, or NaN
+  return Online{top, a.sum * ex2_approx((a.top - top) * kLog2e) + b.sum * ex2_approx((b.top - top) * kLog2e)};
+}
+
+template <typename T, int THREADS>
+__device__ __forceinline__ Online scan_row(const T* __restrict__ x, int V, int tid) {
+  Online o{-INFINITY, 0.f};
+  const int head = head_of(x, V), vecs = (V - head) / 8;
+  if (tid < head) online_one(o, to_f32(x[tid]));
+  const T* body = x + head;
+  int i = tid;
+  for (; i + 3 * THREADS < vecs; i += 4 * THREADS) {           // four loads under way at once
+    rows_impl::Vec8<T> r[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int q = 0; q < rows_impl::Vec8<T>::Q; ++q)
+        r[u].q[q] = __ldg(reinterpret_cast<const uint4*>(body + (int64_t)(i + u * THREADS) * 8) + q);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float f[8];
+      rows_impl::unpack(r[u], f);
+      online_eight(o, f);
+    }
+  }
+  for (; i < vecs; i += THREADS) {
+    rows_impl::Vec8<T> r;
+#pragma unroll
+    for (int q = 0; q < rows_impl::Vec8<T>::Q; ++q)
+      r.q[q] = __ldg(reinterpret_cast<const uint4*>(body + (int64_t)i * 8) + q);
+    float f[8];
+    rows_impl::unpack(r, f);
+    online_eight(o, f);
+  }
+  for (int v = head + vecs * 8 + tid; v < V; v += THREADS) online_one(o, to_f32(x[v]));
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    const Online other{__shfl_xor_sync(0xffffffffu, o.top, d), __shfl_xor_sync(0xffffffffu, o.sum, d)};
+    o = online_join(o, other);
+  }
+  return o;
+}
+
+// The transcript's places in the order of their labels (the blank's own place, number S, among them), so that the
+// gradient adds the posteriors of one class next to one another; and whether any label lies outside the vocabulary.
+__device__ __forceinline__ void plan_utterance(const CtcArgs& a, int b) {
+  const int len = __ldg(a.target_lengths + b);
+  const bool fits = len >= 0 && len <= a.S;
+  const int* targets = a.targets + (int64_t)b * a.S;
+  int* order = a.order + (int64_t)b * a.pitch;
+  int bad = !fits;
+  const int count = fits ? len + 1 : 0;          // entry len: the blank
+  for (int i = threadIdx.x; i < count; i += blockDim.x) {
+    const int v = i < len ? __ldg(targets + i) : a.blank;
+    bad |= v < 0 || v >= a.V;
+    int rank = 0;
+    for (int j = 0; j < count; ++j) {
+      const int u = j < len ? __ldg(targets + j) : a.blank;
+      rank += u < v || (u == v && j < i);
+    }
+    order[rank] = i < len ? i : a.S;
+  }
+  bad = __syncthreads_or(bad);
+  if (threadIdx.x == 0) a.bad[b] = bad;
+}
+
+// emissions against the frame's largest logit, log2: labels at [0, len), impossible up to S, the blank at S + 1
+template <typename T>
+__device__ __forceinline__ void write_emissions(const CtcArgs& a, const T* x, float top, int64_t frame, int b, int tid,
+                                                int threads) {
+  float* em = a.post + frame * a.pitch;
   const int len = min(max(__ldg(a.target_lengths + b), 0), a.S);
-  for (int i = threadIdx.x; i <= len; i += kRowThreads) {
-    const int v = i == 0 ? a.blank : __ldg(a.targets + (int64_t)b * a.S + i - 1);
-    post[i] = v >= 0 && v < a.V ? to_f32(x[v]) - top : NAN;   // NaN: a label outside the vocabulary
+  for (int i = tid; i < a.S + 2; i += threads) {
+    float e = kImpossible;
+    if (i < len || i == a.S + 1) {
+      const int v = i < len ? __ldg(a.targets + (int64_t)b * a.S + i) : a.blank;
+      if (v >= 0 && v < a.V) e = (to_f32(x[v]) - top) * kLog2e;
+      if (!(e >= kLowest)) e = kImpossible;
+    }
+    em[i] = e;
+  }
+}
+
+constexpr int kRowThreads = 256;
+constexpr int kWarpRowV = 2048;                  // up to it a warp takes a row, beyond it a CTA
+
+// block (frames, utterance); the last block of an utterance plans it
+template <typename T, bool WARP_ROW>
+__global__ void __launch_bounds__(kRowThreads) ctc_rows_kernel(CtcArgs a) {
+  const int b = blockIdx.y;
+  if (blockIdx.x == gridDim.x - 1) return plan_utterance(a, b);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int t = WARP_ROW ? blockIdx.x * (kRowThreads / 32) + warp : blockIdx.x;
+  if (t >= min(__ldg(a.input_lengths + b), a.T)) return;
+  const T* x = static_cast<const T*>(a.logits) + b * a.ld_b + t * a.ld_t;
+  const int64_t frame = (int64_t)b * a.T + t;
+  if (WARP_ROW) {
+    const Online o = scan_row<T, 32>(x, a.V, lane);
+    if (lane == 0) a.stats[frame] = make_float2(o.top, o.sum);
+    write_emissions(a, x, o.top, frame, b, lane, 32);
+  } else {
+    __shared__ Online part[kRowThreads / 32];
+    Online o = scan_row<T, kRowThreads>(x, a.V, threadIdx.x);
+    if (lane == 0) part[warp] = o;
+    __syncthreads();
+    o = part[0];
+#pragma unroll
+    for (int i = 1; i < kRowThreads / 32; ++i) o = online_join(o, part[i]);
+    if (threadIdx.x == 0) a.stats[frame] = make_float2(o.top, o.sum);
+    write_emissions(a, x, o.top, frame, b, threadIdx.x, kRowThreads);
   }
 }
 
 // ---- lattice ---------------------------------------------------------------------------------------------------------
-constexpr int kLatticeThreads = 512;
+// Two CTAs an utterance, a cluster: one walks alpha from the first frame, one beta from the last, the same code on
+// reversed frames and labels.  They meet in the middle (frame h): until there each stores its states, behind it each
+// reads the other's and multiplies, so the posteriors need no second chain and half of each chain is stored.  Beta
+// carries its emission; the posterior takes the other side's sum before its own emission, so none counts twice.
+//
+// A pair (blank i, label i) is the unit; a lane holds NP pairs, a warp 32 NP.  A step needs the label of the pair
+// below: one shuffle within the warp.  Across warps, each keeps the top HL lanes' worth of the warp below it as extra
+// pairs of its own at its low end; H steps reach at most 2 H states, so they are refreshed every H frames, and one
+// barrier serves H steps.  Emissions and the other side's states come H frames at a time by bulk copies.
+template <int NP, int H>
+__host__ __device__ constexpr int halo_lanes() { return (H + NP - 1) / NP; }
 
-__device__ __forceinline__ int state_label(const CtcArgs& a, const int* targets, int s) {
-  return s & 1 ? __ldg(targets + (s >> 1)) : a.blank;
+__host__ __device__ constexpr int lattice_warps(int pairs, int NP, int HL) {
+  return pairs <= 32 * NP ? 1 : 1 + (pairs - 32 * NP + (32 - HL) * NP - 1) / ((32 - HL) * NP);
 }
 
-__global__ void __launch_bounds__(kLatticeThreads) ctc_lattice_kernel(CtcArgs a) {
-  extern __shared__ Ext states[];                  // [2][2 S + 1]
-  __shared__ double sums[kLatticeThreads / 32];
-  __shared__ float blanks[kLatticeThreads / 32];
-  const int b = blockIdx.x, tid = threadIdx.x;
+template <int NP, int H, int NBUF, bool GRAD>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 128 : 544) ctc_lattice_kernel(CtcArgs a, int nw) {
+  constexpr int HL = halo_lanes<NP, H>(), NS = 2 * NP;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t full[NBUF];
+  __shared__ int abort_flag;
+  __shared__ double sums[32];
+  __shared__ float zm[32];
+  __shared__ int ze[32];
+  const int dir = blockIdx.x, b = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int n = __ldg(a.input_lengths + b), len = __ldg(a.target_lengths + b);
-  if (n < 0 || n > a.T || len < 0 || len > a.S) {
-    if (tid == 0) a.raw_loss[b] = a.loss[b] = NAN;
-    return;
-  }
-  if (n == 0) {
-    if (tid == 0) {
-      a.raw_loss[b] = len == 0 ? 0.f : INFINITY;
-      a.loss[b] = len == 0 || a.zero_infinity ? 0.f : INFINITY;
+  const bool bad = __ldg(a.bad + b) || n < 0 || n > a.T;
+  if (bad || n == 0) {                             // both CTAs of the cluster leave here
+    if (dir == 0 && tid == 0) {
+      const float raw = bad ? NAN : len == 0 ? 0.f : INFINITY;
+      a.raw_loss[b] = raw;
+      a.loss[b] = a.zero_infinity && raw == INFINITY ? 0.f : raw;
     }
     return;
   }
-  const int* targets = a.targets + (int64_t)b * a.S;
-  const int L = 2 * len + 1, full = 2 * a.S + 1;
-  float* post = a.post + (int64_t)b * a.T * (a.S + 1);
-  float2* alpha = a.alpha ? a.alpha + (int64_t)b * a.T * full : nullptr;
-  bool bad = false;
-  double norm = 0.0;
-  for (int t = tid; t < n; t += kLatticeThreads) norm += (double)__ldg(&a.stats[(int64_t)b * a.T + t].y);
-  for (int t = 0; t < n; ++t) {
-    Ext* now = states + (t & 1) * L;
-    const Ext* old = states + ((t & 1) ^ 1) * L;
-    for (int s = tid; s < L; s += kLatticeThreads) {
-      const float em = post[(int64_t)t * (a.S + 1) + (s & 1 ? 1 + (s >> 1) : 0)];
-      bad |= em != em;
-      Ext v;
-      if (t == 0) {
-        v = s <= 1 ? Ext{1.f, 0} : ext_zero();
-      } else {
-        const bool skip = (s & 1) && s >= 3 && __ldg(targets + (s >> 1)) != a.blank &&
-                          __ldg(targets + (s >> 1)) != __ldg(targets + (s >> 1) - 1);
-        v = ext_add3(old[s], s >= 1 ? old[s - 1] : ext_zero(), skip ? old[s - 2] : ext_zero());
-      }
-      v = ext_mul(v, ext_exp(em));
-      now[s] = v;
-      if (alpha) alpha[(int64_t)t * full + s] = make_float2(v.m, __int_as_float(v.e));
-    }
-    __syncthreads();
-  }
-  const Ext* last = states + ((n - 1) & 1) * L;
-  const Ext z = ext_add3(last[L - 1], L >= 2 ? last[L - 2] : ext_zero(), ext_zero());
-  bad = __syncthreads_or(bad);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, o);
-  if ((tid & 31) == 0) sums[tid >> 5] = norm;
-  __syncthreads();
+  const int pitch = a.pitch, spitch = a.state_pitch;
+  const int64_t frame0 = (int64_t)b * a.T;
+  // shared memory: emission ring, state ring (GRAD), halo exchange, blanks' partial sums (GRAD)
+  float* em_ring = reinterpret_cast<float*>(smem);
+  uint32_t* st_ring = reinterpret_cast<uint32_t*>(em_ring + NBUF * H * pitch);
+  float2* halo = reinterpret_cast<float2*>(st_ring + (GRAD ? NBUF * H * spitch : 0));   // [2][nw][HL * NS]
+  float* blanks = reinterpret_cast<float*>(halo + 2 * nw * HL * NS);                     // [2][H][nw * 32]
+
   if (tid == 0) {
-    norm = 0.0;
-    for (int i = 0; i < kLatticeThreads / 32; ++i) norm += sums[i];
-    float loss = INFINITY;
-    if (z.m > 0.f) loss = (float)(norm - ((double)z.e + log2((double)z.m)) * 0.6931471805599453);
-    if (bad || norm != norm) loss = NAN;
-    a.raw_loss[b] = loss;
-    a.loss[b] = a.zero_infinity && loss == INFINITY ? 0.f : loss;
+    for (int i = 0; i < NBUF; ++i) mbar_init(&full[i], 1);
+    abort_flag = 0;
+    fence_mbar_init();
   }
-  if (!alpha || z.m == 0.f || bad) return;
-  // beta, without the emission at t; states hold beta times that emission
+  // this lane's pairs: labels, whether a jump from the label below is allowed, where they lie in a frame
+  const int i0 = w * (32 - HL) * NP + lane * NP;
+  const bool own = w == 0 || lane >= HL;
+  const int* targets = a.targets + (int64_t)b * a.S;
+  int slot[NP], pen[NP], ob[NP], ol[NP], rb[NP], rl[NP];
+#pragma unroll
+  for (int j = 0; j < NP; ++j) {
+    const int i = i0 + j;
+    const int li = dir ? len - 1 - i : i;
+    slot[j] = i < len ? li : a.S;
+    pen[j] = kZeroExp;
+    if (i >= 1 && i < len) {
+      const int later = __ldg(targets + (dir ? li + 1 : li)), earlier = __ldg(targets + (dir ? li : li - 1));
+      if (later != a.blank && later != earlier) pen[j] = 0;
+    }
+    // the other side's pairs of this blank and label, and the warps that hold them
+    const int qb = i <= len ? len - i : 0, ql = i < len ? len - 1 - i : 0;
+    ob[j] = 2 * qb;
+    ol[j] = 2 * ql + 1;
+    rb[j] = 2 * (pitch) + (qb < 32 * NP ? 0 : 1 + (qb - 32 * NP) / ((32 - HL) * NP));
+    rl[j] = 2 * (pitch) + (ql < 32 * NP ? 0 : 1 + (ql - 32 * NP) / ((32 - HL) * NP));
+  }
+  float m[NS];
+  int e[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    m[s] = 1.f;
+    e[s] = i0 == 0 && s == 0 ? 0 : kZeroExp;       // one path, before the first frame
+  }
+  // the frames' normalisers
+  double norm = 0.0;
+  if (dir == 0)
+    for (int t = tid; t < n; t += blockDim.x) norm += (double)log2f(__ldg(&a.stats[frame0 + t].y));
   __syncthreads();
-  for (int t = n - 1; t >= 0; --t) {
-    Ext* now = states + (t & 1) * L;
-    const Ext* old = states + ((t & 1) ^ 1) * L;
-    float blank = 0.f;
-    for (int s = tid; s < L; s += kLatticeThreads) {
-      Ext v;
-      if (t == n - 1) {
-        v = s >= L - 2 ? Ext{1.f, 0} : ext_zero();
-      } else {
-        const bool skip = (s & 1) && s + 2 < L && __ldg(targets + (s >> 1) + 1) != a.blank &&
-                          __ldg(targets + (s >> 1)) != __ldg(targets + (s >> 1) + 1);
-        v = ext_add3(old[s], s + 1 < L ? old[s + 1] : ext_zero(), skip ? old[s + 2] : ext_zero());
+
+  const int h = (n + 1) / 2, n1 = dir ? n - h : h;  // this side's frames before the meeting
+  const bool active = i0 - lane * NP <= len;        // a warp beyond the last pair only keeps the barriers
+  int issued = 0, waited = 0, blocks = 0, parity = 0;
+  bool fail = false;
+
+  // frames [k, k + cnt) of this side's order are rows lo, lo + 1, ...
+  auto issue = [&](int k, int cnt, bool states) {
+    const int lo = dir ? n - k - cnt : k, buf = issued % NBUF;
+    const uint32_t be = cnt * pitch * 4, bs = states ? cnt * spitch * 4 : 0;
+    mbar_arrive_expect_tx(&full[buf], be + bs);
+    bulk_load(em_ring + buf * H * pitch, a.post + (frame0 + lo) * pitch, be, &full[buf]);
+    if (states) bulk_load(st_ring + buf * H * spitch, a.states + (frame0 + lo) * spitch, bs, &full[buf]);
+  };
+  auto refresh_halo = [&]() {
+    if (w > 0 && lane < HL) {
+      const float2* src = halo + ((parity ^ 1) * nw + w - 1) * HL * NS + lane * NS;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        m[s] = src[s].x;
+        e[s] = __float_as_int(src[s].y);
       }
-      const int slot = s & 1 ? 1 + (s >> 1) : 0;
-      float* p = post + (int64_t)t * (a.S + 1) + slot;
-      now[s] = ext_mul(v, ext_exp(*p));
-      const float2 al = alpha[(int64_t)t * full + s];
-      const int e = __float_as_int(al.y) + v.e - z.e;
-      float gamma = 0.f;
-      if (al.x != 0.f && v.m != 0.f) gamma = al.x * v.m / z.m * pow2_nonpos(min(e, 0)) * (e > 0 ? exp2f((float)e) : 1.f);
-      if (slot)
-        *p = gamma;
-      else
-        blank += gamma;
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) blank += __shfl_xor_sync(0xffffffffu, blank, o);
-    if ((tid & 31) == 0) blanks[tid >> 5] = blank;
-    __syncthreads();
-    if (tid == 0) {
-      blank = 0.f;
-      for (int i = 0; i < kLatticeThreads / 32; ++i) blank += blanks[i];
-      post[(int64_t)t * (a.S + 1)] = blank;
+    for (int s = 0; s < NS; ++s) {                 // leading ones out of m
+      const int bits = __float_as_int(m[s]), k = (bits >> 23) - 127;
+      m[s] = __int_as_float(bits - (k << 23));
+      e[s] += k;
+    }
+  };
+  auto publish_halo = [&]() {
+    if (lane >= 32 - HL) {
+      float2* dst = halo + (parity * nw + w) * HL * NS + (lane - 32 + HL) * NS;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) dst[s] = make_float2(m[s], __int_as_float(e[s]));
+    }
+  };
+  // sums into every state, without the emission: (pm, pe)
+  auto gather = [&](float (&pm)[NS], int (&pe)[NS]) {
+    float um = __shfl_up_sync(0xffffffffu, m[NS - 1], 1);
+    int ue = __shfl_up_sync(0xffffffffu, e[NS - 1], 1);
+    if (lane == 0) ue = kZeroExp;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      const float bm = m[2 * j], lm = m[2 * j + 1];
+      const int be = e[2 * j], le = e[2 * j + 1], je = ue + pen[j];
+      const int eb = max(be, ue), el = max(max(le, be), je);
+      pe[2 * j] = eb;
+      pm[2 * j] = fmaf(bm, pow2i(be - eb), um * pow2i(ue - eb));
+      pe[2 * j + 1] = el;
+      pm[2 * j + 1] = fmaf(lm, pow2i(le - el), fmaf(bm, pow2i(be - el), um * pow2i(je - el)));
+      um = lm;
+      ue = le;
+    }
+  };
+  // multiplies a sum by an emission 2^x
+  auto emit = [&](float x, float& fm, int& fe) {
+    const float k = x + 12582912.f;                // 1.5 * 2^23: the nearest integer in the low bits
+    const int ki = __float_as_int(k) - 0x4B400000;
+    fm = ex2_approx(x - (k - 12582912.f));
+    fe = x < -524288.f ? kZeroExp : ki;
+  };
+
+  float zinv = 0.f;
+  int zexp = 0;
+  auto walk = [&](int k0, int k1, auto second) {
+    constexpr bool SECOND = decltype(second)::value;
+    const int base = blocks;
+    if (tid == 0)
+      for (int u = 0; u < NBUF; ++u)
+        if (k0 + u * H < k1) {
+          issue(k0 + u * H, min(H, k1 - k0 - u * H), SECOND);
+          ++issued;
+        }
+    for (int k = k0; k < k1 && !fail; k += H) {
+      const int cnt = min(H, k1 - k), buf = blocks % NBUF;
+      const bool ok = mbar_wait_bounded(&full[buf], (blocks / NBUF) & 1, &abort_flag, kStatusTimeoutCtc);
+      if (ok) ++waited;
+      if (ok && active) {
+        refresh_halo();
+        int ref = e[0];
+#pragma unroll
+        for (int s = 1; s < NS; ++s) ref = max(ref, e[s]);
+        ref = __reduce_max_sync(0xffffffffu, ref);
+        const float* em0 = em_ring + buf * H * pitch;
+        const uint32_t* st0 = st_ring + buf * H * spitch;
+        for (int f = 0; f < cnt; ++f) {
+          const int row = dir ? cnt - 1 - f : f;
+          const float* em = em0 + row * pitch;
+          const int64_t frame = frame0 + (dir ? n - 1 - k - f : k + f);
+          float pm[NS];
+          int pe[NS];
+          gather(pm, pe);
+          if constexpr (SECOND) {
+            const uint32_t* st = st0 + row * spitch;
+            float* post = a.post + frame * pitch;
+            float blank = 0.f;
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+              const uint32_t vb = st[ob[j]], vl = st[ol[j]];
+              const int eb = (int)(vb >> 17) + (int)st[rb[j]] + pe[2 * j] - zexp;
+              const int el = (int)(vl >> 17) + (int)st[rl[j]] + pe[2 * j + 1] - zexp;
+              const float mb = __uint_as_float(((vb & 0x1FFFFu) << 6) | 0x3F800000u);
+              const float ml = __uint_as_float(((vl & 0x1FFFFu) << 6) | 0x3F800000u);
+              const float gb = vb < kPackZero ? 0.f : pm[2 * j] * mb * zinv * pow2i(eb);
+              const float gl = vl < kPackZero ? 0.f : pm[2 * j + 1] * ml * zinv * pow2i(el);
+              if (own && i0 + j <= len) blank += gb;
+              if (own && i0 + j < len) post[slot[j]] = gl;
+            }
+            blanks[(parity * H + f) * nw * 32 + tid] = blank;
+          }
+          float xm;
+          int xe;
+          emit(em[a.S + 1], xm, xe);
+#pragma unroll
+          for (int j = 0; j < NP; ++j) {
+            m[2 * j] = pm[2 * j] * xm;
+            e[2 * j] = max(pe[2 * j] + xe, kZeroExp);
+          }
+#pragma unroll
+          for (int j = 0; j < NP; ++j) {
+            emit(em[slot[j]], xm, xe);
+            m[2 * j + 1] = pm[2 * j + 1] * xm;
+            e[2 * j + 1] = max(pe[2 * j + 1] + xe, kZeroExp);
+          }
+          if constexpr (GRAD && !SECOND) {
+            uint32_t* dst = a.states + frame * spitch;
+            if (own)
+#pragma unroll
+              for (int j = 0; j < NP; ++j)
+                if (i0 + j <= len)
+                  *reinterpret_cast<uint2*>(dst + 2 * (i0 + j)) =
+                      make_uint2(pack_state(m[2 * j], e[2 * j], ref), pack_state(m[2 * j + 1], e[2 * j + 1], ref));
+            if (lane == 0) dst[2 * pitch + w] = (uint32_t)(ref - 127 - kPackBias);
+          }
+        }
+        publish_halo();
+      }
+      fail = __syncthreads_or(!ok);
+      if constexpr (SECOND) {
+        const int used = min(nw, lattice_warps(len + 1, NP, HL));
+        for (int f = w; f < cnt && !fail; f += nw) {
+          float s = 0.f;
+          for (int i = 0; i < used; ++i) s += blanks[(parity * H + f) * nw * 32 + i * 32 + lane];
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+          if (lane == 0) a.post[(frame0 + (dir ? n - 1 - k - f : k + f)) * pitch + a.S + 1] = s;
+        }
+      }
+      parity ^= 1;
+      ++blocks;
+      const int next = k0 + (blocks - base - 1 + NBUF) * H;
+      if (tid == 0 && next < k1 && !fail) {
+        issue(next, min(H, k1 - next), SECOND);
+        ++issued;
+      }
+    }
+  };
+  auto drain = [&]() {                             // after a wait that ran out: the copies under way land first
+    if (tid == 0)
+      for (int i = waited; i < issued; ++i)
+        mbar_wait_bounded(&full[i % NBUF], (i / NBUF) & 1, nullptr, kStatusTimeoutCtc);
+  };
+
+  publish_halo();
+  parity ^= 1;
+  __syncthreads();
+  walk(0, n1, std::false_type{});
+
+  // the meeting: Z = sum over the states of this side's sum into them times the other side's value
+  float2* mine = a.exchange + ((int64_t)b * 2 + dir) * 2 * pitch;
+  const float2* theirs = a.exchange + ((int64_t)b * 2 + (dir ^ 1)) * 2 * pitch;
+  if (active && own)
+#pragma unroll
+    for (int j = 0; j < NP; ++j)
+      if (i0 + j <= len) {
+        mine[2 * (i0 + j)] = make_float2(m[2 * j], __int_as_float(e[2 * j]));
+        mine[2 * (i0 + j) + 1] = make_float2(m[2 * j + 1], __int_as_float(e[2 * j + 1]));
+      }
+  // the states were stored by plain stores and are fetched by bulk copies of the other CTA
+  asm volatile("fence.proxy.async;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("fence.proxy.async;" ::: "memory");
+  if (fail) return drain();
+  {
+    float zmax_m[NS];
+    int zmax_e[NS];
+    int top = 2 * kZeroExp;
+    float total = 0.f;
+    if (active) {
+      refresh_halo();
+      gather(zmax_m, zmax_e);
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        const bool hb = own && i0 + j <= len, hl = own && i0 + j < len;
+        const float2 vb = hb ? __ldcg(theirs + ob[j]) : make_float2(1.f, __int_as_float(kZeroExp));
+        const float2 vl = hl ? __ldcg(theirs + ol[j]) : make_float2(1.f, __int_as_float(kZeroExp));
+        zmax_m[2 * j] *= vb.x;
+        zmax_e[2 * j] += __float_as_int(vb.y);
+        zmax_m[2 * j + 1] *= vl.x;
+        zmax_e[2 * j + 1] += __float_as_int(vl.y);
+      }
+#pragma unroll
+      for (int s = 0; s < NS; ++s) top = max(top, zmax_e[s]);
+      top = __reduce_max_sync(0xffffffffu, top);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) total = fmaf(zmax_m[s], pow2i(zmax_e[s] - top), total);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, d);
+    if (lane == 0) {
+      zm[w] = total;
+      ze[w] = top;
+      sums[w] = norm;
     }
     __syncthreads();
+    top = ze[0];
+    for (int i = 1; i < nw; ++i) top = max(top, ze[i]);
+    total = 0.f;
+    for (int i = 0; i < nw; ++i) total += zm[i] * pow2i(ze[i] - top);
+    const bool exists = top > kZeroBelow;
+    if (dir == 0 && tid == 0) {
+      norm = 0.0;
+      for (int i = 0; i < nw; ++i) norm += sums[i];
+      float raw = INFINITY;
+      if (exists) raw = (float)((norm - (double)top - log2((double)total)) * 0.6931471805599453);
+      if (!(norm > -INFINITY)) raw = NAN;          // a frame of NaN, +inf or nothing but -inf
+      a.raw_loss[b] = raw;
+      a.loss[b] = a.zero_infinity && raw == INFINITY ? 0.f : raw;
+    }
+    if (!GRAD || !exists) return;
+    const int bits = __float_as_int(total), k = (bits >> 23) - 127;
+    zinv = 1.f / __int_as_float(bits - (k << 23));
+    zexp = top + k;
+  }
+  if constexpr (GRAD) {
+    walk(n1, n, std::true_type{});
+    if (fail) drain();
   }
 }
 
 // ---- gradient --------------------------------------------------------------------------------------------------------
-template <typename T>
+// A frame's d p everywhere, then d (p - posterior) over the classes of the transcript.  `tid` of `threads` work on the
+// frame; `sync` orders the two.
+template <typename T, int THREADS, typename Sync>
+__device__ __forceinline__ void grad_row(const CtcArgs& a, const T* __restrict__ x, T* __restrict__ g, int64_t frame,
+                                         int b, int tid, Sync sync) {
+  const float2 st = a.stats[frame];
+  const float d = __ldg(a.dloss + b), f = d / st.y;
+  const int V = a.V;
+  auto value = [&](float v) { return f * ex2_approx((v - st.x) * kLog2e); };
+  int head = head_of(g, V), vecs = (V - head) / 8;
+  if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(g)) & 15) != 0) {
+    head = V;                                      // another alignment than the gradient's: element by element
+    vecs = 0;
+  }
+  for (int v = tid; v < head; v += THREADS) g[v] = from_f32<T>(value(to_f32(x[v])));
+  for (int i = tid; i < vecs; i += THREADS) {
+    rows_impl::Vec8<T> r;
+#pragma unroll
+    for (int q = 0; q < rows_impl::Vec8<T>::Q; ++q)
+      r.q[q] = __ldg(reinterpret_cast<const uint4*>(x + head + (int64_t)i * 8) + q);
+    float e[8];
+    rows_impl::unpack(r, e);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) e[k] = value(e[k]);
+    rows_impl::pack(e, r);
+#pragma unroll
+    for (int q = 0; q < rows_impl::Vec8<T>::Q; ++q)
+      *(reinterpret_cast<uint4*>(g + head + (int64_t)i * 8) + q) = r.q[q];
+  }
+  for (int v = head + vecs * 8 + tid; v < V; v += THREADS) g[v] = from_f32<T>(value(to_f32(x[v])));
+  sync();
+  if (tid >= 32) return;
+  // the posteriors in the order of their classes: a running sum within each class, its last place writes
+  const float* post = a.post + frame * a.pitch;
+  const int* order = a.order + (int64_t)b * a.pitch;
+  const int* targets = a.targets + (int64_t)b * a.S;
+  const int count = __ldg(a.target_lengths + b) + 1;
+  float carry = 0.f;
+  int carry_v = -1;
+  for (int q0 = 0; q0 < count; q0 += 32) {
+    const int q = q0 + tid;
+    int v = -2;
+    float s = 0.f;
+    if (q < count) {
+      const int i = __ldg(order + q);
+      v = i == a.S ? a.blank : __ldg(targets + i);
+      s = post[i == a.S ? a.S + 1 : i];
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float us = __shfl_up_sync(0xffffffffu, s, o);
+      const int uv = __shfl_up_sync(0xffffffffu, v, o);
+      if (tid >= o && uv == v) s += us;            // sorted: equal o below means one class in between
+    }
+    if (v == carry_v) s += carry;
+    const int above = __shfl_down_sync(0xffffffffu, v, 1);
+    int next = above;
+    if (tid == 31) {
+      next = -3;
+      if (q + 1 < count) {
+        const int i = __ldg(order + q + 1);
+        next = i == a.S ? a.blank : __ldg(targets + i);
+      }
+    }
+    if (v >= 0 && next != v) g[v] = from_f32<T>(value(to_f32(x[v])) - d * s);
+    carry = __shfl_sync(0xffffffffu, s, 31);
+    carry_v = __shfl_sync(0xffffffffu, v, 31);
+  }
+}
+
+template <typename T, int THREADS>
+__device__ __forceinline__ void fill_row(T* __restrict__ g, int V, float value, int tid) {
+  const int head = head_of(g, V), vecs = (V - head) / 8;
+  if (tid < head) g[tid] = from_f32<T>(value);
+  const float f[8] = {value, value, value, value, value, value, value, value};
+  rows_impl::Vec8<T> r;
+  rows_impl::pack(f, r);
+  for (int i = tid; i < vecs; i += THREADS)
+#pragma unroll
+    for (int q = 0; q < rows_impl::Vec8<T>::Q; ++q)
+      *(reinterpret_cast<uint4*>(g + head + (int64_t)i * 8) + q) = r.q[q];
+  for (int v = head + vecs * 8 + tid; v < V; v += THREADS) g[v] = from_f32<T>(value);
+}
+
+template <typename T, bool WARP_ROW>
 __global__ void __launch_bounds__(kRowThreads) ctc_grad_kernel(CtcArgs a) {
-  const int t = blockIdx.x, b = blockIdx.y;
-  T* g = static_cast<T*>(a.dlogits) + ((int64_t)b * a.T + t) * a.V;
-  const int n = __ldg(a.input_lengths + b), len = __ldg(a.target_lengths + b);
+  constexpr int THREADS = WARP_ROW ? 32 : kRowThreads;
+  const int b = blockIdx.y;
+  const int t = WARP_ROW ? blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5) : blockIdx.x;
+  if (t >= a.T) return;
+  const int tid = WARP_ROW ? threadIdx.x & 31 : threadIdx.x;
+  const int64_t frame = (int64_t)b * a.T + t;
+  T* g = static_cast<T*>(a.dlogits) + frame * a.V;
+  const int n = __ldg(a.input_lengths + b);
   const float raw = __ldg(a.raw_loss + b);
   const bool nan = raw != raw || (raw == INFINITY && !a.zero_infinity);
   const bool padding = t >= n && n >= 0 && n <= a.T;
-  if (padding || nan || raw == INFINITY) {
-    const float f = !padding && nan ? NAN : 0.f;
-    for (int v = threadIdx.x; v < a.V; v += kRowThreads) g[v] = from_f32<T>(f);
-    return;
-  }
+  if (padding || nan || raw == INFINITY) return fill_row<T, THREADS>(g, a.V, !padding && nan ? NAN : 0.f, tid);
   const T* x = static_cast<const T*>(a.logits) + b * a.ld_b + t * a.ld_t;
-  const float2 st = a.stats[(int64_t)b * a.T + t];
-  const float d = __ldg(a.dloss + b);
-  for (int v = threadIdx.x; v < a.V; v += kRowThreads)
-    g[v] = from_f32<T>(d * __expf(to_f32(x[v]) - st.x - st.y));
-  __syncthreads();
-  // the labels' posteriors, each label by the thread of its first place in the transcript
-  const float* post = a.post + ((int64_t)b * a.T + t) * (a.S + 1);
-  const int* targets = a.targets + (int64_t)b * a.S;
-  for (int i = threadIdx.x; i <= len; i += kRowThreads) {
-    const int v = i == 0 ? a.blank : __ldg(targets + i - 1);
-    float s = post[i];
-    bool first = i == 0 || v != a.blank;
-    for (int j = 1; j < i && first; ++j) first = __ldg(targets + j - 1) != v;
-    if (!first) continue;
-    for (int j = i + 1; j <= len; ++j)
-      if (__ldg(targets + j - 1) == v) s += post[j];
-    g[v] = from_f32<T>(d * (__expf(to_f32(x[v]) - st.x - st.y) - s));
-  }
+  grad_row<T, THREADS>(a, x, g, frame, b, tid, [] {
+    if (WARP_ROW)
+      __syncwarp();
+    else
+      __syncthreads();
+  });
+}
+
+template <int NP, int H, int NBUF, bool GRAD>
+int launch_lattice(const CtcArgs& a, cudaStream_t stream) {
+  constexpr int HL = halo_lanes<NP, H>(), NS = 2 * NP;
+  const int nw = lattice_warps(a.S + 1, NP, HL);
+  const size_t smem = (size_t)NBUF * H * a.pitch * 4 + (GRAD ? (size_t)NBUF * H * a.state_pitch * 4 : 0) +
+                      (size_t)2 * nw * HL * NS * sizeof(float2) + (GRAD ? (size_t)2 * H * nw * 32 * 4 : 0);
+  auto* kernel = ctc_lattice_kernel<NP, H, NBUF, GRAD>;
+  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
+  kernel<<<dim3(2, a.B), nw * 32, smem, stream>>>(a, nw);
+  return (int)cudaGetLastError();
+}
+
+// Pairs a lane: as few as four warps hold (one a scheduler of the SM, so that a step issues in the least time); beyond
+// those, four pairs a lane and more warps.
+template <bool GRAD>
+int launch_lattice_for(const CtcArgs& a, cudaStream_t stream) {
+  const int pairs = a.S + 1;
+  if (lattice_warps(pairs, 1, halo_lanes<1, 8>()) <= 4) return launch_lattice<1, 8, 3, GRAD>(a, stream);
+  if (lattice_warps(pairs, 2, halo_lanes<2, 8>()) <= 4) return launch_lattice<2, 8, 3, GRAD>(a, stream);
+  if (lattice_warps(pairs, 3, halo_lanes<3, 8>()) <= 4) return launch_lattice<3, 8, 3, GRAD>(a, stream);
+  return launch_lattice<4, 4, 2, GRAD>(a, stream);
+}
+
+// utterances [b0, b0 + 65535): a grid's second extent
+CtcArgs batch_part(const CtcArgs& a, int b0, int size) {
+  CtcArgs c = a;
+  c.B = a.B - b0 < 65535 ? a.B - b0 : 65535;
+  const int64_t frames = (int64_t)b0 * a.T;
+  c.logits = static_cast<const char*>(a.logits) + b0 * a.ld_b * size;
+  c.targets += (int64_t)b0 * a.S;
+  c.input_lengths += b0;
+  c.target_lengths += b0;
+  c.stats += frames;
+  c.post += frames * a.pitch;
+  c.order += (int64_t)b0 * a.pitch;
+  c.raw_loss += b0;
+  if (c.loss) c.loss += b0;
+  if (c.bad) c.bad += b0;
+  if (c.exchange) c.exchange += (int64_t)b0 * 4 * a.pitch;
+  if (c.states) c.states += frames * a.state_pitch;
+  if (c.dloss) c.dloss += b0;
+  if (c.dlogits) c.dlogits = static_cast<char*>(a.dlogits) + frames * a.V * size;
+  return c;
 }
 
 template <typename T>
 int launch_loss(const CtcArgs& a, cudaStream_t stream) {
   for (int b0 = 0; b0 < a.B; b0 += 65535) {
-    CtcArgs c = a;
-    c.B = a.B - b0 < 65535 ? a.B - b0 : 65535;
-    const int64_t frames = (int64_t)b0 * a.T;
-    c.logits = static_cast<const T*>(a.logits) + b0 * a.ld_b;
-    c.targets += (int64_t)b0 * a.S;
-    c.input_lengths += b0;
-    c.target_lengths += b0;
-    c.stats += frames;
-    c.post += frames * (a.S + 1);
-    c.raw_loss += b0;
-    c.loss += b0;
-    if (c.alpha) c.alpha += frames * (2 * a.S + 1);
-    if (a.T > 0) ctc_rows_kernel<T><<<dim3(a.T, c.B), kRowThreads, 0, stream>>>(c);
+    const CtcArgs c = batch_part(a, b0, sizeof(T));
+    constexpr int per = kRowThreads / 32;
+    if (a.V <= kWarpRowV)
+      ctc_rows_kernel<T, true><<<dim3((a.T + per - 1) / per + 1, c.B), kRowThreads, 0, stream>>>(c);
+    else
+      ctc_rows_kernel<T, false><<<dim3(a.T + 1, c.B), kRowThreads, 0, stream>>>(c);
     if (cudaError_t e = cudaGetLastError()) return (int)e;
-    const size_t smem = (size_t)2 * (2 * a.S + 1) * sizeof(Ext);
-    if (smem > 48 * 1024)
-      if (cudaError_t e = cudaFuncSetAttribute(ctc_lattice_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem))
-        return (int)e;
-    ctc_lattice_kernel<<<c.B, kLatticeThreads, smem, stream>>>(c);
-    if (cudaError_t e = cudaGetLastError()) return (int)e;
+    if (int rc = c.states ? launch_lattice_for<true>(c, stream) : launch_lattice_for<false>(c, stream)) return rc;
   }
   return 0;
 }
@@ -277,28 +697,30 @@ int launch_loss(const CtcArgs& a, cudaStream_t stream) {
 template <typename T>
 int launch_grad(const CtcArgs& a, cudaStream_t stream) {
   for (int b0 = 0; b0 < a.B; b0 += 65535) {
-    CtcArgs c = a;
-    c.B = a.B - b0 < 65535 ? a.B - b0 : 65535;
-    const int64_t frames = (int64_t)b0 * a.T;
-    c.logits = static_cast<const T*>(a.logits) + b0 * a.ld_b;
-    c.targets += (int64_t)b0 * a.S;
-    c.input_lengths += b0;
-    c.target_lengths += b0;
-    c.stats += frames;
-    c.post += frames * (a.S + 1);
-    c.raw_loss += b0;
-    c.dloss += b0;
-    c.dlogits = static_cast<T*>(a.dlogits) + frames * a.V;
-    ctc_grad_kernel<T><<<dim3(a.T, c.B), kRowThreads, 0, stream>>>(c);
+    const CtcArgs c = batch_part(a, b0, sizeof(T));
+    constexpr int per = kRowThreads / 32;
+    if (a.V <= kWarpRowV)
+      ctc_grad_kernel<T, true><<<dim3((a.T + per - 1) / per, c.B), kRowThreads, 0, stream>>>(c);
+    else
+      ctc_grad_kernel<T, false><<<dim3(a.T, c.B), kRowThreads, 0, stream>>>(c);
     if (cudaError_t e = cudaGetLastError()) return (int)e;
   }
   return 0;
 }
 
-}  // namespace ctc_impl
+}  // namespace ctc_loss_impl
+
+int ctc_pitch(int S) { return (S + 2 + 3) / 4 * 4; }
+
+int ctc_state_pitch(int S) {
+  using namespace ctc_loss_impl;
+  // the states of S + 1 pairs, and a reference for each warp (at most as many as one pair a lane needs)
+  const int warps = lattice_warps(S + 1, 1, halo_lanes<1, 8>());
+  return 2 * ctc_pitch(S) + (warps + 3) / 4 * 4;
+}
 
 int launch_ctc_loss(const CtcArgs& args, int dtype, cudaStream_t stream) {
-  using namespace ctc_impl;
+  using namespace ctc_loss_impl;
   switch (dtype) {
     case 0: return launch_loss<__nv_bfloat16>(args, stream);
     case 1: return launch_loss<__half>(args, stream);
@@ -307,7 +729,7 @@ int launch_ctc_loss(const CtcArgs& args, int dtype, cudaStream_t stream) {
 }
 
 int launch_ctc_grad(const CtcArgs& args, int dtype, cudaStream_t stream) {
-  using namespace ctc_impl;
+  using namespace ctc_loss_impl;
   switch (dtype) {
     case 0: return launch_grad<__nv_bfloat16>(args, stream);
     case 1: return launch_grad<__half>(args, stream);

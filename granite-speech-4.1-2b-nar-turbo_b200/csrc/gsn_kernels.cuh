@@ -183,7 +183,7 @@ int launch_row_op(const RowArgs& args, int op, int dtype, cudaStream_t stream);
 
 // ---- CTC loss and its gradient (ctc_loss.cu) ---------------------------------------------------------------------
 constexpr int kMaxCtcLabels = 2000;
-constexpr int kMaxCtcFrames = 32768;
+constexpr int kMaxCtcFrames = 16384;
 struct CtcArgs {
   const void* logits = nullptr;  // [B, T, V], strides ld_b, ld_t, 1
   int64_t ld_b = 0, ld_t = 0;
@@ -192,14 +192,21 @@ struct CtcArgs {
   const int* target_lengths = nullptr;
   int B = 0, T = 0, V = 0, S = 0, blank = 0;
   int zero_infinity = 0;
-  float2* stats = nullptr;       // [B, T] (largest logit, log of the sum of exp(logit - largest))
-  float* post = nullptr;         // [B, T, S + 1]: logit - largest of blank and labels, then their posteriors
+  int pitch = 0;                 // ctc_pitch(S)
+  int state_pitch = 0;           // ctc_state_pitch(S)
+  float2* stats = nullptr;       // [B, T] (largest logit, sum of exp(logit - largest))
+  float* post = nullptr;         // [B, T, pitch]: emissions, then posteriors, of the labels; blank's at S + 1
+  int* order = nullptr;          // [B, pitch] the transcript's places in the order of their labels
   float* raw_loss = nullptr;     // [B] loss, inf where no path exists, NaN for bad input
   float* loss = nullptr;         // [B] loss with zero_infinity applied
-  float2* alpha = nullptr;       // workspace [B, T, 2 S + 1], or null: no posteriors wanted
+  int* bad = nullptr;            // workspace [B]: a length or label out of range
+  float2* exchange = nullptr;    // workspace [B, 2, 2 pitch]: both sides' states where they meet
+  uint32_t* states = nullptr;    // workspace [B, T, state_pitch], or null: no posteriors wanted
   const float* dloss = nullptr;  // [B]
   void* dlogits = nullptr;       // [B, T, V] dense
 };
+int ctc_pitch(int S);
+int ctc_state_pitch(int S);
 int launch_ctc_loss(const CtcArgs& args, int dtype, cudaStream_t stream);
 int launch_ctc_grad(const CtcArgs& args, int dtype, cudaStream_t stream);
 

@@ -17,6 +17,7 @@ enum : int {
   kStatusTimeoutMma = 0x102,        // MMA issuer gave up waiting for a loaded stage / a drained accumulator
   kStatusTimeoutEpilogue = 0x103,   // epilogue gave up waiting for a finished accumulator
   kStatusTimeoutDw = 0x104,         // depthwise kernel gave up waiting for its TMA tile
+  kStatusTimeoutCtc = 0x105,        // CTC lattice gave up waiting for its frames' copy
   kStatusTimeoutSelftest = 0x1FF,   // the deliberate self-test wait ran out (expected in that test)
 };
 
@@ -132,6 +133,13 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
                ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(src)), "r"(c0), "r"(c1)
+               : "memory");
+}
+
+// untiled bulk copy into shared memory: both addresses 16-byte aligned, bytes a multiple of 16
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
 

@@ -33,7 +33,7 @@ _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _HERE = contextlib.nullcontext()
 MAX_NORM_WIDTH = 8192
 MAX_CTC_LABELS = 2000
-MAX_CTC_FRAMES = 32768
+MAX_CTC_FRAMES = 16384
 
 
 def _on(device: torch.device):
@@ -400,6 +400,10 @@ def _ctc_operands(logits, targets, input_lengths, target_lengths):
     return logits, sb, st if T > 1 else V, i32
 
 
+def _ctc_pitch(S: int) -> int:
+    return (S + 2 + 3) // 4 * 4                    # gsn_ctc_loss_pitch
+
+
 def _ctc_loss(logits, targets, input_lengths, target_lengths, blank, zero_infinity, gradient):
     name = "granite::ctc_loss"
     _ctc_check(name, logits, targets, input_lengths, target_lengths, blank)
@@ -409,29 +413,34 @@ def _ctc_loss(logits, targets, input_lengths, target_lengths, blank, zero_infini
     loss = torch.empty((B,), dtype=torch.float32, device=dev)
     raw = torch.empty((B,), dtype=torch.float32, device=dev)
     stats = torch.empty((B, T, 2), dtype=torch.float32, device=dev)
-    post = torch.empty((B, T, S + 1), dtype=torch.float32, device=dev)
+    pitch = _ctc_pitch(S)
+    post = torch.empty((B, T, pitch), dtype=torch.float32, device=dev)
+    order = torch.empty((B, pitch), dtype=torch.int32, device=dev)
     with _on(dev):
         x, sb, st, (tg, il, tl) = _ctc_operands(logits, targets, input_lengths, target_lengths)
-        nbytes = _lib.lib().gsn_ctc_loss_workspace_bytes(B, T, S) if gradient else 0
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
+        nbytes = _lib.lib().gsn_ctc_loss_workspace_bytes(B, T, S, int(gradient))
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
         _lib.call("gsn_ctc_loss_fwd", x.data_ptr(), sb, st, tg.data_ptr(), il.data_ptr(), tl.data_ptr(), B, T, V, S,
-                  blank, int(zero_infinity), _TYPES[x.dtype], loss.data_ptr(), raw.data_ptr(), stats.data_ptr(),
-                  post.data_ptr(), _ptr(ws), nbytes, _stream(dev))
-    return loss, raw, stats, post
+                  blank, int(zero_infinity), int(gradient), _TYPES[x.dtype], loss.data_ptr(), raw.data_ptr(),
+                  stats.data_ptr(), post.data_ptr(), order.data_ptr(), ws.data_ptr(), nbytes, _stream(dev))
+    return loss, raw, stats, post, order
 
 
-def _ctc_loss_backward(dloss, logits, targets, input_lengths, target_lengths, raw, stats, post, blank, zero_infinity):
+def _ctc_loss_backward(dloss, logits, targets, input_lengths, target_lengths, raw, stats, post, order,
+                       blank, zero_infinity):
     name = "granite::ctc_loss_backward"
     _ctc_check(name, logits, targets, input_lengths, target_lengths, blank)
-    _check_device(name, logits, dloss, raw, stats, post)
+    _check_device(name, logits, dloss, raw, stats, post, order)
     B, T, V = logits.shape
     S = targets.shape[1]
-    if dloss.shape != (B,) or raw.shape != (B,) or stats.shape != (B, T, 2) or post.shape != (B, T, S + 1):
-        raise RuntimeError(f"{name}: dloss {tuple(dloss.shape)}, raw_loss {tuple(raw.shape)}, stats "
-                           f"{tuple(stats.shape)}, posteriors {tuple(post.shape)} beside logits {(B, T, V)} and "
-                           f"targets {(B, S)}")
-    if any(t.dtype != torch.float32 or not t.is_contiguous() for t in (raw, stats, post)):
-        raise RuntimeError(f"{name}: raw_loss, stats and posteriors must be the fp32 outputs of granite::ctc_loss")
+    if dloss.shape != (B,):
+        raise RuntimeError(f"{name}: dloss must be [{B}], got {tuple(dloss.shape)}")
+    pitch = _ctc_pitch(S)
+    kept = ((raw, (B,), torch.float32), (stats, (B, T, 2), torch.float32), (post, (B, T, pitch), torch.float32),
+            (order, (B, pitch), torch.int32))
+    if any(t.shape != shape or t.dtype != dtype or not t.is_contiguous() for t, shape, dtype in kept):
+        raise RuntimeError(f"{name}: raw_loss, stats, posteriors and order must be the outputs of granite::ctc_loss "
+                           f"for logits {(B, T, V)} and targets {(B, S)}")
     dev = logits.device
     dx = torch.empty((B, T, V), dtype=logits.dtype, device=dev)
     with _on(dev):
@@ -439,15 +448,16 @@ def _ctc_loss_backward(dloss, logits, targets, input_lengths, target_lengths, ra
         d = dloss.to(torch.float32).contiguous()
         _lib.call("gsn_ctc_loss_bwd", d.data_ptr(), x.data_ptr(), sb, st, tg.data_ptr(), il.data_ptr(), tl.data_ptr(),
                   B, T, V, S, blank, int(zero_infinity), _TYPES[x.dtype], raw.data_ptr(), stats.data_ptr(),
-                  post.data_ptr(), dx.data_ptr(), _stream(dev))
+                  post.data_ptr(), order.data_ptr(), dx.data_ptr(), _stream(dev))
     return dx
 
 
 @torch.library.custom_op("granite::ctc_loss", mutates_args=(), device_types="cuda")
 def ctc_loss_op(logits: torch.Tensor, targets: torch.Tensor, input_lengths: torch.Tensor,
                 target_lengths: torch.Tensor, blank: int, zero_infinity: bool
-                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(loss [B], and what the gradient needs: raw_loss [B], stats [B, T, 2], posteriors [B, T, S + 1]), all fp32."""
+                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(loss [B] fp32, and what the gradient needs: raw_loss [B], stats [B, T, 2], posteriors [B, T, P] fp32 and order
+    [B, P] int32, P = S + 2 rounded up to four)."""
     return _ctc_loss(logits, targets, input_lengths, target_lengths, blank, zero_infinity, True)
 
 
@@ -455,29 +465,29 @@ def ctc_loss_op(logits: torch.Tensor, targets: torch.Tensor, input_lengths: torc
 def _(logits, targets, input_lengths, target_lengths, blank, zero_infinity):
     B, T, _ = logits.shape
     f = dict(dtype=torch.float32)
+    pitch = _ctc_pitch(targets.shape[1])
     return (logits.new_empty((B,), **f), logits.new_empty((B,), **f), logits.new_empty((B, T, 2), **f),
-            logits.new_empty((B, T, targets.shape[1] + 1), **f))
+            logits.new_empty((B, T, pitch), **f), logits.new_empty((B, pitch), dtype=torch.int32))
 
 
 @torch.library.custom_op("granite::ctc_loss_backward", mutates_args=(), device_types="cuda")
 def ctc_loss_backward_op(dloss: torch.Tensor, logits: torch.Tensor, targets: torch.Tensor,
                          input_lengths: torch.Tensor, target_lengths: torch.Tensor, raw_loss: torch.Tensor,
-                         stats: torch.Tensor, posteriors: torch.Tensor, blank: int,
+                         stats: torch.Tensor, posteriors: torch.Tensor, order: torch.Tensor, blank: int,
                          zero_infinity: bool) -> torch.Tensor:
     """The gradient of granite::ctc_loss's logits for the gradient dloss [B] of its loss."""
     return _ctc_loss_backward(dloss, logits, targets, input_lengths, target_lengths, raw_loss, stats, posteriors,
-                              blank, zero_infinity)
+                              order, blank, zero_infinity)
 
 
 @ctc_loss_backward_op.register_fake
-def _(dloss, logits, targets, input_lengths, target_lengths, raw_loss, stats, posteriors, blank, zero_infinity):
+def _(dloss, logits, targets, input_lengths, target_lengths, raw_loss, stats, posteriors, order, blank, zero_infinity):
     return torch.empty_like(logits, memory_format=torch.contiguous_format)
 
 
 def _ctc_loss_setup(ctx, inputs, output):
     logits, targets, input_lengths, target_lengths, ctx.blank, ctx.zero_infinity = inputs
-    _, raw, stats, post = output
-    ctx.save_for_backward(logits, targets, input_lengths, target_lengths, raw, stats, post)
+    ctx.save_for_backward(logits, targets, input_lengths, target_lengths, *output[1:])
     ctx.set_materialize_grads(False)
 
 
