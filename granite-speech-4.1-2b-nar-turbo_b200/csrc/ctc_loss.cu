@@ -215,8 +215,9 @@ __host__ __device__ constexpr int lattice_warps(int pairs, int NP, int HL) {
   return pairs <= 32 * NP ? 1 : 1 + (pairs - 32 * NP + (32 - HL) * NP - 1) / ((32 - HL) * NP);
 }
 
+// Four warps at most hold up to three pairs a lane; one more warp fetches the frames and adds up the blanks.
 template <int NP, int H, int NBUF, bool GRAD>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 128 : 544) ctc_lattice_kernel(CtcArgs a, int nw) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) ctc_lattice_kernel(CtcArgs a, int nw) {
   constexpr int HL = halo_lanes<NP, H>(), NS = 2 * NP;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[NBUF];
@@ -249,11 +250,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 128 : 544) 
     abort_flag = 0;
     fence_mbar_init();
   }
-  // this lane's pairs: labels, whether a jump from the label below is allowed, where they lie in a frame
+  const bool producer = w == nw;
+  // this lane's pairs: where their labels lie in a frame, whether a jump from the label below is allowed (0) or not
   const int i0 = w * (32 - HL) * NP + lane * NP;
-  const bool own = w == 0 || lane >= HL;
+  const bool own = !producer && (w == 0 || lane >= HL);
+  const bool active = !producer && i0 - lane * NP <= len;   // a warp beyond the last pair only keeps the barriers
   const int* targets = a.targets + (int64_t)b * a.S;
-  int slot[NP], pen[NP], ob[NP], ol[NP], rb[NP], rl[NP];
+  const int step = dir ? -1 : 1;
+  int slot[NP], pen[NP];
 #pragma unroll
   for (int j = 0; j < NP; ++j) {
     const int i = i0 + j;
@@ -264,28 +268,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 128 : 544) 
       const int later = __ldg(targets + (dir ? li + 1 : li)), earlier = __ldg(targets + (dir ? li : li - 1));
       if (later != a.blank && later != earlier) pen[j] = 0;
     }
-    // the other side's pairs of this blank and label, and the warps that hold them
-    const int qb = i <= len ? len - i : 0, ql = i < len ? len - 1 - i : 0;
-    ob[j] = 2 * qb;
-    ol[j] = 2 * ql + 1;
-    rb[j] = 2 * (pitch) + (qb < 32 * NP ? 0 : 1 + (qb - 32 * NP) / ((32 - HL) * NP));
-    rl[j] = 2 * (pitch) + (ql < 32 * NP ? 0 : 1 + (ql - 32 * NP) / ((32 - HL) * NP));
   }
+  const int blanks_here = own ? min(max(len + 1 - i0, 0), NP) : 0, labels_here = own ? min(max(len - i0, 0), NP) : 0;
+  // The other side's order is the reverse: its pair len - i has this pair's blank, its pair len - 1 - i this label.
+  // So this lane reads its pairs q0, q0 - 1, ..., q0 - NP; they lie in at most two of its warps, whose references are
+  // found behind the states: `second` of the NP + 1 pairs belong to the lower one.
+  const int q0 = len - i0;
+  auto owner = [&](int q) { return q < 32 * NP ? 0 : 1 + (q - 32 * NP) / ((32 - HL) * NP); };
+  const int ref_hi = 2 * pitch + owner(max(q0, 0)), ref_lo = 2 * pitch + owner(max(q0 - NP, 0));
+  int from_lo = NP + 1;                            // pairs q0 - from_lo and below are the lower warp's
+  for (int j = NP; j >= 1; --j)
+    if (owner(max(q0 - j, 0)) != owner(max(q0, 0))) from_lo = j;
+
   float m[NS];
   int e[NS];
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     m[s] = 1.f;
-    e[s] = i0 == 0 && s == 0 ? 0 : kZeroExp;       // one path, before the first frame
+    e[s] = i0 == 0 && s == 0 && !producer ? 0 : kZeroExp;   // one path, before the first frame
   }
-  // the frames' normalisers
+  // the frames' normalisers, by the warp that has the time
   double norm = 0.0;
-  if (dir == 0)
-    for (int t = tid; t < n; t += blockDim.x) norm += (double)log2f(__ldg(&a.stats[frame0 + t].y));
+  if (dir == 0 && producer)
+    for (int t = lane; t < n; t += 32) norm += (double)log2f(__ldg(&a.stats[frame0 + t].y));
   __syncthreads();
 
   const int h = (n + 1) / 2, n1 = dir ? n - h : h;  // this side's frames before the meeting
-  const bool active = i0 - lane * NP <= len;        // a warp beyond the last pair only keeps the barriers
   int issued = 0, waited = 0, blocks = 0, parity = 0;
   bool fail = false;
 
@@ -296,6 +304,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 128 : 544) 
     mbar_arrive_expect_tx(&full[buf], be + bs);
     bulk_load(em_ring + buf * H * pitch, a.post + (frame0 + lo) * pitch, be, &full[buf]);
     if (states) bulk_load(st_ring + buf * H * spitch, a.states + (frame0 + lo) * spitch, bs, &full[buf]);
+    ++issued;
   };
   auto refresh_halo = [&]() {
     if (w > 0 && lane < HL) {
@@ -320,43 +329,124 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 128 : 544) 
       for (int s = 0; s < NS; ++s) dst[s] = make_float2(m[s], __int_as_float(e[s]));
     }
   };
+  float um;
+  int ue;                                          // the label of the pair below this lane's
+  auto fetch_below = [&]() {
+    um = __shfl_up_sync(0xffffffffu, m[NS - 1], 1);
+    ue = __shfl_up_sync(0xffffffffu, e[NS - 1], 1);
+    if (lane == 0) ue = kZeroExp;
+  };
   // sums into every state, without the emission: (pm, pe)
   auto gather = [&](float (&pm)[NS], int (&pe)[NS]) {
-    float um = __shfl_up_sync(0xffffffffu, m[NS - 1], 1);
-    int ue = __shfl_up_sync(0xffffffffu, e[NS - 1], 1);
-    if (lane == 0) ue = kZeroExp;
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-      const float bm = m[2 * j], lm = m[2 * j + 1];
-      const int be = e[2 * j], le = e[2 * j + 1], je = ue + pen[j];
-      const int eb = max(be, ue), el = max(max(le, be), je);
+      const float bm = m[2 * j], lm = m[2 * j + 1], vm = j ? m[j ? 2 * j - 1 : 0] : um;
+      const int be = e[2 * j], le = e[2 * j + 1], ve = j ? e[j ? 2 * j - 1 : 0] : ue, je = ve + pen[j];
+      const int eb = max(be, ve), el = max(max(le, be), je);
       pe[2 * j] = eb;
-      pm[2 * j] = fmaf(bm, pow2i(be - eb), um * pow2i(ue - eb));
+      pm[2 * j] = fmaf(bm, pow2i(be - eb), vm * pow2i(ve - eb));
       pe[2 * j + 1] = el;
-      pm[2 * j + 1] = fmaf(lm, pow2i(le - el), fmaf(bm, pow2i(be - el), um * pow2i(je - el)));
-      um = lm;
-      ue = le;
+      pm[2 * j + 1] = fmaf(lm, pow2i(le - el), fmaf(bm, pow2i(be - el), vm * pow2i(je - el)));
     }
-  };
-  // multiplies a sum by an emission 2^x
-  auto emit = [&](float x, float& fm, int& fe) {
-    const float k = x + 12582912.f;                // 1.5 * 2^23: the nearest integer in the low bits
-    const int ki = __float_as_int(k) - 0x4B400000;
-    fm = ex2_approx(x - (k - 12582912.f));
-    fe = x < -524288.f ? kZeroExp : ki;
   };
 
   float zinv = 0.f;
   int zexp = 0;
+  // One block of up to H frames from shared memory.  What a frame needs is loaded and turned into factors while the
+  // frame before it is summed: the chain itself is a shuffle, a maximum of exponents, a scaling and a product.
+  auto frames = [&](auto second, auto whole, int k, int cnt, const float* em, const uint32_t* st, int ref) {
+    constexpr bool SECOND = decltype(second)::value, WHOLE = decltype(whole)::value;
+    const int first = dir ? cnt - 1 : 0;
+    em += first * pitch;
+    st += first * spitch;
+    const int64_t frame = frame0 + (dir ? n - 1 - k : k);
+    float* post = a.post + frame * pitch;
+    uint32_t* dst = a.states + frame * spitch;
+    float* bl = blanks + parity * H * nw * 32 + tid;
+    float x[NP + 1], xm[NP + 1];
+    int xe[NP + 1], rh = 0, rl = 0;
+    uint2 sv[NP + 1];
+    auto load_em = [&]() {
+#pragma unroll
+      for (int j = 0; j < NP; ++j) x[j] = em[slot[j]];
+      x[NP] = em[a.S + 1];
+    };
+    auto load_st = [&]() {
+      if constexpr (SECOND) {
+        rh = (int)st[ref_hi] - zexp;
+        rl = (int)st[ref_lo] - zexp;
+#pragma unroll
+        for (int j = 0; j <= NP; ++j) sv[j] = *reinterpret_cast<const uint2*>(st + 2 * max(q0 - j, 0));
+      }
+    };
+    auto convert = [&]() {                         // an emission 2^x as factor and exponent
+#pragma unroll
+      for (int j = 0; j <= NP; ++j) {
+        const float r = x[j] + 12582912.f;         // 1.5 * 2^23: the nearest integer in the low bits
+        xm[j] = ex2_approx(x[j] - (r - 12582912.f));
+        xe[j] = x[j] < -524288.f ? kZeroExp : __float_as_int(r) - 0x4B400000;
+      }
+    };
+    load_em();
+    load_st();
+    convert();
+    fetch_below();
+#pragma unroll(WHOLE && NP < 4 ? H : 1)
+    for (int f = 0; f < (WHOLE ? H : cnt); ++f) {
+      const bool more = f + 1 < (WHOLE ? H : cnt);
+      if (more) {
+        em += step * pitch;
+        load_em();
+      }
+      float pm[NS];
+      int pe[NS];
+      gather(pm, pe);
+#pragma unroll
+      for (int j = 0; j < NP; ++j) {
+        m[2 * j] = pm[2 * j] * xm[NP];
+        e[2 * j] = max(pe[2 * j] + xe[NP], kZeroExp);
+        m[2 * j + 1] = pm[2 * j + 1] * xm[j];
+        e[2 * j + 1] = max(pe[2 * j + 1] + xe[j], kZeroExp);
+      }
+      if (more) fetch_below();
+      if constexpr (SECOND) {
+        float blank = 0.f;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          const uint32_t vb = sv[j].x, vl = sv[j + 1].y;
+          const int eb = (int)(vb >> 17) + (j < from_lo ? rh : rl) + pe[2 * j];
+          const int el = (int)(vl >> 17) + (j + 1 < from_lo ? rh : rl) + pe[2 * j + 1];
+          const float mb = __uint_as_float(((vb & 0x1FFFFu) << 6) | 0x3F800000u) * zinv;
+          const float ml = __uint_as_float(((vl & 0x1FFFFu) << 6) | 0x3F800000u) * zinv;
+          const float gb = vb < kPackZero ? 0.f : pm[2 * j] * mb * pow2i(eb);
+          const float gl = vl < kPackZero ? 0.f : pm[2 * j + 1] * ml * pow2i(el);
+          if (j < blanks_here) blank += gb;
+          if (j < labels_here) post[slot[j]] = gl;
+        }
+        if (more) {
+          st += step * spitch;
+          load_st();
+        }
+        bl[f * nw * 32] = blank;
+        post += step * pitch;
+      } else if constexpr (GRAD) {
+#pragma unroll
+        for (int j = 0; j < NP; ++j)
+          if (j < blanks_here)
+            *reinterpret_cast<uint2*>(dst + 2 * (i0 + j)) =
+                make_uint2(pack_state(m[2 * j], e[2 * j], ref), pack_state(m[2 * j + 1], e[2 * j + 1], ref));
+        if (lane == 0) dst[2 * pitch + w] = (uint32_t)(ref - 127 - kPackBias);
+        dst += step * spitch;
+      }
+      if (more) convert();
+    }
+  };
   auto walk = [&](int k0, int k1, auto second) {
     constexpr bool SECOND = decltype(second)::value;
-    const int base = blocks;
-    if (tid == 0)
+    const int used = lattice_warps(len + 1, NP, HL);
+    if (producer && lane == 0)
       for (int u = 0; u < NBUF; ++u)
-        if (k0 + u * H < k1) {
-          issue(k0 + u * H, min(H, k1 - k0 - u * H), SECOND);
-          ++issued;
-        }
+        if (k0 + u * H < k1) issue(k0 + u * H, min(H, k1 - k0 - u * H), SECOND);
     for (int k = k0; k < k1 && !fail; k += H) {
       const int cnt = min(H, k1 - k), buf = blocks % NBUF;
       const bool ok = mbar_wait_bounded(&full[buf], (blocks / NBUF) & 1, &abort_flag, kStatusTimeoutCtc);
@@ -367,87 +457,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 128 : 544) 
 #pragma unroll
         for (int s = 1; s < NS; ++s) ref = max(ref, e[s]);
         ref = __reduce_max_sync(0xffffffffu, ref);
-        const float* em0 = em_ring + buf * H * pitch;
-        const uint32_t* st0 = st_ring + buf * H * spitch;
-        for (int f = 0; f < cnt; ++f) {
-          const int row = dir ? cnt - 1 - f : f;
-          const float* em = em0 + row * pitch;
-          const int64_t frame = frame0 + (dir ? n - 1 - k - f : k + f);
-          float pm[NS];
-          int pe[NS];
-          gather(pm, pe);
-          if constexpr (SECOND) {
-            const uint32_t* st = st0 + row * spitch;
-            float* post = a.post + frame * pitch;
-            float blank = 0.f;
-#pragma unroll
-            for (int j = 0; j < NP; ++j) {
-              const uint32_t vb = st[ob[j]], vl = st[ol[j]];
-              const int eb = (int)(vb >> 17) + (int)st[rb[j]] + pe[2 * j] - zexp;
-              const int el = (int)(vl >> 17) + (int)st[rl[j]] + pe[2 * j + 1] - zexp;
-              const float mb = __uint_as_float(((vb & 0x1FFFFu) << 6) | 0x3F800000u);
-              const float ml = __uint_as_float(((vl & 0x1FFFFu) << 6) | 0x3F800000u);
-              const float gb = vb < kPackZero ? 0.f : pm[2 * j] * mb * zinv * pow2i(eb);
-              const float gl = vl < kPackZero ? 0.f : pm[2 * j + 1] * ml * zinv * pow2i(el);
-              if (own && i0 + j <= len) blank += gb;
-              if (own && i0 + j < len) post[slot[j]] = gl;
-            }
-            blanks[(parity * H + f) * nw * 32 + tid] = blank;
-          }
-          float xm;
-          int xe;
-          emit(em[a.S + 1], xm, xe);
-#pragma unroll
-          for (int j = 0; j < NP; ++j) {
-            m[2 * j] = pm[2 * j] * xm;
-            e[2 * j] = max(pe[2 * j] + xe, kZeroExp);
-          }
-#pragma unroll
-          for (int j = 0; j < NP; ++j) {
-            emit(em[slot[j]], xm, xe);
-            m[2 * j + 1] = pm[2 * j + 1] * xm;
-            e[2 * j + 1] = max(pe[2 * j + 1] + xe, kZeroExp);
-          }
-          if constexpr (GRAD && !SECOND) {
-            uint32_t* dst = a.states + frame * spitch;
-            if (own)
-#pragma unroll
-              for (int j = 0; j < NP; ++j)
-                if (i0 + j <= len)
-                  *reinterpret_cast<uint2*>(dst + 2 * (i0 + j)) =
-                      make_uint2(pack_state(m[2 * j], e[2 * j], ref), pack_state(m[2 * j + 1], e[2 * j + 1], ref));
-            if (lane == 0) dst[2 * pitch + w] = (uint32_t)(ref - 127 - kPackBias);
-          }
-        }
+        const float* em = em_ring + buf * H * pitch;
+        const uint32_t* st = st_ring + buf * H * spitch;
+        if (cnt == H)
+          frames(second, std::true_type{}, k, cnt, em, st, ref);
+        else
+          frames(second, std::false_type{}, k, cnt, em, st, ref);
         publish_halo();
       }
       fail = __syncthreads_or(!ok);
-      if constexpr (SECOND) {
-        const int used = min(nw, lattice_warps(len + 1, NP, HL));
-        for (int f = w; f < cnt && !fail; f += nw) {
-          float s = 0.f;
-          for (int i = 0; i < used; ++i) s += blanks[(parity * H + f) * nw * 32 + i * 32 + lane];
+      if (producer && !fail) {
+        const int next = k + NBUF * H;
+        if (lane == 0 && next < k1) issue(next, min(H, k1 - next), SECOND);
+        if constexpr (SECOND) {
+          float s[H];
 #pragma unroll
-          for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-          if (lane == 0) a.post[(frame0 + (dir ? n - 1 - k - f : k + f)) * pitch + a.S + 1] = s;
+          for (int f = 0; f < H; ++f) {
+            s[f] = 0.f;
+            if (f < cnt)
+              for (int i = 0; i < used; ++i) s[f] += blanks[((parity * H + f) * nw + i) * 32 + lane];
+          }
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1)
+#pragma unroll
+            for (int f = 0; f < H; ++f) s[f] += __shfl_xor_sync(0xffffffffu, s[f], d);
+#pragma unroll
+          for (int f = 0; f < H; ++f)
+            if (lane == f && f < cnt) a.post[(frame0 + (dir ? n - 1 - k - f : k + f)) * pitch + a.S + 1] = s[f];
         }
       }
       parity ^= 1;
       ++blocks;
-      const int next = k0 + (blocks - base - 1 + NBUF) * H;
-      if (tid == 0 && next < k1 && !fail) {
-        issue(next, min(H, k1 - next), SECOND);
-        ++issued;
-      }
     }
   };
   auto drain = [&]() {                             // after a wait that ran out: the copies under way land first
-    if (tid == 0)
+    if (producer && lane == 0)
       for (int i = waited; i < issued; ++i)
         mbar_wait_bounded(&full[i % NBUF], (i / NBUF) & 1, nullptr, kStatusTimeoutCtc);
   };
 
-  publish_halo();
+  if (!producer) publish_halo();
   parity ^= 1;
   __syncthreads();
   walk(0, n1, std::false_type{});
@@ -455,50 +504,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 128 : 544) 
   // the meeting: Z = sum over the states of this side's sum into them times the other side's value
   float2* mine = a.exchange + ((int64_t)b * 2 + dir) * 2 * pitch;
   const float2* theirs = a.exchange + ((int64_t)b * 2 + (dir ^ 1)) * 2 * pitch;
-  if (active && own)
 #pragma unroll
-    for (int j = 0; j < NP; ++j)
-      if (i0 + j <= len) {
-        mine[2 * (i0 + j)] = make_float2(m[2 * j], __int_as_float(e[2 * j]));
-        mine[2 * (i0 + j) + 1] = make_float2(m[2 * j + 1], __int_as_float(e[2 * j + 1]));
-      }
+  for (int j = 0; j < NP; ++j)
+    if (j < blanks_here) {
+      mine[2 * (i0 + j)] = make_float2(m[2 * j], __int_as_float(e[2 * j]));
+      mine[2 * (i0 + j) + 1] = make_float2(m[2 * j + 1], __int_as_float(e[2 * j + 1]));
+    }
   // the states were stored by plain stores and are fetched by bulk copies of the other CTA
   asm volatile("fence.proxy.async;" ::: "memory");
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   asm volatile("fence.proxy.async;" ::: "memory");
   if (fail) return drain();
   {
-    float zmax_m[NS];
-    int zmax_e[NS];
     int top = 2 * kZeroExp;
     float total = 0.f;
     if (active) {
+      float pm[NS];
+      int pe[NS];
       refresh_halo();
-      gather(zmax_m, zmax_e);
+      fetch_below();
+      gather(pm, pe);
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
-        const bool hb = own && i0 + j <= len, hl = own && i0 + j < len;
-        const float2 vb = hb ? __ldcg(theirs + ob[j]) : make_float2(1.f, __int_as_float(kZeroExp));
-        const float2 vl = hl ? __ldcg(theirs + ol[j]) : make_float2(1.f, __int_as_float(kZeroExp));
-        zmax_m[2 * j] *= vb.x;
-        zmax_e[2 * j] += __float_as_int(vb.y);
-        zmax_m[2 * j + 1] *= vl.x;
-        zmax_e[2 * j + 1] += __float_as_int(vl.y);
+        const float2 none = make_float2(1.f, __int_as_float(kZeroExp));
+        const float2 vb = j < blanks_here ? __ldcg(theirs + 2 * (q0 - j)) : none;
+        const float2 vl = j < labels_here ? __ldcg(theirs + 2 * (q0 - j - 1) + 1) : none;
+        pm[2 * j] *= vb.x;
+        pe[2 * j] += __float_as_int(vb.y);
+        pm[2 * j + 1] *= vl.x;
+        pe[2 * j + 1] += __float_as_int(vl.y);
       }
 #pragma unroll
-      for (int s = 0; s < NS; ++s) top = max(top, zmax_e[s]);
+      for (int s = 0; s < NS; ++s) top = max(top, pe[s]);
       top = __reduce_max_sync(0xffffffffu, top);
 #pragma unroll
-      for (int s = 0; s < NS; ++s) total = fmaf(zmax_m[s], pow2i(zmax_e[s] - top), total);
+      for (int s = 0; s < NS; ++s) total = fmaf(pm[s], pow2i(pe[s] - top), total);
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
     }
+    if (producer) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, d);
-    if (lane == 0) {
+      for (int d = 16; d > 0; d >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, d);
+      if (lane == 0) sums[0] = norm;
+    } else if (lane == 0) {
       zm[w] = total;
       ze[w] = top;
-      sums[w] = norm;
     }
     __syncthreads();
     top = ze[0];
@@ -507,8 +557,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 128 : 544) 
     for (int i = 0; i < nw; ++i) total += zm[i] * pow2i(ze[i] - top);
     const bool exists = top > kZeroBelow;
     if (dir == 0 && tid == 0) {
-      norm = 0.0;
-      for (int i = 0; i < nw; ++i) norm += sums[i];
+      norm = sums[0];
       float raw = INFINITY;
       if (exists) raw = (float)((norm - (double)top - log2((double)total)) * 0.6931471805599453);
       if (!(norm > -INFINITY)) raw = NAN;          // a frame of NaN, +inf or nothing but -inf
@@ -642,7 +691,7 @@ int launch_lattice(const CtcArgs& a, cudaStream_t stream) {
                       (size_t)2 * nw * HL * NS * sizeof(float2) + (GRAD ? (size_t)2 * H * nw * 32 * 4 : 0);
   auto* kernel = ctc_lattice_kernel<NP, H, NBUF, GRAD>;
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
-  kernel<<<dim3(2, a.B), nw * 32, smem, stream>>>(a, nw);
+  kernel<<<dim3(2, a.B), (nw + 1) * 32, smem, stream>>>(a, nw);
   return (int)cudaGetLastError();
 }
 
