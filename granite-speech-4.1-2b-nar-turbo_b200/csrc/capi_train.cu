@@ -224,7 +224,8 @@ int gsn_ctc_loss_pitch(int S) { return S < 0 ? 0 : ctc_pitch(S); }
 
 size_t gsn_ctc_loss_workspace_bytes(int B, int T, int S, int gradient) {
   if (B <= 0 || T < 0 || S < 0 || S > kMaxCtcLabels) return 0;
-  size_t n = align256((size_t)B * sizeof(int)) + align256((size_t)B * 4 * ctc_pitch(S) * sizeof(float2));
+  size_t n = align256((size_t)B * sizeof(int)) + align256((size_t)B * T * sizeof(float)) +
+             align256((size_t)B * 4 * ctc_pitch(S) * sizeof(float2));
   if (gradient) n += (size_t)B * T * ctc_state_pitch(S) * sizeof(uint32_t);
   return n;
 }
@@ -267,6 +268,8 @@ int gsn_ctc_loss_fwd(const void* logits, int64_t ld_b, int64_t ld_t, const int32
   char* ws = static_cast<char*>(workspace);
   a.bad = (int*)ws;
   ws += align256((size_t)B * sizeof(int));
+  a.norms = (float*)ws;
+  ws += align256((size_t)B * T * sizeof(float));
   a.exchange = (float2*)ws;
   if (gradient) a.states = (uint32_t*)(ws + align256((size_t)B * 4 * a.pitch * sizeof(float2)));
   return finish(launch_ctc_loss(a, dtype, (cudaStream_t)stream), name);

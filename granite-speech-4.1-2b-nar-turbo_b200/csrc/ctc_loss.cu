@@ -10,6 +10,8 @@
 // lattice (both chains, the posteriors; a chain of n dependent steps), gradient (HBM-bound).  The emissions are taken
 // against the frame's largest logit, so the frame's normaliser stays out of the chain: it cancels in the posteriors,
 // and the loss adds the normalisers in 64 bits.
+#include <limits.h>
+
 #include <type_traits>
 
 #include "gsn_kernels.cuh"
@@ -28,28 +30,26 @@ constexpr float kLog2e = 1.4426950408889634f;
 // A state is m * 2^e with its own integer exponent.  Sums over paths leave fp32's range within a few dozen frames, and
 // a state thousands of octaves below its frame's largest can still carry the whole posterior (a confident model and
 // another transcript), so neither fp32 with a scale a frame nor fp64 holds them; the logarithm in fp32 would lose
-// 2^-12 at -4000, and costs three exponentials and a logarithm a step where this costs none.  m >= 1 always; a zero
-// has e near kZeroExp, so that its terms vanish in any sum.
-//   bounds: a frame's emission is 2^-15871 at the least (kLowest) or impossible, kMaxCtcFrames of them reach -2^28;
+// 2^-12 at -4000.  m lies within a few octaves of 1; a zero has e near kZeroExp, so that its terms vanish in any sum.
+//   bounds: a frame's emission is 2^-1020 at the least or impossible, kMaxCtcFrames of them reach -2^24;
 //   kZeroExp = -2^29, e is held at or above it, and no sum of three exponents leaves an int.
 constexpr int kZeroExp = -(1 << 29);
-constexpr int kZeroBelow = -(3 << 27);        // exponents below it are zeros
-constexpr float kLowest = -15870.f;           // log2 of an emission against the frame's largest; below it: impossible
-constexpr float kImpossible = -1048576.f;     // how an impossible emission is stored (log2)
+constexpr int kZeroBelow = -(1 << 28);        // exponents below it are zeros
 
 // 2^d for d <= 127 (0 from -127 down)
 __device__ __forceinline__ float pow2i(int d) { return __int_as_float(max(d + 127, 0) << 23); }
 
-// Stored states: 15 bits of exponent against a reference of the frame's warp, 17 bits of mantissa after the leading
-// one.  Four bytes a state keep half the traffic of a pair; the posterior's rounding of 2^-18 lies below what the
-// chain leaves.  The reference is the largest exponent of the warp's states (its neighbours below included) when its
-// frames of one block began: no state can outgrow it within the block.  A state 2^32600 below it counts as zero.
-constexpr int kPackBias = 32600;
-__device__ __forceinline__ uint32_t pack_state(float m, int e, int ref) {
-  const int t = max(e - ref, -kPackBias - 120);                // m < 2^17: the fields never touch
-  return ((__float_as_uint(m) + 0x20u) >> 6) + ((uint32_t)(t + kPackBias) << 17);
+// Stored numbers, emissions and states alike, are the high word of an fp64: 11 bits of exponent, 20 of mantissa,
+// rounded to nearest (2^-21, an eighth of an fp32 logit's own step at 10).  0 is zero.  An emission is against the
+// frame's likeliest class of the transcript; a state against its lane's reference exponent, stored beside it.
+constexpr uint32_t kWordOne = 1u << 20;       // words below it are zeros
+__device__ __forceinline__ uint32_t to_word(float m, int e) {          // m * 2^e, 0 where it leaves the range
+  const uint32_t v = ((__float_as_uint(m) + 4u) >> 3) + ((uint32_t)(e + 896) << 20);
+  return e < -1000 ? 0u : v;
 }
-constexpr uint32_t kPackZero = 64u << 17;                      // below: a zero
+__device__ __forceinline__ float word_mantissa(uint32_t v) {
+  return __uint_as_float(((v & (kWordOne - 1)) << 3) | 0x3F800000u);
+}
 
 // ---- vectors of eight logits at any alignment ------------------------------------------------------------------------
 // Elements before the first 16-byte boundary of a row, which the vector loops leave to single loads.
@@ -151,21 +151,51 @@ __device__ __forceinline__ void plan_utterance(const CtcArgs& a, int b) {
   if (threadIdx.x == 0) a.bad[b] = bad;
 }
 
-// emissions against the frame's largest logit, log2: labels at [0, len), impossible up to S, the blank at S + 1
+// 2^l as a stored word, for l <= 0 = a / ln 2
+__device__ __forceinline__ uint32_t emission_word(float a, float& l) {
+  constexpr double log2e = 1.4426950408889634;
+  constexpr float hi = (float)log2e, lo = (float)(log2e - (double)hi);
+  l = a * hi;
+  if (!(l >= -1000.f)) return 0u;                // impossible (NaN: the frame's sum tells)
+  const float k = rintf(l);
+  // the fraction from 1 / ln 2 in two parts: one rounding near zero instead of one near |l|
+  return to_word(ex2_approx(fmaf(a, lo, fmaf(a, hi, -k))), (int)k);
+}
+
+// Emission words of one frame: labels at [0, len), a zero at S, the blank at S + 1, and at S + 2 how many octaves the
+// least of them lies below the likeliest.  Returns that one's logit (one warp, the same in every lane).
 template <typename T>
-__device__ __forceinline__ void write_emissions(const CtcArgs& a, const T* x, float top, int64_t frame, int b, int tid,
-                                                int threads) {
-  float* em = a.post + frame * a.pitch;
+__device__ __forceinline__ float write_emissions(const CtcArgs& a, const T* x, int64_t frame, int b, int lane) {
+  uint32_t* em = reinterpret_cast<uint32_t*>(a.post) + frame * a.pitch;
   const int len = min(max(__ldg(a.target_lengths + b), 0), a.S);
-  for (int i = tid; i < a.S + 2; i += threads) {
-    float e = kImpossible;
-    if (i < len || i == a.S + 1) {
-      const int v = i < len ? __ldg(a.targets + (int64_t)b * a.S + i) : a.blank;
-      if (v >= 0 && v < a.V) e = (to_f32(x[v]) - top) * kLog2e;
-      if (!(e >= kLowest)) e = kImpossible;
-    }
-    em[i] = e;
+  const int* targets = a.targets + (int64_t)b * a.S;
+  auto logit = [&](int i) {
+    const int v = i < len ? __ldg(targets + i) : a.blank;
+    return v >= 0 && v < a.V ? to_f32(x[v]) : -INFINITY;
+  };
+  float best = -INFINITY;
+  for (int i = lane; i <= len; i += 32) best = fmaxf(best, logit(i));
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
+  float least = 0.f;
+  for (int i = lane; i <= len; i += 32) {
+    float l;
+    const uint32_t v = emission_word(logit(i) - best, l);
+    if (v) least = fminf(least, l);
+    em[i < len ? i : a.S + 1] = v;
   }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, d));
+  if (lane == 0) {
+    em[a.S] = 0u;
+    em[a.S + 2] = (uint32_t)(int)ceilf(-least);
+  }
+  return best;
+}
+
+// what the frame adds to -log2 Z: its emissions are against `best` instead of the softmax's denominator
+__device__ __forceinline__ float frame_norm(const Online& o, float best) {
+  return log2f(o.sum) + (best == -INFINITY ? 0.f : (o.top - best) * kLog2e);
 }
 
 constexpr int kRowThreads = 256;
@@ -183,18 +213,25 @@ __global__ void __launch_bounds__(kRowThreads) ctc_rows_kernel(CtcArgs a) {
   const int64_t frame = (int64_t)b * a.T + t;
   if (WARP_ROW) {
     const Online o = scan_row<T, 32>(x, a.V, lane);
-    if (lane == 0) a.stats[frame] = make_float2(o.top, o.sum);
-    write_emissions(a, x, o.top, frame, b, lane, 32);
+    const float best = write_emissions(a, x, frame, b, lane);
+    if (lane == 0) {
+      a.stats[frame] = make_float2(o.top, o.sum);
+      a.norms[frame] = frame_norm(o, best);
+    }
   } else {
     __shared__ Online part[kRowThreads / 32];
     Online o = scan_row<T, kRowThreads>(x, a.V, threadIdx.x);
     if (lane == 0) part[warp] = o;
     __syncthreads();
+    if (warp > 0) return;
     o = part[0];
 #pragma unroll
     for (int i = 1; i < kRowThreads / 32; ++i) o = online_join(o, part[i]);
-    if (threadIdx.x == 0) a.stats[frame] = make_float2(o.top, o.sum);
-    write_emissions(a, x, o.top, frame, b, threadIdx.x, kRowThreads);
+    const float best = write_emissions(a, x, frame, b, lane);
+    if (lane == 0) {
+      a.stats[frame] = make_float2(o.top, o.sum);
+      a.norms[frame] = frame_norm(o, best);
+    }
   }
 }
 
@@ -208,6 +245,14 @@ __global__ void __launch_bounds__(kRowThreads) ctc_rows_kernel(CtcArgs a) {
 // below: one shuffle within the warp.  Across warps, each keeps the top HL lanes' worth of the warp below it as extra
 // pairs of its own at its low end; H steps reach at most 2 H states, so they are refreshed every H frames, and one
 // barrier serves H steps.  Emissions and the other side's states come H frames at a time by bulk copies.
+//
+// Within a block of H frames a lane may hold its states as fp64 against one exponent, the largest of the states that
+// can reach it: a step is then two additions, a multiply-add and two products a pair, and the stored words are used as
+// they are.  A warp takes this form where the states of each reach and the block's emissions together span no more
+// than kFastSpan octaves, which keeps every state of weight a normal number; any other block, and one that is not
+// whole, runs on the exponent of every state, at three times the instructions.
+constexpr int kFastSpan = 950;
+
 template <int NP, int H>
 __host__ __device__ constexpr int halo_lanes() { return (H + NP - 1) / NP; }
 
@@ -240,8 +285,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
   const int pitch = a.pitch, spitch = a.state_pitch;
   const int64_t frame0 = (int64_t)b * a.T;
   // shared memory: emission ring, state ring (GRAD), halo exchange, blanks' partial sums (GRAD)
-  float* em_ring = reinterpret_cast<float*>(smem);
-  uint32_t* st_ring = reinterpret_cast<uint32_t*>(em_ring + NBUF * H * pitch);
+  uint32_t* em_ring = reinterpret_cast<uint32_t*>(smem);
+  uint32_t* st_ring = em_ring + NBUF * H * pitch;
   float2* halo = reinterpret_cast<float2*>(st_ring + (GRAD ? NBUF * H * spitch : 0));   // [2][nw][HL * NS]
   float* blanks = reinterpret_cast<float*>(halo + 2 * nw * HL * NS);                     // [2][H][nw * 32]
 
@@ -271,14 +316,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
   }
   const int blanks_here = own ? min(max(len + 1 - i0, 0), NP) : 0, labels_here = own ? min(max(len - i0, 0), NP) : 0;
   // The other side's order is the reverse: its pair len - i has this pair's blank, its pair len - 1 - i this label.
-  // So this lane reads its pairs q0, q0 - 1, ..., q0 - NP; they lie in at most two of its warps, whose references are
-  // found behind the states: `second` of the NP + 1 pairs belong to the lower one.
+  // So this lane reads its pairs q0, q0 - 1, ..., q0 - NP; they lie in two of its lanes at most, whose references are
+  // found behind the states: pairs q0 - from_lo and below are the lower lane's.
   const int q0 = len - i0;
-  auto owner = [&](int q) { return q < 32 * NP ? 0 : 1 + (q - 32 * NP) / ((32 - HL) * NP); };
-  const int ref_hi = 2 * pitch + owner(max(q0, 0)), ref_lo = 2 * pitch + owner(max(q0 - NP, 0));
-  int from_lo = NP + 1;                            // pairs q0 - from_lo and below are the lower warp's
+  auto owner = [&](int q) {
+    q = max(q, 0);
+    const int ow = q < 32 * NP ? 0 : 1 + (q - 32 * NP) / ((32 - HL) * NP);
+    return ow * 32 + (q - ow * (32 - HL) * NP) / NP;
+  };
+  const int ref_hi = 2 * pitch + owner(q0), ref_lo = 2 * pitch + owner(q0 - NP);
+  int from_lo = NP + 1;
+#pragma unroll
   for (int j = NP; j >= 1; --j)
-    if (owner(max(q0 - j, 0)) != owner(max(q0, 0))) from_lo = j;
+    if (owner(q0 - j) != owner(q0)) from_lo = j;
 
   float m[NS];
   int e[NS];
@@ -290,7 +340,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
   // the frames' normalisers, by the warp that has the time
   double norm = 0.0;
   if (dir == 0 && producer)
-    for (int t = lane; t < n; t += 32) norm += (double)log2f(__ldg(&a.stats[frame0 + t].y));
+    for (int t = lane; t < n; t += 32) norm += (double)__ldg(a.norms + frame0 + t);
   __syncthreads();
 
   const int h = (n + 1) / 2, n1 = dir ? n - h : h;  // this side's frames before the meeting
@@ -352,20 +402,106 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
 
   float zinv = 0.f;
   int zexp = 0;
-  // One block of up to H frames from shared memory.  What a frame needs is loaded and turned into factors while the
-  // frame before it is summed: the chain itself is a shuffle, a maximum of exponents, a scaling and a product.
-  auto frames = [&](auto second, auto whole, int k, int cnt, const float* em, const uint32_t* st, int ref) {
-    constexpr bool SECOND = decltype(second)::value, WHOLE = decltype(whole)::value;
+  // One block of frames on the exponent of every state.
+  auto frames = [&](auto second, int k, int cnt, const uint32_t* em, const uint32_t* st) {
+    constexpr bool SECOND = decltype(second)::value;
     const int first = dir ? cnt - 1 : 0;
+    const int64_t frame = frame0 + (dir ? n - 1 - k : k);
     em += first * pitch;
     st += first * spitch;
+    [[maybe_unused]] float* post = a.post + frame * pitch;
+    [[maybe_unused]] uint32_t* dst = a.states + frame * spitch;
+    [[maybe_unused]] float* bl = blanks + parity * H * nw * 32 + tid;
+    for (int f = 0; f < cnt; ++f) {
+      float pm[NS];
+      int pe[NS];
+      fetch_below();
+      gather(pm, pe);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const uint32_t x = em[s & 1 ? slot[s / 2] : a.S + 1];
+        m[s] = pm[s] * word_mantissa(x);
+        e[s] = max(pe[s] + (x < kWordOne ? kZeroExp : (int)(x >> 20) - 1023), kZeroExp);
+      }
+      if constexpr (SECOND) {
+        const int rh = (int)st[ref_hi] - zexp, rl = (int)st[ref_lo] - zexp;
+        float blank = 0.f;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          const uint32_t vb = st[2 * max(q0 - j, 0)], vl = st[2 * max(q0 - j - 1, 0) + 1];
+          const int eb = (int)(vb >> 20) + (j < from_lo ? rh : rl) + pe[2 * j];
+          const int el = (int)(vl >> 20) + (j + 1 < from_lo ? rh : rl) + pe[2 * j + 1];
+          const float gb = vb < kWordOne ? 0.f : pm[2 * j] * (word_mantissa(vb) * zinv) * pow2i(eb);
+          const float gl = vl < kWordOne ? 0.f : pm[2 * j + 1] * (word_mantissa(vl) * zinv) * pow2i(el);
+          if (j < blanks_here) blank += gb;
+          if (j < labels_here) post[slot[j]] = gl;
+        }
+        bl[f * nw * 32] = blank;
+        post += step * pitch;
+        st += step * spitch;
+      } else if constexpr (GRAD) {
+        int ref = e[0];
+#pragma unroll
+        for (int s = 1; s < NS; ++s) ref = max(ref, e[s]);
+#pragma unroll
+        for (int j = 0; j < NP; ++j)
+          if (j < blanks_here)
+            *reinterpret_cast<uint2*>(dst + 2 * (i0 + j)) =
+                make_uint2(to_word(m[2 * j], e[2 * j] - ref), to_word(m[2 * j + 1], e[2 * j + 1] - ref));
+        if (own) dst[2 * pitch + tid] = (uint32_t)(ref - 1023);
+        dst += step * spitch;
+      }
+      em += step * pitch;
+    }
+  };
+
+  // Whether a whole block can run as fp64 against E, and E: the largest exponent of the states that reach this lane.
+  int E = 0;
+  double below = 0.0;                              // the label below comes against its own lane's E
+  auto fast_block = [&](const uint32_t* em) {
+    int hi = e[0], lo = INT_MAX;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      hi = max(hi, e[s]);
+      lo = min(lo, e[s] < kZeroBelow ? INT_MAX : e[s]);
+    }
+#pragma unroll
+    for (int d = 1; d <= HL; d *= 2) {
+      const int uh = __shfl_up_sync(0xffffffffu, hi, d), ul = __shfl_up_sync(0xffffffffu, lo, d);
+      if (lane >= d) {
+        hi = max(hi, uh);
+        lo = min(lo, ul);
+      }
+    }
+    E = hi;
+    // where nothing but zeros reaches a lane, nothing comes from below within the block either
+    const int lower = __shfl_up_sync(0xffffffffu, E, 1) - E;
+    const bool closed = lane == 0 || E < kZeroBelow;
+    below = __hiloint2double(closed || lower < -1000 ? 0 : (min(lower, 1000) + 1023) << 20, 0);
+    const int span = __reduce_add_sync(0xffffffffu, lane < H ? em[lane * pitch + a.S + 2] : 0u);
+    return __all_sync(0xffffffffu, (lo == INT_MAX || hi - lo + span <= kFastSpan) && (closed || lower <= 900));
+  };
+  auto fast_frames = [&](auto second, int k, const uint32_t* em, const uint32_t* st) {
+    constexpr bool SECOND = decltype(second)::value;
+    const int first = dir ? H - 1 : 0;
     const int64_t frame = frame0 + (dir ? n - 1 - k : k);
-    float* post = a.post + frame * pitch;
-    uint32_t* dst = a.states + frame * spitch;
-    float* bl = blanks + parity * H * nw * 32 + tid;
-    float x[NP + 1], xm[NP + 1];
-    int xe[NP + 1], rh = 0, rl = 0;
-    uint2 sv[NP + 1];
+    em += first * pitch;
+    st += first * spitch;
+    [[maybe_unused]] float* post = a.post + frame * pitch;
+    [[maybe_unused]] uint32_t* dst = a.states + frame * spitch;
+    [[maybe_unused]] float* bl = blanks + parity * H * nw * 32 + tid;
+    double v[NS], jump[NP];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const uint32_t bits = __float_as_uint(m[s]);
+      const int d = e[s] - E;
+      v[s] = d < -1000 ? 0.0 : __hiloint2double((int)(bits >> 3) + ((d + 896) << 20), (int)(bits << 29));
+    }
+#pragma unroll
+    for (int j = 0; j < NP; ++j) jump[j] = pen[j] == 0 ? 1.0 : 0.0;
+    uint32_t x[NP + 1];
+    [[maybe_unused]] uint2 sv[NP + 1];
+    [[maybe_unused]] int rh = 0, rl = 0;
     auto load_em = [&]() {
 #pragma unroll
       for (int j = 0; j < NP; ++j) x[j] = em[slot[j]];
@@ -373,72 +509,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
     };
     auto load_st = [&]() {
       if constexpr (SECOND) {
-        rh = (int)st[ref_hi] - zexp;
-        rl = (int)st[ref_lo] - zexp;
+        rh = (int)st[ref_hi];
+        rl = (int)st[ref_lo];
 #pragma unroll
         for (int j = 0; j <= NP; ++j) sv[j] = *reinterpret_cast<const uint2*>(st + 2 * max(q0 - j, 0));
       }
     };
-    auto convert = [&]() {                         // an emission 2^x as factor and exponent
-#pragma unroll
-      for (int j = 0; j <= NP; ++j) {
-        const float r = x[j] + 12582912.f;         // 1.5 * 2^23: the nearest integer in the low bits
-        xm[j] = ex2_approx(x[j] - (r - 12582912.f));
-        xe[j] = x[j] < -524288.f ? kZeroExp : __float_as_int(r) - 0x4B400000;
-      }
-    };
     load_em();
     load_st();
-    convert();
-    fetch_below();
-#pragma unroll(WHOLE && NP < 4 ? H : 1)
-    for (int f = 0; f < (WHOLE ? H : cnt); ++f) {
-      const bool more = f + 1 < (WHOLE ? H : cnt);
-      if (more) {
+    double u = __shfl_up_sync(0xffffffffu, v[NS - 1], 1);
+#pragma unroll
+    for (int f = 0; f < H; ++f) {
+      double p[NP + 1], pre[NS];
+#pragma unroll
+      for (int j = 0; j <= NP; ++j) p[j] = __hiloint2double((int)x[j], 0);
+      if (f + 1 < H) {
         em += step * pitch;
         load_em();
       }
-      float pm[NS];
-      int pe[NS];
-      gather(pm, pe);
+      const double ub = u * below;
 #pragma unroll
-      for (int j = 0; j < NP; ++j) {
-        m[2 * j] = pm[2 * j] * xm[NP];
-        e[2 * j] = max(pe[2 * j] + xe[NP], kZeroExp);
-        m[2 * j + 1] = pm[2 * j + 1] * xm[j];
-        e[2 * j + 1] = max(pe[2 * j + 1] + xe[j], kZeroExp);
+      for (int j = NP - 1; j >= 0; --j) {
+        const double ul = j ? v[j ? 2 * j - 1 : 0] : ub;
+        pre[2 * j + 1] = fma(jump[j], ul, v[2 * j + 1] + v[2 * j]);
+        pre[2 * j] = v[2 * j] + ul;
+        v[2 * j + 1] = pre[2 * j + 1] * p[j];
+        v[2 * j] = pre[2 * j] * p[NP];
+        if (j == NP - 1 && f + 1 < H) u = __shfl_up_sync(0xffffffffu, v[NS - 1], 1);
       }
-      if (more) fetch_below();
       if constexpr (SECOND) {
+        // the other side's value against 2^(zexp - E), as fp64; what lies above its range meets a zero
+        const int sh = rh + E - zexp + 1023, sl = rl + E - zexp + 1023;
+        auto other = [&](uint32_t word, int shift) {
+          const int field = min(max((int)(word >> 20) + shift, 0), 2046);
+          return __hiloint2double(word < kWordOne ? 0 : (int)((field << 20) | (word & (kWordOne - 1))), 0);
+        };
         float blank = 0.f;
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
-          const uint32_t vb = sv[j].x, vl = sv[j + 1].y;
-          const int eb = (int)(vb >> 17) + (j < from_lo ? rh : rl) + pe[2 * j];
-          const int el = (int)(vl >> 17) + (j + 1 < from_lo ? rh : rl) + pe[2 * j + 1];
-          const float mb = __uint_as_float(((vb & 0x1FFFFu) << 6) | 0x3F800000u) * zinv;
-          const float ml = __uint_as_float(((vl & 0x1FFFFu) << 6) | 0x3F800000u) * zinv;
-          const float gb = vb < kPackZero ? 0.f : pm[2 * j] * mb * pow2i(eb);
-          const float gl = vl < kPackZero ? 0.f : pm[2 * j + 1] * ml * pow2i(el);
+          const float gb = (float)(pre[2 * j] * other(sv[j].x, j < from_lo ? sh : sl)) * zinv;
+          const float gl = (float)(pre[2 * j + 1] * other(sv[j + 1].y, j + 1 < from_lo ? sh : sl)) * zinv;
           if (j < blanks_here) blank += gb;
           if (j < labels_here) post[slot[j]] = gl;
         }
-        if (more) {
+        if (f + 1 < H) {
           st += step * spitch;
           load_st();
         }
         bl[f * nw * 32] = blank;
         post += step * pitch;
       } else if constexpr (GRAD) {
+        auto word = [](double d) { return (uint32_t)__double2hiint(d) + ((uint32_t)__double2loint(d) >> 31); };
 #pragma unroll
         for (int j = 0; j < NP; ++j)
-          if (j < blanks_here)
-            *reinterpret_cast<uint2*>(dst + 2 * (i0 + j)) =
-                make_uint2(pack_state(m[2 * j], e[2 * j], ref), pack_state(m[2 * j + 1], e[2 * j + 1], ref));
-        if (lane == 0) dst[2 * pitch + w] = (uint32_t)(ref - 127 - kPackBias);
+          if (j < blanks_here) *reinterpret_cast<uint2*>(dst + 2 * (i0 + j)) = make_uint2(word(v[2 * j]), word(v[2 * j + 1]));
+        if (own) dst[2 * pitch + tid] = (uint32_t)(E - 1023);
         dst += step * spitch;
       }
-      if (more) convert();
+    }
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const int hi = __double2hiint(v[s]);
+      const bool zero = hi < (int)kWordOne;
+      m[s] = zero ? 1.f : (float)__hiloint2double((hi & (int)(kWordOne - 1)) | 0x3FF00000, __double2loint(v[s]));
+      e[s] = zero ? kZeroExp : (hi >> 20) - 1023 + E;
     }
   };
   auto walk = [&](int k0, int k1, auto second) {
@@ -453,16 +587,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
       if (ok) ++waited;
       if (ok && active) {
         refresh_halo();
-        int ref = e[0];
-#pragma unroll
-        for (int s = 1; s < NS; ++s) ref = max(ref, e[s]);
-        ref = __reduce_max_sync(0xffffffffu, ref);
-        const float* em = em_ring + buf * H * pitch;
+        const uint32_t* em = em_ring + buf * H * pitch;
         const uint32_t* st = st_ring + buf * H * spitch;
-        if (cnt == H)
-          frames(second, std::true_type{}, k, cnt, em, st, ref);
+        if (cnt == H && fast_block(em))
+          fast_frames(second, k, em, st);
         else
-          frames(second, std::false_type{}, k, cnt, em, st, ref);
+          frames(second, k, cnt, em, st);
         publish_halo();
       }
       fail = __syncthreads_or(!ok);
@@ -721,6 +851,7 @@ CtcArgs batch_part(const CtcArgs& a, int b0, int size) {
   c.raw_loss += b0;
   if (c.loss) c.loss += b0;
   if (c.bad) c.bad += b0;
+  if (c.norms) c.norms += frames;
   if (c.exchange) c.exchange += (int64_t)b0 * 4 * a.pitch;
   if (c.states) c.states += frames * a.state_pitch;
   if (c.dloss) c.dloss += b0;
@@ -759,13 +890,13 @@ int launch_grad(const CtcArgs& a, cudaStream_t stream) {
 
 }  // namespace ctc_loss_impl
 
-int ctc_pitch(int S) { return (S + 2 + 3) / 4 * 4; }
+int ctc_pitch(int S) { return (S + 3 + 3) / 4 * 4; }
 
 int ctc_state_pitch(int S) {
   using namespace ctc_loss_impl;
-  // the states of S + 1 pairs, and a reference for each warp (at most as many as one pair a lane needs)
-  const int warps = lattice_warps(S + 1, 1, halo_lanes<1, 8>());
-  return 2 * ctc_pitch(S) + (warps + 3) / 4 * 4;
+  // the states of the pairs, and a reference for every lane of the warps that hold them
+  int warps = lattice_warps(S + 1, 4, halo_lanes<4, 4>());
+  return 2 * ctc_pitch(S) + 32 * (warps > 4 ? warps : 4);
 }
 
 int launch_ctc_loss(const CtcArgs& args, int dtype, cudaStream_t stream) {

@@ -195,11 +195,12 @@ struct CtcArgs {
   int pitch = 0;                 // ctc_pitch(S)
   int state_pitch = 0;           // ctc_state_pitch(S)
   float2* stats = nullptr;       // [B, T] (largest logit, sum of exp(logit - largest))
-  float* post = nullptr;         // [B, T, pitch]: emissions, then posteriors, of the labels; blank's at S + 1
+  float* post = nullptr;         // [B, T, pitch]: emission words, then posteriors, of the labels; blank's at S + 1
   int* order = nullptr;          // [B, pitch] the transcript's places in the order of their labels
   float* raw_loss = nullptr;     // [B] loss, inf where no path exists, NaN for bad input
   float* loss = nullptr;         // [B] loss with zero_infinity applied
   int* bad = nullptr;            // workspace [B]: a length or label out of range
+  float* norms = nullptr;        // workspace [B, T]: what each frame adds to -log2 Z
   float2* exchange = nullptr;    // workspace [B, 2, 2 pitch]: both sides' states where they meet
   uint32_t* states = nullptr;    // workspace [B, T, state_pitch], or null: no posteriors wanted
   const float* dloss = nullptr;  // [B]

@@ -401,7 +401,7 @@ def _ctc_operands(logits, targets, input_lengths, target_lengths):
 
 
 def _ctc_pitch(S: int) -> int:
-    return (S + 2 + 3) // 4 * 4                    # gsn_ctc_loss_pitch
+    return (S + 3 + 3) // 4 * 4                    # gsn_ctc_loss_pitch
 
 
 def _ctc_loss(logits, targets, input_lengths, target_lengths, blank, zero_infinity, gradient):
@@ -457,7 +457,7 @@ def ctc_loss_op(logits: torch.Tensor, targets: torch.Tensor, input_lengths: torc
                 target_lengths: torch.Tensor, blank: int, zero_infinity: bool
                 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(loss [B] fp32, and what the gradient needs: raw_loss [B], stats [B, T, 2], posteriors [B, T, P] fp32 and order
-    [B, P] int32, P = S + 2 rounded up to four)."""
+    [B, P] int32, P = S + 3 rounded up to four)."""
     return _ctc_loss(logits, targets, input_lengths, target_lengths, blank, zero_infinity, True)
 
 
