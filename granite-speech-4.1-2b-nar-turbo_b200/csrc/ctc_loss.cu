@@ -47,6 +47,12 @@ __device__ __forceinline__ uint32_t to_word(float m, int e) {          // m * 2^
   const uint32_t v = ((__float_as_uint(m) + 4u) >> 3) + ((uint32_t)(e + 896) << 20);
   return e < -1000 ? 0u : v;
 }
+// A double in [0, 2^127) cut to fp32, zero below 2^-126: three integer instructions (the conversion instruction from
+// fp64 runs at a sixteenth of their rate or less: with it a frame of three pairs a lane took 455 cycles, not 160).
+__device__ __forceinline__ float to_float(double d) {
+  const uint32_t hi = (uint32_t)__double2hiint(d), lo = (uint32_t)__double2loint(d);
+  return hi < (897u << 20) ? 0.f : __uint_as_float(__funnelshift_l(lo, hi - (896u << 20), 3));
+}
 __device__ __forceinline__ float word_mantissa(uint32_t v) {
   return __uint_as_float(((v & (kWordOne - 1)) << 3) | 0x3F800000u);
 }
@@ -248,10 +254,11 @@ __global__ void __launch_bounds__(kRowThreads) ctc_rows_kernel(CtcArgs a) {
 //
 // Within a block of H frames a lane may hold its states as fp64 against one exponent, the largest of the states that
 // can reach it: a step is then two additions, a multiply-add and two products a pair, and the stored words are used as
-// they are.  A warp takes this form where the states of each reach and the block's emissions together span no more
-// than kFastSpan octaves, which keeps every state of weight a normal number; any other block, and one that is not
-// whole, runs on the exponent of every state, at three times the instructions.
-constexpr int kFastSpan = 950;
+// they are.  A warp takes this form where its states (else the states of each lane's reach) and the block's emissions
+// together span no more than kFastSpan octaves, which keeps every state of weight a normal number; any other block,
+// and one that is not whole, runs on the exponent of every state, at three times the instructions.
+constexpr int kFastSpan = 1850;
+constexpr int kFastBias = 900;                // the largest state starts a block at 2^900
 
 template <int NP, int H>
 __host__ __device__ constexpr int halo_lanes() { return (H + NP - 1) / NP; }
@@ -262,11 +269,10 @@ __host__ __device__ constexpr int lattice_warps(int pairs, int NP, int HL) {
 
 // Four warps at most hold up to three pairs a lane; one more warp fetches the frames and adds up the blanks.
 template <int NP, int H, int NBUF, bool GRAD>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) ctc_lattice_kernel(CtcArgs a, int nw) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 8 ? 288 : 576) ctc_lattice_kernel(CtcArgs a, int nw) {
   constexpr int HL = halo_lanes<NP, H>(), NS = 2 * NP;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[NBUF];
-  __shared__ int abort_flag;
   __shared__ double sums[32];
   __shared__ float zm[32];
   __shared__ int ze[32];
@@ -282,17 +288,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
     }
     return;
   }
-  const int pitch = a.pitch, spitch = a.state_pitch;
+  const int pitch = a.pitch, spitch = a.state_pitch, brow = nw * 32 + 4;
   const int64_t frame0 = (int64_t)b * a.T;
   // shared memory: emission ring, state ring (GRAD), halo exchange, blanks' partial sums (GRAD)
   uint32_t* em_ring = reinterpret_cast<uint32_t*>(smem);
   uint32_t* st_ring = em_ring + NBUF * H * pitch;
   float2* halo = reinterpret_cast<float2*>(st_ring + (GRAD ? NBUF * H * spitch : 0));   // [2][nw][HL * NS]
-  float* blanks = reinterpret_cast<float*>(halo + 2 * nw * HL * NS);                     // [2][H][nw * 32]
+  float* blanks = reinterpret_cast<float*>(halo + 2 * nw * HL * NS);                     // [2][H][nw * 32 + 4]
 
   if (tid == 0) {
     for (int i = 0; i < NBUF; ++i) mbar_init(&full[i], 1);
-    abort_flag = 0;
     fence_mbar_init();
   }
   const bool producer = w == nw;
@@ -365,12 +370,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
         e[s] = __float_as_int(src[s].y);
       }
     }
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {                 // leading ones out of m
-      const int bits = __float_as_int(m[s]), k = (bits >> 23) - 127;
-      m[s] = __int_as_float(bits - (k << 23));
-      e[s] += k;
-    }
   };
   auto publish_halo = [&]() {
     if (lane >= 32 - HL) {
@@ -402,7 +401,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
 
   float zinv = 0.f;
   int zexp = 0;
-  // One block of frames on the exponent of every state.
+  // One block of frames on the exponent of every state; m grows by less than 2^2.6 a frame in between.
   auto frames = [&](auto second, int k, int cnt, const uint32_t* em, const uint32_t* st) {
     constexpr bool SECOND = decltype(second)::value;
     const int first = dir ? cnt - 1 : 0;
@@ -411,7 +410,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
     st += first * spitch;
     [[maybe_unused]] float* post = a.post + frame * pitch;
     [[maybe_unused]] uint32_t* dst = a.states + frame * spitch;
-    [[maybe_unused]] float* bl = blanks + parity * H * nw * 32 + tid;
+    [[maybe_unused]] float* bl = blanks + parity * H * brow + tid;
     for (int f = 0; f < cnt; ++f) {
       float pm[NS];
       int pe[NS];
@@ -436,7 +435,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
           if (j < blanks_here) blank += gb;
           if (j < labels_here) post[slot[j]] = gl;
         }
-        bl[f * nw * 32] = blank;
+        bl[f * brow] = blank;
         post += step * pitch;
         st += step * spitch;
       } else if constexpr (GRAD) {
@@ -453,9 +452,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
       }
       em += step * pitch;
     }
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {                 // leading ones out of m
+      const int bits = __float_as_int(m[s]), d = (bits >> 23) - 127;
+      m[s] = __int_as_float(bits - (d << 23));
+      e[s] += d;
+    }
   };
 
-  // Whether a whole block can run as fp64 against E, and E: the largest exponent of the states that reach this lane.
+  // Whether a whole block can run as fp64 against E, and E: the largest exponent of the warp's states, or of those that
+  // reach this lane.
   int E = 0;
   double below = 0.0;                              // the label below comes against its own lane's E
   auto fast_block = [&](const uint32_t* em) {
@@ -465,6 +471,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
       hi = max(hi, e[s]);
       lo = min(lo, e[s] < kZeroBelow ? INT_MAX : e[s]);
     }
+    const int span = __reduce_add_sync(0xffffffffu, lane < H ? em[lane * pitch + a.S + 2] : 0u);
+    const int top = __reduce_max_sync(0xffffffffu, hi), least = __reduce_min_sync(0xffffffffu, lo);
+    E = top;
+    below = lane == 0 ? 0.0 : 1.0;
+    if (least == INT_MAX || top - least + span <= kFastSpan) return true;
 #pragma unroll
     for (int d = 1; d <= HL; d *= 2) {
       const int uh = __shfl_up_sync(0xffffffffu, hi, d), ul = __shfl_up_sync(0xffffffffu, lo, d);
@@ -478,8 +489,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
     const int lower = __shfl_up_sync(0xffffffffu, E, 1) - E;
     const bool closed = lane == 0 || E < kZeroBelow;
     below = __hiloint2double(closed || lower < -1000 ? 0 : (min(lower, 1000) + 1023) << 20, 0);
-    const int span = __reduce_add_sync(0xffffffffu, lane < H ? em[lane * pitch + a.S + 2] : 0u);
-    return __all_sync(0xffffffffu, (lo == INT_MAX || hi - lo + span <= kFastSpan) && (closed || lower <= 900));
+    return __all_sync(0xffffffffu, (lo == INT_MAX || hi - lo + span <= kFastSpan) && (closed || lower <= 900)) != 0;
   };
   auto fast_frames = [&](auto second, int k, const uint32_t* em, const uint32_t* st) {
     constexpr bool SECOND = decltype(second)::value;
@@ -489,16 +499,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
     st += first * spitch;
     [[maybe_unused]] float* post = a.post + frame * pitch;
     [[maybe_unused]] uint32_t* dst = a.states + frame * spitch;
-    [[maybe_unused]] float* bl = blanks + parity * H * nw * 32 + tid;
-    double v[NS], jump[NP];
+    [[maybe_unused]] float* bl = blanks + parity * H * brow + tid;
+    double v[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       const uint32_t bits = __float_as_uint(m[s]);
       const int d = e[s] - E;
-      v[s] = d < -1000 ? 0.0 : __hiloint2double((int)(bits >> 3) + ((d + 896) << 20), (int)(bits << 29));
+      v[s] = d < -kFastSpan - 50 ? 0.0 : __hiloint2double((int)(bits >> 3) + ((d + 896 + kFastBias) << 20), (int)(bits << 29));
     }
-#pragma unroll
-    for (int j = 0; j < NP; ++j) jump[j] = pen[j] == 0 ? 1.0 : 0.0;
     uint32_t x[NP + 1];
     [[maybe_unused]] uint2 sv[NP + 1];
     [[maybe_unused]] int rh = 0, rl = 0;
@@ -518,28 +526,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
     load_em();
     load_st();
     double u = __shfl_up_sync(0xffffffffu, v[NS - 1], 1);
-#pragma unroll
+    // as far unrolled as the instruction cache holds: three pairs and eight frames of the second half took 2.2 times
+    // as long as two
+    constexpr int UNROLL = !SECOND ? 8 : NP == 1 ? 4 : 2;
+#pragma unroll(UNROLL)
     for (int f = 0; f < H; ++f) {
       double p[NP + 1], pre[NS];
 #pragma unroll
       for (int j = 0; j <= NP; ++j) p[j] = __hiloint2double((int)x[j], 0);
-      if (f + 1 < H) {
+      const bool more = f + 1 < H;
+      if (more) {
         em += step * pitch;
         load_em();
       }
       const double ub = u * below;
+      // from the top pair down: each reads the label below it before that changes
 #pragma unroll
       for (int j = NP - 1; j >= 0; --j) {
         const double ul = j ? v[j ? 2 * j - 1 : 0] : ub;
-        pre[2 * j + 1] = fma(jump[j], ul, v[2 * j + 1] + v[2 * j]);
-        pre[2 * j] = v[2 * j] + ul;
-        v[2 * j + 1] = pre[2 * j + 1] * p[j];
-        v[2 * j] = pre[2 * j] * p[NP];
-        if (j == NP - 1 && f + 1 < H) u = __shfl_up_sync(0xffffffffu, v[NS - 1], 1);
+        if constexpr (SECOND) {
+          pre[2 * j + 1] = fma(pen[j] == 0 ? 1.0 : 0.0, ul, v[2 * j + 1] + v[2 * j]);
+          pre[2 * j] = v[2 * j] + ul;
+          v[2 * j + 1] = pre[2 * j + 1] * p[j];
+          v[2 * j] = pre[2 * j] * p[NP];
+        } else {                                   // the shortest chain: one multiply-add behind the shuffle, two in a lane
+          v[2 * j + 1] = fma(pen[j] == 0 ? p[j] : 0.0, ul, fma(p[j], v[2 * j + 1], p[j] * v[2 * j]));
+          v[2 * j] = fma(p[NP], ul, p[NP] * v[2 * j]);
+        }
+        if (j == NP - 1 && more) u = __shfl_up_sync(0xffffffffu, v[NS - 1], 1);
       }
       if constexpr (SECOND) {
-        // the other side's value against 2^(zexp - E), as fp64; what lies above its range meets a zero
-        const int sh = rh + E - zexp + 1023, sl = rl + E - zexp + 1023;
+        // the other side's value against 2^(zexp - E + kFastBias), as fp64; what lies above its range meets a zero
+        const int sh = rh + E - kFastBias - zexp + 1023, sl = rl + E - kFastBias - zexp + 1023;
         auto other = [&](uint32_t word, int shift) {
           const int field = min(max((int)(word >> 20) + shift, 0), 2046);
           return __hiloint2double(word < kWordOne ? 0 : (int)((field << 20) | (word & (kWordOne - 1))), 0);
@@ -547,45 +565,75 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
         float blank = 0.f;
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
-          const float gb = (float)(pre[2 * j] * other(sv[j].x, j < from_lo ? sh : sl)) * zinv;
-          const float gl = (float)(pre[2 * j + 1] * other(sv[j + 1].y, j + 1 < from_lo ? sh : sl)) * zinv;
+          const float gb = to_float(pre[2 * j] * other(sv[j].x, j < from_lo ? sh : sl)) * zinv;
+          const float gl = to_float(pre[2 * j + 1] * other(sv[j + 1].y, j + 1 < from_lo ? sh : sl)) * zinv;
           if (j < blanks_here) blank += gb;
           if (j < labels_here) post[slot[j]] = gl;
         }
-        if (f + 1 < H) {
+        if (more) {
           st += step * spitch;
           load_st();
         }
-        bl[f * nw * 32] = blank;
+        bl[f * brow] = blank;
         post += step * pitch;
       } else if constexpr (GRAD) {
         auto word = [](double d) { return (uint32_t)__double2hiint(d) + ((uint32_t)__double2loint(d) >> 31); };
 #pragma unroll
         for (int j = 0; j < NP; ++j)
           if (j < blanks_here) *reinterpret_cast<uint2*>(dst + 2 * (i0 + j)) = make_uint2(word(v[2 * j]), word(v[2 * j + 1]));
-        if (own) dst[2 * pitch + tid] = (uint32_t)(E - 1023);
+        if (own) dst[2 * pitch + tid] = (uint32_t)(E - kFastBias - 1023);
         dst += step * spitch;
       }
     }
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      const int hi = __double2hiint(v[s]);
+      const long long bits = __double_as_longlong(v[s]) + (1ll << 28);   // to_float cuts: rounds to nearest
+      const int hi = (int)(bits >> 32);
       const bool zero = hi < (int)kWordOne;
-      m[s] = zero ? 1.f : (float)__hiloint2double((hi & (int)(kWordOne - 1)) | 0x3FF00000, __double2loint(v[s]));
-      e[s] = zero ? kZeroExp : (hi >> 20) - 1023 + E;
+      m[s] = zero ? 1.f : to_float(__hiloint2double((hi & (int)(kWordOne - 1)) | 0x3FF00000, (int)bits));
+      e[s] = zero ? kZeroExp : (hi >> 20) - 1023 - kFastBias + E;
     }
+  };
+  // The fetching warp waits for the frames one block ahead, so the barrier behind a block also hands over the next.
+  auto wait_block = [&](int block) {
+    const bool ok = mbar_wait_bounded(&full[block % NBUF], (block / NBUF) & 1, nullptr, kStatusTimeoutCtc);
+    if (ok) ++waited;
+    return ok;
   };
   auto walk = [&](int k0, int k1, auto second) {
     constexpr bool SECOND = decltype(second)::value;
-    const int used = lattice_warps(len + 1, NP, HL);
-    if (producer && lane == 0)
-      for (int u = 0; u < NBUF; ++u)
-        if (k0 + u * H < k1) issue(k0 + u * H, min(H, k1 - k0 - u * H), SECOND);
+    if (k0 >= k1) return;
+    const int vecs = lattice_warps(len + 1, NP, HL) * 8;        // of four blanks a frame
+    auto add_blanks = [&](int k, int cnt, int half) {           // 32 / H lanes a frame
+      const int f = lane / (32 / H);
+      float s = 0.f;
+      const float4* src = reinterpret_cast<const float4*>(blanks + (half * H + f) * brow);
+      if (f < cnt)
+        for (int i = lane % (32 / H); i < vecs; i += 32 / H) {
+          const float4 q = src[i];
+          s += (q.x + q.y) + (q.z + q.w);
+        }
+#pragma unroll
+      for (int d = 16 / H; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+      if (f < cnt && lane % (32 / H) == 0) a.post[(frame0 + (dir ? n - 1 - k - f : k + f)) * pitch + a.S + 1] = s;
+    };
+    bool ok = true;
+    if (producer) {
+      if (lane == 0)
+        for (int u = 0; u < NBUF; ++u)
+          if (k0 + u * H < k1) issue(k0 + u * H, min(H, k1 - k0 - u * H), SECOND);
+      ok = wait_block(blocks);
+    }
+    fail = __syncthreads_or(!ok);
     for (int k = k0; k < k1 && !fail; k += H) {
       const int cnt = min(H, k1 - k), buf = blocks % NBUF;
-      const bool ok = mbar_wait_bounded(&full[buf], (blocks / NBUF) & 1, &abort_flag, kStatusTimeoutCtc);
-      if (ok) ++waited;
-      if (ok && active) {
+      if (producer) {
+        const int next = k + (NBUF - 1) * H;                     // into the buffer of the block before this one
+        if (lane == 0 && k > k0 && next < k1) issue(next, min(H, k1 - next), SECOND);
+        if constexpr (SECOND)
+          if (k > k0) add_blanks(k - H, H, parity ^ 1);
+        if (k + H < k1) ok = wait_block(blocks + 1);
+      } else if (active) {
         refresh_halo();
         const uint32_t* em = em_ring + buf * H * pitch;
         const uint32_t* st = st_ring + buf * H * spitch;
@@ -596,29 +644,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : 576) 
         publish_halo();
       }
       fail = __syncthreads_or(!ok);
-      if (producer && !fail) {
-        const int next = k + NBUF * H;
-        if (lane == 0 && next < k1) issue(next, min(H, k1 - next), SECOND);
-        if constexpr (SECOND) {
-          float s[H];
-#pragma unroll
-          for (int f = 0; f < H; ++f) {
-            s[f] = 0.f;
-            if (f < cnt)
-              for (int i = 0; i < used; ++i) s[f] += blanks[((parity * H + f) * nw + i) * 32 + lane];
-          }
-#pragma unroll
-          for (int d = 16; d > 0; d >>= 1)
-#pragma unroll
-            for (int f = 0; f < H; ++f) s[f] += __shfl_xor_sync(0xffffffffu, s[f], d);
-#pragma unroll
-          for (int f = 0; f < H; ++f)
-            if (lane == f && f < cnt) a.post[(frame0 + (dir ? n - 1 - k - f : k + f)) * pitch + a.S + 1] = s[f];
-        }
-      }
       parity ^= 1;
       ++blocks;
     }
+    if constexpr (SECOND)
+      if (producer && !fail) {
+        const int last = (k1 - k0 - 1) / H * H;
+        add_blanks(k0 + last, k1 - k0 - last, parity ^ 1);
+      }
   };
   auto drain = [&]() {                             // after a wait that ran out: the copies under way land first
     if (producer && lane == 0)
@@ -818,21 +851,23 @@ int launch_lattice(const CtcArgs& a, cudaStream_t stream) {
   constexpr int HL = halo_lanes<NP, H>(), NS = 2 * NP;
   const int nw = lattice_warps(a.S + 1, NP, HL);
   const size_t smem = (size_t)NBUF * H * a.pitch * 4 + (GRAD ? (size_t)NBUF * H * a.state_pitch * 4 : 0) +
-                      (size_t)2 * nw * HL * NS * sizeof(float2) + (GRAD ? (size_t)2 * H * nw * 32 * 4 : 0);
+                      (size_t)2 * nw * HL * NS * sizeof(float2) + (GRAD ? (size_t)2 * H * (nw * 32 + 4) * 4 : 0);
   auto* kernel = ctc_lattice_kernel<NP, H, NBUF, GRAD>;
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
   kernel<<<dim3(2, a.B), (nw + 1) * 32, smem, stream>>>(a, nw);
   return (int)cudaGetLastError();
 }
 
-// Pairs a lane: as few as four warps hold (one a scheduler of the SM, so that a step issues in the least time); beyond
-// those, four pairs a lane and more warps.
+// Pairs a lane: as few as four warps hold (one a scheduler of the SM, so that a step issues in the least time), then
+// four pairs and more warps.  Frames a block: 16 where they fit (48 utterances of 1536 frames with 300 labels: 195 us,
+// with 8 frames 252 us: about 500 cycles go into a block's begin and end), fewer where the rows get long.
 template <bool GRAD>
 int launch_lattice_for(const CtcArgs& a, cudaStream_t stream) {
   const int pairs = a.S + 1;
-  if (lattice_warps(pairs, 1, halo_lanes<1, 8>()) <= 4) return launch_lattice<1, 8, 3, GRAD>(a, stream);
-  if (lattice_warps(pairs, 2, halo_lanes<2, 8>()) <= 4) return launch_lattice<2, 8, 3, GRAD>(a, stream);
-  if (lattice_warps(pairs, 3, halo_lanes<3, 8>()) <= 4) return launch_lattice<3, 8, 3, GRAD>(a, stream);
+  if (lattice_warps(pairs, 1, halo_lanes<1, 16>()) <= 4) return launch_lattice<1, 16, 2, GRAD>(a, stream);
+  if (lattice_warps(pairs, 2, halo_lanes<2, 16>()) <= 4) return launch_lattice<2, 16, 2, GRAD>(a, stream);
+  if (lattice_warps(pairs, 3, halo_lanes<3, 16>()) <= 4) return launch_lattice<3, 16, 2, GRAD>(a, stream);
+  if (lattice_warps(pairs, 4, halo_lanes<4, 8>()) <= 8) return launch_lattice<4, 8, 2, GRAD>(a, stream);
   return launch_lattice<4, 4, 2, GRAD>(a, stream);
 }
 

@@ -291,7 +291,7 @@ def check_ctc(logits, targets, il, tl, blank=0, zero_infinity=False, dloss=None)
     weighs at most log V) and n steps of the chain; the posteriors carry the chain's roundings from both sides."""
     B, T, V = logits.shape
     rl, rg = R.ctc(logits, targets, il, tl, blank, zero_infinity)
-    x = logits.detach().clone().requires_grad_()
+    x = logits.detach().requires_grad_()           # as it lies, strides and alignment
     loss = tr.ctc_loss(x, targets, il, tl, blank=blank, zero_infinity=zero_infinity)
     d = torch.linspace(0.5, 2.0, B, device=DEV) if dloss is None else dloss
     grad, = torch.autograd.grad(loss, x, d)
@@ -393,17 +393,19 @@ def test_ctc_bad_input_is_nan():
 
 
 def test_ctc_strides_and_index_types():
-    """Frames first, int64 indices, a broadcast batch, a padded class axis, off the 16-byte grid: the same bits."""
+    """Frames first, a padded class axis, classes outermost, each within the bounds (a row's sum begins at its own
+    16-byte boundary, so its order is the alignment's); int64 indices and a broadcast batch, the same bits."""
     logits, targets, il, tl = ctc_case(10, 3, 21, 40, 5, BF)
     base = check_ctc(logits, targets, il, tl)
-    time_first = logits.transpose(0, 1).contiguous().transpose(0, 1)
     wide = torch.zeros(3, 21, 47, dtype=BF, device=DEV)
     wide[..., 3:43] = logits
-    for x in (time_first, wide[..., 3:43], logits.transpose(1, 2).contiguous().transpose(1, 2)):
-        x = x.detach().requires_grad_()
-        loss = tr.ctc_loss(x, targets.long(), il.long(), tl.long())
-        grad, = torch.autograd.grad(loss, x, torch.linspace(0.5, 2.0, 3, device=DEV))
-        assert torch.equal(loss, base[0]) and torch.equal(grad, base[1])
+    for x in (logits.transpose(0, 1).contiguous().transpose(0, 1), wide[..., 3:43],
+              logits.transpose(1, 2).contiguous().transpose(1, 2)):
+        check_ctc(x, targets, il, tl)
+    x = logits.clone().requires_grad_()
+    loss = tr.ctc_loss(x, targets.long(), il.long(), tl.long())
+    grad, = torch.autograd.grad(loss, x, torch.linspace(0.5, 2.0, 3, device=DEV))
+    assert torch.equal(loss, base[0]) and torch.equal(grad, base[1])
     one = logits[:1].expand(3, -1, -1)
     same = tr.ctc_loss(one, targets[:1].expand(3, -1), il, tl)
     assert torch.equal(same, tr.ctc_loss(logits[:1], targets[:1], il[:1], tl[:1]).expand(3))
