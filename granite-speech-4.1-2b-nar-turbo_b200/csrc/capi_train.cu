@@ -239,9 +239,9 @@ int gsn_ctc_loss_fwd(const void* logits, int64_t ld_b, int64_t ld_t, const int32
   if (!input_lengths || !target_lengths || !loss || !raw_loss || !order || (S > 0 && !targets) ||
       (T > 0 && (!logits || !stats || !posteriors)))
     return fail(GSN_ERR_INVALID_ARG, "%s: null pointer", name);
-  if (!aligned(logits, type_size(dtype)) || !aligned(stats, 8) || !aligned(posteriors, 16))
-    return fail(GSN_ERR_UNSUPPORTED, "%s: logits must be aligned to their type, stats to 8 and posteriors to 16 bytes",
-                name);
+  if (!aligned(logits, type_size(dtype)) || !aligned(stats, 8) || !aligned(posteriors, 16) || !aligned(order, 8))
+    return fail(GSN_ERR_UNSUPPORTED,
+                "%s: logits must be aligned to their type, stats and order to 8, posteriors to 16 bytes", name);
   const size_t need = gsn_ctc_loss_workspace_bytes(B, T, S, gradient);
   if (workspace_bytes < need) return fail(GSN_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", name, workspace_bytes, need);
   if (!workspace || !aligned(workspace, 16)) return fail(GSN_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", name);
@@ -264,7 +264,7 @@ int gsn_ctc_loss_fwd(const void* logits, int64_t ld_b, int64_t ld_t, const int32
   a.raw_loss = raw_loss;
   a.stats = (float2*)stats;
   a.post = posteriors;
-  a.order = order;
+  a.order = (int2*)order;
   char* ws = static_cast<char*>(workspace);
   a.bad = (int*)ws;
   ws += align256((size_t)B * sizeof(int));
@@ -285,8 +285,10 @@ int gsn_ctc_loss_bwd(const float* dloss, const void* logits, int64_t ld_b, int64
   if (!dloss || !logits || !input_lengths || !target_lengths || (S > 0 && !targets) || !raw_loss || !stats ||
       !posteriors || !order || !dlogits)
     return fail(GSN_ERR_INVALID_ARG, "%s: null pointer", name);
-  if (!aligned(logits, type_size(dtype)) || !aligned(dlogits, type_size(dtype)) || !aligned(stats, 8))
-    return fail(GSN_ERR_UNSUPPORTED, "%s: logits and dlogits must be aligned to their type, stats to 8 bytes", name);
+  if (!aligned(logits, type_size(dtype)) || !aligned(dlogits, type_size(dtype)) || !aligned(stats, 8) ||
+      !aligned(order, 8))
+    return fail(GSN_ERR_UNSUPPORTED, "%s: logits and dlogits must be aligned to their type, stats and order to 8 bytes",
+                name);
   CtcArgs a;
   a.logits = logits;
   a.ld_b = ld_b;
@@ -304,7 +306,7 @@ int gsn_ctc_loss_bwd(const float* dloss, const void* logits, int64_t ld_b, int64
   a.raw_loss = const_cast<float*>(raw_loss);
   a.stats = (float2*)const_cast<float*>(stats);
   a.post = const_cast<float*>(posteriors);
-  a.order = const_cast<int*>(order);
+  a.order = (int2*)const_cast<int32_t*>(order);
   a.dloss = dloss;
   a.dlogits = dlogits;
   return finish(launch_ctc_grad(a, dtype, (cudaStream_t)stream), name);

@@ -126,12 +126,14 @@ __device__ __forceinline__ Online scan_row(const T* __restrict__ x, int V, int t
     online_eight(o, f);
   }
   for (int v = head + vecs * 8 + tid; v < V; v += THREADS) online_one(o, to_f32(x[v]));
+  // one rescaling to the warp's largest, then plain sums
+  float top = o.top;
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    const Online other{__shfl_xor_sync(0xffffffffu, o.top, d), __shfl_xor_sync(0xffffffffu, o.sum, d)};
-    o = online_join(o, other);
-  }
-  return o;
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  float sum = o.top == top ? o.sum : o.top == -INFINITY ? o.sum : o.sum * ex2_approx((o.top - top) * kLog2e);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  return Online{top, sum};
 }
 
 // The transcript's places in the order of their labels (the blank's own place, number S, among them), so that the
@@ -140,63 +142,100 @@ __device__ __forceinline__ void plan_utterance(const CtcArgs& a, int b) {
   const int len = __ldg(a.target_lengths + b);
   const bool fits = len >= 0 && len <= a.S;
   const int* targets = a.targets + (int64_t)b * a.S;
-  int* order = a.order + (int64_t)b * a.pitch;
+  int2* order = a.order + (int64_t)b * a.pitch;
   int bad = !fits;
   const int count = fits ? len + 1 : 0;          // entry len: the blank
+  __shared__ int labels[kMaxCtcLabels + 1];
+  for (int i = threadIdx.x; i < count; i += blockDim.x) labels[i] = i < len ? __ldg(targets + i) : a.blank;
+  __syncthreads();
   for (int i = threadIdx.x; i < count; i += blockDim.x) {
-    const int v = i < len ? __ldg(targets + i) : a.blank;
+    const int v = labels[i];
     bad |= v < 0 || v >= a.V;
     int rank = 0;
-    for (int j = 0; j < count; ++j) {
-      const int u = j < len ? __ldg(targets + j) : a.blank;
-      rank += u < v || (u == v && j < i);
-    }
-    order[rank] = i < len ? i : a.S;
+    for (int j = 0; j < i; ++j) rank += labels[j] <= v;
+    for (int j = i + 1; j < count; ++j) rank += labels[j] < v;
+    order[rank] = make_int2(i < len ? i : a.S + 1, v);           // where its posterior lies, its class
   }
   bad = __syncthreads_or(bad);
   if (threadIdx.x == 0) a.bad[b] = bad;
 }
 
-// 2^l as a stored word, for l <= 0 = a / ln 2
-__device__ __forceinline__ uint32_t emission_word(float a, float& l) {
-  constexpr double log2e = 1.4426950408889634;
-  constexpr float hi = (float)log2e, lo = (float)(log2e - (double)hi);
-  l = a * hi;
-  if (!(l >= -1000.f)) return 0u;                // impossible (NaN: the frame's sum tells)
-  const float k = rintf(l);
-  // the fraction from 1 / ln 2 in two parts: one rounding near zero instead of one near |l|
-  return to_word(ex2_approx(fmaf(a, lo, fmaf(a, hi, -k))), (int)k);
+// exp(a) as a stored word, for a <= 0; 0 (impossible) below kLowest and for NaN (the frame's sum tells of it)
+constexpr float kLowest = -690.f;
+__device__ __forceinline__ uint32_t emission_word(float a) {
+  const float r = fmaf(a, kLog2e, 12582912.f);   // 1.5 * 2^23: the nearest integer of a / ln 2 in the low bits
+  const float f = fmaf(a, kLog2e, 12582912.f - r);
+  const uint32_t v = ((__float_as_uint(ex2_approx(f)) + 4u) >> 3) + (__float_as_uint(r) << 20) + (896u << 20);
+  return a >= kLowest ? v : 0u;
 }
 
-// Emission words of one frame: labels at [0, len), a zero at S, the blank at S + 1, and at S + 2 how many octaves the
-// least of them lies below the likeliest.  Returns that one's logit (one warp, the same in every lane).
-template <typename T>
-__device__ __forceinline__ float write_emissions(const CtcArgs& a, const T* x, int64_t frame, int b, int lane) {
+// Emission words of F frames that follow one another (frame, x: of the first; count <= F of them are there): labels at
+// [0, len), a zero at S, the blank at S + 1, and at S + 2 how many octaves the least of them lies below the likeliest.
+// best[f]: the likeliest one's logit.  One warp; a label is looked up once for all its frames, and the first 32 KEEP
+// labels' logits stay in registers between the two passes.
+template <typename T, int F, int KEEP>
+__device__ __forceinline__ void write_emissions(const CtcArgs& a, const T* x, int64_t frame, int count, int b, int lane,
+                                                float (&best)[F]) {
   uint32_t* em = reinterpret_cast<uint32_t*>(a.post) + frame * a.pitch;
   const int len = min(max(__ldg(a.target_lengths + b), 0), a.S);
   const int* targets = a.targets + (int64_t)b * a.S;
-  auto logit = [&](int i) {
+  auto label = [&](int i) {
     const int v = i < len ? __ldg(targets + i) : a.blank;
-    return v >= 0 && v < a.V ? to_f32(x[v]) : -INFINITY;
+    return v < 0 || v >= a.V ? -1 : v;
   };
-  float best = -INFINITY;
-  for (int i = lane; i <= len; i += 32) best = fmaxf(best, logit(i));
+  auto logit = [&](int v, int f) { return v < 0 || f >= count ? -INFINITY : to_f32(x[f * a.ld_t + v]); };
+  float kept[KEEP][F], least[F];
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
-  float least = 0.f;
-  for (int i = lane; i <= len; i += 32) {
-    float l;
-    const uint32_t v = emission_word(logit(i) - best, l);
-    if (v) least = fminf(least, l);
-    em[i < len ? i : a.S + 1] = v;
+  for (int f = 0; f < F; ++f) {
+    best[f] = logit(a.blank, f);
+    least[f] = 0.f;
   }
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, d));
-  if (lane == 0) {
-    em[a.S] = 0u;
-    em[a.S + 2] = (uint32_t)(int)ceilf(-least);
+  for (int u = 0; u < KEEP; ++u)
+    if (u * 32 < len) {
+      const int v = u * 32 + lane < len ? label(u * 32 + lane) : -1;
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        kept[u][f] = logit(v, f);
+        best[f] = fmaxf(best[f], kept[u][f]);
+      }
+    }
+  for (int i = KEEP * 32 + lane; i < len; i += 32) {
+    const int v = label(i);
+#pragma unroll
+    for (int f = 0; f < F; ++f) best[f] = fmaxf(best[f], logit(v, f));
   }
-  return best;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1)
+#pragma unroll
+    for (int f = 0; f < F; ++f) best[f] = fmaxf(best[f], __shfl_xor_sync(0xffffffffu, best[f], d));
+  auto put = [&](int i, int f, float logit) {
+    const float x = logit - best[f];
+    if (x >= kLowest) least[f] = fminf(least[f], x);
+    em[(int64_t)f * a.pitch + i] = emission_word(x);
+  };
+#pragma unroll
+  for (int f = 0; f < F; ++f)
+    if (f < count) {
+#pragma unroll
+      for (int u = 0; u < KEEP; ++u)
+        if (u * 32 + lane < len) put(u * 32 + lane, f, kept[u][f]);
+      if (lane == 0) {
+        put(a.S + 1, f, logit(a.blank, f));
+        em[(int64_t)f * a.pitch + a.S] = 0u;
+      }
+    }
+  for (int i = KEEP * 32 + lane; i < len; i += 32) {
+    const int v = label(i);
+    for (int f = 0; f < count; ++f) put(i, f, logit(v, f));
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1)
+#pragma unroll
+    for (int f = 0; f < F; ++f) least[f] = fminf(least[f], __shfl_xor_sync(0xffffffffu, least[f], d));
+#pragma unroll
+  for (int f = 0; f < F; ++f)
+    if (lane == f && f < count) em[(int64_t)f * a.pitch + a.S + 2] = (uint32_t)(int)ceilf(-least[f] * kLog2e);
 }
 
 // what the frame adds to -log2 Z: its emissions are against `best` instead of the softmax's denominator
@@ -207,38 +246,44 @@ __device__ __forceinline__ float frame_norm(const Online& o, float best) {
 constexpr int kRowThreads = 256;
 constexpr int kWarpRowV = 2048;                  // up to it a warp takes a row, beyond it a CTA
 
+// Frames of one utterance that a warp takes: two, which share what is looked up of the transcript, where that leaves
+// 16 warps an SM; a CTA takes one.
+int warp_frames(const CtcArgs& a) { return (int64_t)a.B * a.T >= 32 * device_sm_count() ? 2 : 1; }
+
 // block (frames, utterance); the last block of an utterance plans it
-template <typename T, bool WARP_ROW>
+template <typename T, int F, bool WARP_ROW>
 __global__ void __launch_bounds__(kRowThreads) ctc_rows_kernel(CtcArgs a) {
   const int b = blockIdx.y;
   if (blockIdx.x == gridDim.x - 1) return plan_utterance(a, b);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t = WARP_ROW ? blockIdx.x * (kRowThreads / 32) + warp : blockIdx.x;
-  if (t >= min(__ldg(a.input_lengths + b), a.T)) return;
+  const int t = WARP_ROW ? (blockIdx.x * (kRowThreads / 32) + warp) * F : blockIdx.x;
+  const int count = min(min(__ldg(a.input_lengths + b), a.T) - t, F);
+  if (count <= 0) return;
   const T* x = static_cast<const T*>(a.logits) + b * a.ld_b + t * a.ld_t;
   const int64_t frame = (int64_t)b * a.T + t;
+  Online o[F];
   if (WARP_ROW) {
-    const Online o = scan_row<T, 32>(x, a.V, lane);
-    const float best = write_emissions(a, x, frame, b, lane);
-    if (lane == 0) {
-      a.stats[frame] = make_float2(o.top, o.sum);
-      a.norms[frame] = frame_norm(o, best);
-    }
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+      if (f < count) o[f] = scan_row<T, 32>(x + f * a.ld_t, a.V, lane);
   } else {
     __shared__ Online part[kRowThreads / 32];
-    Online o = scan_row<T, kRowThreads>(x, a.V, threadIdx.x);
-    if (lane == 0) part[warp] = o;
+    o[0] = scan_row<T, kRowThreads>(x, a.V, threadIdx.x);
+    if (lane == 0) part[warp] = o[0];
     __syncthreads();
     if (warp > 0) return;
-    o = part[0];
+    o[0] = part[0];
 #pragma unroll
-    for (int i = 1; i < kRowThreads / 32; ++i) o = online_join(o, part[i]);
-    const float best = write_emissions(a, x, frame, b, lane);
-    if (lane == 0) {
-      a.stats[frame] = make_float2(o.top, o.sum);
-      a.norms[frame] = frame_norm(o, best);
-    }
+    for (int i = 1; i < kRowThreads / 32; ++i) o[0] = online_join(o[0], part[i]);
   }
+  float best[F];
+  write_emissions<T, F, WARP_ROW ? 10 : 1>(a, x, frame, count, b, lane, best);
+#pragma unroll
+  for (int f = 0; f < F; ++f)
+    if (lane == f && f < count) {
+      a.stats[frame + f] = make_float2(o[f].top, o[f].sum);
+      a.norms[frame + f] = frame_norm(o[f], best[f]);
+    }
 }
 
 // ---- lattice ---------------------------------------------------------------------------------------------------------
@@ -739,21 +784,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 
 }
 
 // ---- gradient --------------------------------------------------------------------------------------------------------
-// A frame's d p everywhere, then d (p - posterior) over the classes of the transcript.  `tid` of `threads` work on the
-// frame; `sync` orders the two.
-template <typename T, int THREADS, typename Sync>
-__device__ __forceinline__ void grad_row(const CtcArgs& a, const T* __restrict__ x, T* __restrict__ g, int64_t frame,
-                                         int b, int tid, Sync sync) {
+// What a frame's gradient is made of: d p = scale * 2^((logit - top) / ln 2).
+struct FrameGrad {
+  float top, scale, d;
+  __device__ __forceinline__ float operator()(float x) const { return scale * ex2_approx((x - top) * kLog2e); }
+};
+
+__device__ __forceinline__ FrameGrad frame_grad(const CtcArgs& a, int64_t frame, int b) {
   const float2 st = a.stats[frame];
-  const float d = __ldg(a.dloss + b), f = d / st.y;
-  const int V = a.V;
-  auto value = [&](float v) { return f * ex2_approx((v - st.x) * kLog2e); };
+  const float d = __ldg(a.dloss + b);
+  return FrameGrad{st.x, d / st.y, d};
+}
+
+// d p over all classes of a frame
+template <typename T, int THREADS>
+__device__ __forceinline__ void grad_row(const FrameGrad& p, const T* __restrict__ x, T* __restrict__ g, int V, int tid) {
   int head = head_of(g, V), vecs = (V - head) / 8;
   if (((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(g)) & 15) != 0) {
     head = V;                                      // another alignment than the gradient's: element by element
     vecs = 0;
   }
-  for (int v = tid; v < head; v += THREADS) g[v] = from_f32<T>(value(to_f32(x[v])));
+  for (int v = tid; v < head; v += THREADS) g[v] = from_f32<T>(p(to_f32(x[v])));
   for (int i = tid; i < vecs; i += THREADS) {
     rows_impl::Vec8<T> r;
 #pragma unroll
@@ -762,50 +813,55 @@ __device__ __forceinline__ void grad_row(const CtcArgs& a, const T* __restrict__
     float e[8];
     rows_impl::unpack(r, e);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) e[k] = value(e[k]);
+    for (int k = 0; k < 8; ++k) e[k] = p(e[k]);
     rows_impl::pack(e, r);
 #pragma unroll
     for (int q = 0; q < rows_impl::Vec8<T>::Q; ++q)
       *(reinterpret_cast<uint4*>(g + head + (int64_t)i * 8) + q) = r.q[q];
   }
-  for (int v = head + vecs * 8 + tid; v < V; v += THREADS) g[v] = from_f32<T>(value(to_f32(x[v])));
-  sync();
-  if (tid >= 32) return;
-  // the posteriors in the order of their classes: a running sum within each class, its last place writes
+  for (int v = head + vecs * 8 + tid; v < V; v += THREADS) g[v] = from_f32<T>(p(to_f32(x[v])));
+}
+
+// d (p - posterior) over the transcript's classes of `count` frames that follow one another: the posteriors in the
+// order of their classes, a running sum within each class, its last place writes.  One warp; the order is looked up
+// once for all frames.
+template <typename T, int F>
+__device__ __forceinline__ void grad_labels(const CtcArgs& a, const FrameGrad (&p)[F], const T* __restrict__ x,
+                                            T* __restrict__ g, int64_t frame, int count, int b, int lane) {
   const float* post = a.post + frame * a.pitch;
-  const int* order = a.order + (int64_t)b * a.pitch;
-  const int* targets = a.targets + (int64_t)b * a.S;
-  const int count = __ldg(a.target_lengths + b) + 1;
-  float carry = 0.f;
+  const int2* order = a.order + (int64_t)b * a.pitch;
+  const int places = __ldg(a.target_lengths + b) + 1;
+  const int2 none = make_int2(-1, -2);
+  float carry[F] = {};
   int carry_v = -1;
-  for (int q0 = 0; q0 < count; q0 += 32) {
-    const int q = q0 + tid;
-    int v = -2;
-    float s = 0.f;
-    if (q < count) {
-      const int i = __ldg(order + q);
-      v = i == a.S ? a.blank : __ldg(targets + i);
-      s = post[i == a.S ? a.S + 1 : i];
+  int2 here = lane < places ? __ldg(order + lane) : none;
+  for (int q0 = 0; q0 < places; q0 += 32) {
+    const int q = q0 + lane;
+    const int2 ahead = q + 32 < places ? __ldg(order + q + 32) : none;
+    const int v = here.y;
+    int next = __shfl_down_sync(0xffffffffu, v, 1);
+    const int first_ahead = __shfl_sync(0xffffffffu, ahead.y, 0);
+    if (lane == 31) next = first_ahead;
+    const bool last = here.x >= 0 && next != v;
+    float joins[6];                                // 1 where the value that far below is of the same class
+    joins[5] = v == carry_v ? 1.f : 0.f;
+#pragma unroll
+    for (int k = 0; k < 5; ++k) {                  // sorted: equal 2^k below means one class in between
+      const int uv = __shfl_up_sync(0xffffffffu, v, 1 << k);
+      joins[k] = lane >= (1 << k) && uv == v ? 1.f : 0.f;
     }
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const float us = __shfl_up_sync(0xffffffffu, s, o);
-      const int uv = __shfl_up_sync(0xffffffffu, v, o);
-      if (tid >= o && uv == v) s += us;            // sorted: equal o below means one class in between
+    for (int f = 0; f < F; ++f) {
+      if (f >= count) break;
+      float s = here.x < 0 ? 0.f : post[(int64_t)f * a.pitch + here.x];
+#pragma unroll
+      for (int k = 0; k < 5; ++k) s = fmaf(joins[k], __shfl_up_sync(0xffffffffu, s, 1 << k), s);
+      s = fmaf(joins[5], carry[f], s);
+      if (last) g[(int64_t)f * a.V + v] = from_f32<T>(p[f](to_f32(x[f * a.ld_t + v])) - p[f].d * s);
+      carry[f] = __shfl_sync(0xffffffffu, s, 31);
     }
-    if (v == carry_v) s += carry;
-    const int above = __shfl_down_sync(0xffffffffu, v, 1);
-    int next = above;
-    if (tid == 31) {
-      next = -3;
-      if (q + 1 < count) {
-        const int i = __ldg(order + q + 1);
-        next = i == a.S ? a.blank : __ldg(targets + i);
-      }
-    }
-    if (v >= 0 && next != v) g[v] = from_f32<T>(value(to_f32(x[v])) - d * s);
-    carry = __shfl_sync(0xffffffffu, s, 31);
     carry_v = __shfl_sync(0xffffffffu, v, 31);
+    here = ahead;
   }
 }
 
@@ -823,27 +879,40 @@ __device__ __forceinline__ void fill_row(T* __restrict__ g, int V, float value, 
   for (int v = head + vecs * 8 + tid; v < V; v += THREADS) g[v] = from_f32<T>(value);
 }
 
-template <typename T, bool WARP_ROW>
+template <typename T, int F, bool WARP_ROW>
 __global__ void __launch_bounds__(kRowThreads) ctc_grad_kernel(CtcArgs a) {
   constexpr int THREADS = WARP_ROW ? 32 : kRowThreads;
   const int b = blockIdx.y;
-  const int t = WARP_ROW ? blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5) : blockIdx.x;
+  const int t = WARP_ROW ? (blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5)) * F : blockIdx.x;
   if (t >= a.T) return;
   const int tid = WARP_ROW ? threadIdx.x & 31 : threadIdx.x;
   const int64_t frame = (int64_t)b * a.T + t;
+  const T* x = static_cast<const T*>(a.logits) + b * a.ld_b + t * a.ld_t;
   T* g = static_cast<T*>(a.dlogits) + frame * a.V;
   const int n = __ldg(a.input_lengths + b);
   const float raw = __ldg(a.raw_loss + b);
-  const bool nan = raw != raw || (raw == INFINITY && !a.zero_infinity);
-  const bool padding = t >= n && n >= 0 && n <= a.T;
-  if (padding || nan || raw == INFINITY) return fill_row<T, THREADS>(g, a.V, !padding && nan ? NAN : 0.f, tid);
-  const T* x = static_cast<const T*>(a.logits) + b * a.ld_b + t * a.ld_t;
-  grad_row<T, THREADS>(a, x, g, frame, b, tid, [] {
-    if (WARP_ROW)
-      __syncwarp();
-    else
-      __syncthreads();
-  });
+  // frames of the utterance: a gradient where there is a finite loss, else zeros or NaN; behind it zeros.  A length out
+  // of range makes all its frames NaN.
+  const bool fits = n >= 0 && n <= a.T, finite = fabsf(raw) < INFINITY;
+  const float other = raw == INFINITY && a.zero_infinity ? 0.f : NAN;
+  const int count = fits ? min(n - t, F) : F;      // frames of the F that are not padding
+  FrameGrad p[F];
+#pragma unroll
+  for (int f = 0; f < F; ++f) {
+    if (t + f >= a.T) break;
+    if (f < count && finite) {
+      p[f] = frame_grad(a, frame + f, b);
+      grad_row<T, THREADS>(p[f], x + f * a.ld_t, g + (int64_t)f * a.V, a.V, tid);
+    } else {
+      fill_row<T, THREADS>(g + (int64_t)f * a.V, a.V, f < count ? other : 0.f, tid);
+    }
+  }
+  if (!finite || count <= 0) return;
+  if (WARP_ROW)
+    __syncwarp();
+  else
+    __syncthreads();
+  if (tid < 32) grad_labels<T, F>(a, p, x, g, frame, count, b, tid);
 }
 
 template <int NP, int H, int NBUF, bool GRAD>
@@ -898,11 +967,14 @@ template <typename T>
 int launch_loss(const CtcArgs& a, cudaStream_t stream) {
   for (int b0 = 0; b0 < a.B; b0 += 65535) {
     const CtcArgs c = batch_part(a, b0, sizeof(T));
-    constexpr int per = kRowThreads / 32;
-    if (a.V <= kWarpRowV)
-      ctc_rows_kernel<T, true><<<dim3((a.T + per - 1) / per + 1, c.B), kRowThreads, 0, stream>>>(c);
+    const int frames = warp_frames(a), per = kRowThreads / 32 * frames;
+    const dim3 warp_grid((a.T + per - 1) / per + 1, c.B);
+    if (a.V > kWarpRowV)
+      ctc_rows_kernel<T, 1, false><<<dim3(a.T + 1, c.B), kRowThreads, 0, stream>>>(c);
+    else if (frames == 2)
+      ctc_rows_kernel<T, 2, true><<<warp_grid, kRowThreads, 0, stream>>>(c);
     else
-      ctc_rows_kernel<T, false><<<dim3(a.T + 1, c.B), kRowThreads, 0, stream>>>(c);
+      ctc_rows_kernel<T, 1, true><<<warp_grid, kRowThreads, 0, stream>>>(c);
     if (cudaError_t e = cudaGetLastError()) return (int)e;
     if (int rc = c.states ? launch_lattice_for<true>(c, stream) : launch_lattice_for<false>(c, stream)) return rc;
   }
@@ -913,11 +985,14 @@ template <typename T>
 int launch_grad(const CtcArgs& a, cudaStream_t stream) {
   for (int b0 = 0; b0 < a.B; b0 += 65535) {
     const CtcArgs c = batch_part(a, b0, sizeof(T));
-    constexpr int per = kRowThreads / 32;
-    if (a.V <= kWarpRowV)
-      ctc_grad_kernel<T, true><<<dim3((a.T + per - 1) / per, c.B), kRowThreads, 0, stream>>>(c);
+    const int frames = warp_frames(a), per = kRowThreads / 32 * frames;
+    const dim3 warp_grid((a.T + per - 1) / per, c.B);
+    if (a.V > kWarpRowV)
+      ctc_grad_kernel<T, 1, false><<<dim3(a.T, c.B), kRowThreads, 0, stream>>>(c);
+    else if (frames == 2)
+      ctc_grad_kernel<T, 2, true><<<warp_grid, kRowThreads, 0, stream>>>(c);
     else
-      ctc_grad_kernel<T, false><<<dim3(a.T, c.B), kRowThreads, 0, stream>>>(c);
+      ctc_grad_kernel<T, 1, true><<<warp_grid, kRowThreads, 0, stream>>>(c);
     if (cudaError_t e = cudaGetLastError()) return (int)e;
   }
   return 0;

@@ -196,7 +196,7 @@ struct CtcArgs {
   int state_pitch = 0;           // ctc_state_pitch(S)
   float2* stats = nullptr;       // [B, T] (largest logit, sum of exp(logit - largest))
   float* post = nullptr;         // [B, T, pitch]: emission words, then posteriors, of the labels; blank's at S + 1
-  int* order = nullptr;          // [B, pitch] the transcript's places in the order of their labels
+  int2* order = nullptr;         // [B, pitch] (place in post, class) in the order of the classes
   float* raw_loss = nullptr;     // [B] loss, inf where no path exists, NaN for bad input
   float* loss = nullptr;         // [B] loss with zero_infinity applied
   int* bad = nullptr;            // workspace [B]: a length or label out of range

@@ -415,7 +415,7 @@ def _ctc_loss(logits, targets, input_lengths, target_lengths, blank, zero_infini
     stats = torch.empty((B, T, 2), dtype=torch.float32, device=dev)
     pitch = _ctc_pitch(S)
     post = torch.empty((B, T, pitch), dtype=torch.float32, device=dev)
-    order = torch.empty((B, pitch), dtype=torch.int32, device=dev)
+    order = torch.empty((B, pitch, 2), dtype=torch.int32, device=dev)
     with _on(dev):
         x, sb, st, (tg, il, tl) = _ctc_operands(logits, targets, input_lengths, target_lengths)
         nbytes = _lib.lib().gsn_ctc_loss_workspace_bytes(B, T, S, int(gradient))
@@ -437,7 +437,7 @@ def _ctc_loss_backward(dloss, logits, targets, input_lengths, target_lengths, ra
         raise RuntimeError(f"{name}: dloss must be [{B}], got {tuple(dloss.shape)}")
     pitch = _ctc_pitch(S)
     kept = ((raw, (B,), torch.float32), (stats, (B, T, 2), torch.float32), (post, (B, T, pitch), torch.float32),
-            (order, (B, pitch), torch.int32))
+            (order, (B, pitch, 2), torch.int32))
     if any(t.shape != shape or t.dtype != dtype or not t.is_contiguous() for t, shape, dtype in kept):
         raise RuntimeError(f"{name}: raw_loss, stats, posteriors and order must be the outputs of granite::ctc_loss "
                            f"for logits {(B, T, V)} and targets {(B, S)}")
@@ -457,7 +457,7 @@ def ctc_loss_op(logits: torch.Tensor, targets: torch.Tensor, input_lengths: torc
                 target_lengths: torch.Tensor, blank: int, zero_infinity: bool
                 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(loss [B] fp32, and what the gradient needs: raw_loss [B], stats [B, T, 2], posteriors [B, T, P] fp32 and order
-    [B, P] int32, P = S + 3 rounded up to four)."""
+    [B, P, 2] int32, P = S + 3 rounded up to four)."""
     return _ctc_loss(logits, targets, input_lengths, target_lengths, blank, zero_infinity, True)
 
 
@@ -467,7 +467,7 @@ def _(logits, targets, input_lengths, target_lengths, blank, zero_infinity):
     f = dict(dtype=torch.float32)
     pitch = _ctc_pitch(targets.shape[1])
     return (logits.new_empty((B,), **f), logits.new_empty((B,), **f), logits.new_empty((B, T, 2), **f),
-            logits.new_empty((B, T, pitch), **f), logits.new_empty((B, pitch), dtype=torch.int32))
+            logits.new_empty((B, T, pitch), **f), logits.new_empty((B, pitch, 2), dtype=torch.int32))
 
 
 @torch.library.custom_op("granite::ctc_loss_backward", mutates_args=(), device_types="cuda")

@@ -401,7 +401,7 @@ int gsn_dropout_add_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* dh
  * gsn_ctc_loss_fwd: loss[b] = -log p(targets[b, :target_lengths[b]] | softmax(logits[b, :input_lengths[b]])), inf where
  *   no alignment exists (0 with zero_infinity), NaN where a length lies outside [0, T] or [0, S], a label outside
  *   [0, V), or a valid frame holds NaN, +inf or nothing but -inf.  raw_loss [B], stats [B, T, 2], posteriors [B, T, P]
- *   (fp32; P = gsn_ctc_loss_pitch(S)) and order (int32 [B, P]) are buffers that the backward pass reads; it may be
+ *   (fp32; P = gsn_ctc_loss_pitch(S)) and order (int32 [B, P, 2]) are buffers that the backward pass reads; it may be
  *   called after a forward pass with gradient != 0.  A class of the transcript, the blank among them, whose logit lies
  *   more than 690 below the largest of them counts as impossible in that frame.
  *   workspace: gsn_ctc_loss_workspace_bytes(B, T, S, gradient) bytes, 16-byte aligned.

@@ -322,6 +322,13 @@ def test_ctc_loss(B, T, V, S, dtype):
     check_ctc(*ctc_case(B * 1000 + T, B, T, V, S, dtype))
 
 
+@pytest.mark.parametrize("S", [79, 80, 207, 208, 329, 330, 900, 967, 968])
+def test_ctc_label_counts(S):
+    """Around the counts where a lane holds more of them or a block fewer frames; long and short chains beside them."""
+    il, tl = [2 * S + 40, S + 30, 17], [S, S // 3, 5]
+    check_ctc(*ctc_case(100 + S, 3, 2 * S + 40, 50, S, BF, (il, tl)))
+
+
 def test_ctc_ragged_batch_and_padding():
     """Lengths from zero up, with garbage behind them, and the blank inside the vocabulary."""
     il, tl = [40, 13, 1, 0, 25, 0], [12, 6, 1, 0, 0, 2]

@@ -98,27 +98,34 @@ def ctc_one(logits, target, blank):
         return (0.0 if L == 1 else math.inf), np.zeros((0, V))
     top = x.max(1, keepdims=True)
     logp = x - top - np.log(np.exp(x - top).sum(1, keepdims=True))
-    skip = [s >= 2 and states[s] != blank and states[s] != states[s - 2] for s in range(L)]
+    lab = np.asarray(states)
+    em = logp[:, lab]
+    skip = np.zeros(L, dtype=bool)
+    skip[2:] = (lab[2:] != blank) & (lab[2:] != lab[:-2])
+
+    def shifted(v, by, keep):
+        """v moved up (by > 0) or down the states, -inf coming in; only where `keep`."""
+        out = np.full(L, -math.inf)
+        if by > 0:
+            out[by:] = v[:-by] if L > by else []
+        else:
+            out[:by] = v[-by:] if L > -by else []
+        return np.where(keep, out, -math.inf)
+
     alpha = np.full((n, L), -math.inf)
-    alpha[0, 0] = logp[0, states[0]]
-    if L > 1:
-        alpha[0, 1] = logp[0, states[1]]
+    alpha[0, :2] = em[0, :2]
     for t in range(1, n):
-        for s in range(L):
-            alpha[t, s] = logp[t, states[s]] + _logsum([alpha[t - 1, s]] + ([alpha[t - 1, s - 1]] if s else [])
-                                                       + ([alpha[t - 1, s - 2]] if skip[s] else []))
+        a = alpha[t - 1]
+        alpha[t] = em[t] + np.logaddexp(np.logaddexp(a, shifted(a, 1, True)), shifted(a, 2, skip))
     logz = _logsum([alpha[-1, -1]] + ([alpha[-1, -2]] if L > 1 else []))
     if logz == -math.inf:
         return math.inf, None
     beta = np.full((n, L), -math.inf)
-    beta[-1, -1] = 0.0
-    if L > 1:
-        beta[-1, -2] = 0.0
+    beta[-1, -2:] = 0.0
+    jump = np.append(skip[2:], [False] * min(2, L))[:L]
     for t in range(n - 2, -1, -1):
-        q = [beta[t + 1, s] + logp[t + 1, states[s]] for s in range(L)]
-        for s in range(L):
-            beta[t, s] = _logsum([q[s]] + ([q[s + 1]] if s + 1 < L else [])
-                                 + ([q[s + 2]] if s + 2 < L and skip[s + 2] else []))
+        q = beta[t + 1] + em[t + 1]
+        beta[t] = np.logaddexp(np.logaddexp(q, shifted(q, -1, True)), shifted(q, -2, jump))
     gamma = np.exp(alpha + beta - logz)
     grad = np.exp(logp)
     for s in range(L):
