@@ -51,7 +51,8 @@ void set_dropout(RowArgs& a, const int64_t* rng, uint32_t site, double p, double
   a.rng = rng;
   a.site = site;
   a.threshold = (uint32_t)nearbyint(p * 65536.0);
-  a.factor = a.threshold < 65536u ? (float)(scale * 65536.0 / (65536.0 - a.threshold)) : 0.f;
+  a.drop_all = a.threshold > 65535u;
+  a.factor = !a.drop_all ? (float)(scale * 65536.0 / (65536.0 - a.threshold)) : 0.f;
 }
 
 RowArgs row_args(int64_t M, int D, float eps, const int32_t* lengths, int T, int param_dtype) {

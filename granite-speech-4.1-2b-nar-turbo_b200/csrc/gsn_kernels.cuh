@@ -171,6 +171,7 @@ struct RowArgs {
   int64_t partial_rows = 0;      // row_partial_rows(M, D)
   const int64_t* rng = nullptr;  // device (seed, offset)
   uint32_t site = 0, threshold = 0;   // an element is dropped where its 16-bit number is below the threshold
+  int drop_all = 0;              // threshold 65536
   float factor = 1.f;            // a kept element is multiplied by it
   const int* lengths = nullptr;  // [M / T] or null
   int64_t M = 0;

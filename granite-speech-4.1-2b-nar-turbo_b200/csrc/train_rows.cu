@@ -83,24 +83,37 @@ __device__ __forceinline__ void pack(const float (&f)[8], Vec8<float>& r) {
                         __float_as_uint(f[4 * k + 3]));
 }
 
-// Columns [col, col + 8) of a row of D elements; columns past D read as zero.  VEC: D % 8 == 0 and 16-byte rows.
+// A warp's block of 256 columns: lane l holds eight of them.  VEC (rows aligned to 16 bytes, D % 8 == 0): columns
+// 8 l .. 8 l + 7, one 16-byte word of a 16-bit type.  Otherwise columns l + 32 k, so that single elements still make
+// whole 32-byte sectors (eight neighbours a lane cost 8 times the L2 writes: 80 -> 23 us at 11376 x 1001 fp16).
+template <bool VEC>
+__device__ __forceinline__ int column(int base, int lane, int k) {
+  return VEC ? base + lane * 8 + k : base + k * 32 + lane;
+}
+
+// columns past D read as zero
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* __restrict__ row, int col, int D, Vec8<T>& r) {
+__device__ __forceinline__ void load8(const T* __restrict__ row, int base, int lane, int D, Vec8<T>& r) {
   if (VEC) {
+    const int col = base + lane * 8;
 #pragma unroll
     for (int i = 0; i < Vec8<T>::Q; ++i)
       r.q[i] = col < D ? __ldg(reinterpret_cast<const uint4*>(row + col) + i) : make_uint4(0, 0, 0, 0);
   } else {
     float f[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = col + k < D ? to_f32(row[col + k]) : 0.f;
+    for (int k = 0; k < 8; ++k) {
+      const int col = column<VEC>(base, lane, k);
+      f[k] = col < D ? to_f32(row[col]) : 0.f;
+    }
     pack(f, r);                     // exact: the values are of type T
   }
 }
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* __restrict__ row, int col, int D, const float (&f)[8]) {
+__device__ __forceinline__ void store8(T* __restrict__ row, int base, int lane, int D, const float (&f)[8]) {
   if (VEC) {
+    const int col = base + lane * 8;
     if (col >= D) return;
     Vec8<T> r;
     pack(f, r);
@@ -108,20 +121,58 @@ __device__ __forceinline__ void store8(T* __restrict__ row, int col, int D, cons
     for (int i = 0; i < Vec8<T>::Q; ++i) *(reinterpret_cast<uint4*>(row + col) + i) = r.q[i];
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (col + k < D) row[col + k] = from_f32<T>(f[k]);
+    for (int k = 0; k < 8; ++k) {
+      const int col = column<VEC>(base, lane, k);
+      if (col < D) row[col] = from_f32<T>(f[k]);
+    }
   }
 }
 
-// Weight or bias columns [col, col + 8) as fp32; `fp32`: stored as fp32, else as T.
-template <typename T>
-__device__ __forceinline__ void load_param8(const void* p, int fp32, int col, int D, float (&f)[8]) {
+// The lane's columns of weight or bias as fp32; `fp32`: stored as fp32, else as T.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_param8(const void* p, int fp32, int base, int lane, int D, float (&f)[8]) {
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const int c = col + k;
+    const int c = column<VEC>(base, lane, k);
     f[k] = c >= D ? 0.f : fp32 ? __ldg(static_cast<const float*>(p) + c) : to_f32(static_cast<const T*>(p)[c]);
   }
 }
+
+__device__ __forceinline__ void copy16(void* smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(gmem) : "memory");
+}
+
+// Rows under way: each thread copies the 16-byte words that it will itself read, some rows ahead, so the loads need
+// neither registers nor a barrier.  TENSORS inputs of NV vectors a lane; slots [stage][tensor][vector][word][thread].
+template <typename T, int NV, int TENSORS>
+struct Ring {
+  static constexpr int Q = Vec8<T>::Q, WORDS = TENSORS * NV * Q;
+  uint4* slots;                                    // shared memory, stages * WORDS * blockDim.x
+  __device__ __forceinline__ uint4* at(int stage, int tensor, int i) const {
+    return slots + ((stage * TENSORS + tensor) * NV + i) * Q * blockDim.x + threadIdx.x;
+  }
+  __device__ __forceinline__ void fetch(int stage, int tensor, int i, const T* row, int col, int D) const {
+    uint4* dst = at(stage, tensor, i);
+    if (col < D)
+#pragma unroll
+      for (int q = 0; q < Q; ++q) copy16(dst + q * blockDim.x, reinterpret_cast<const uint4*>(row + col) + q);
+  }
+  __device__ __forceinline__ void read(int stage, int tensor, int i, Vec8<T>& r) const {
+    const uint4* src = at(stage, tensor, i);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) r.q[q] = src[q * blockDim.x];
+  }
+  // columns past D are never copied: zeros, once
+  __device__ __forceinline__ void clear(int stages) const {
+    for (int i = 0; i < stages * WORDS; ++i) slots[i * blockDim.x + threadIdx.x] = make_uint4(0, 0, 0, 0);
+  }
+};
+
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
 // ---- the dropout generator -------------------------------------------------------------------------------------------
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", SC 2011).  One call gives
@@ -154,15 +205,34 @@ __device__ __forceinline__ Generator load_generator(const int64_t* rng, uint32_t
   return Generator{(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)offset, site};
 }
 
-// bit j: element j of the group is kept (its 16-bit number is not below the threshold)
-__device__ __forceinline__ uint32_t keep_bits(const Generator& g, uint64_t group, uint32_t threshold) {
+// bit j: element j of the group is kept (its 16-bit number is not below the threshold, given shifted up by 16)
+__device__ __forceinline__ uint32_t keep_bits(const Generator& g, uint64_t group, uint32_t threshold16) {
   const uint4 r = philox(g, group);
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
   uint32_t bits = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    if ((w[k] & 0xFFFFu) >= threshold) bits |= 1u << (2 * k);
-    if ((w[k] >> 16) >= threshold) bits |= 2u << (2 * k);
+    bits |= (w[k] << 16) >= threshold16 ? 1u << (2 * k) : 0u;
+    bits |= w[k] >= threshold16 ? 2u << (2 * k) : 0u;
+  }
+  return bits;
+}
+
+// The keep bits of a lane's elements of NV blocks, eight a block: bit 8 i + k.  The generator's groups are neighbours,
+// so without VEC a lane's elements belong to eight groups, drawn by eight lanes.
+template <int NV, bool VEC>
+__device__ __forceinline__ uint32_t keep_row(const Generator& g, uint64_t row_group, const int (&base)[NV], int lane,
+                                             uint32_t threshold16) {
+  static_assert(NV <= 4, "eight bits a block in one word");
+  uint32_t own = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) own |= keep_bits(g, row_group + (base[i] >> 3) + lane, threshold16) << (8 * i);
+  if (VEC) return own;
+  uint32_t bits = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {                    // column base + 32 k + lane: group 4 k + lane / 8, its bit lane % 8
+    const uint32_t w = __shfl_sync(0xffffffffu, own, 4 * k + (lane >> 3)) >> (lane & 7);
+    bits |= (w & 0x01010101u) << k;
   }
   return bits;
 }
@@ -206,65 +276,103 @@ __device__ __forceinline__ bool padding_row(const RowArgs& a, int row) {
   return row - b * a.T >= __ldg(a.lengths + b);
 }
 
-// LayerNorm forward; DROP: of h = residual + dropout(x), which is stored too.  W warps a row, NV vectors of eight
-// columns a lane: a row stays in registers between the two passes of its statistics.
+// Rows under way a warp: what the SM's shared memory holds for two CTAs (forward, short rows) or one.
+__host__ __device__ constexpr int ring_stages(int words) { return words <= 4 ? 4 : words <= 16 ? 3 : 2; }
+
+// LayerNorm forward; DROP: of h = residual + dropout(x), which is stored too.  W warps a row, NV blocks of 256 columns
+// a warp: a row stays in registers between the two passes of its statistics, its weights for all rows of the warp.
 template <typename T, int NV, bool VEC, bool DROP>
-__global__ void __launch_bounds__(256) ln_fwd_kernel(RowArgs a) {
+__global__ void __launch_bounds__(256, 2) ln_fwd_kernel(RowArgs a) {
   __shared__ float2 exchange[8][2 * kMaxRowWarps];
+  extern __shared__ uint4 ring_slots[];
+  constexpr int TENSORS = DROP ? 2 : 1, S = ring_stages(Ring<T, NV, TENSORS>::WORDS);
+  const Ring<T, NV, TENSORS> ring{ring_slots};
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W, R = (blockDim.x >> 5) / W;
   const int group = warp / W;
   RowGroup rg{W, warp - group * W, 1 + group, exchange[group], 0};
   const int D = a.D;
-  int col[NV];
+  int base[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) base[i] = (i * W + rg.sub) * 256;
+  const int64_t stride = (int64_t)gridDim.x * R, first = (int64_t)blockIdx.x * R + group;
+  auto fetch = [&](int64_t row, int stage) {
+    if (VEC && row < a.M) {
+      const bool pad = padding_row(a, (int)row);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = base[i] + lane * 8;
+        if (!pad && !(DROP && a.drop_all)) ring.fetch(stage, 0, i, static_cast<const T*>(a.x) + row * a.ld_x, col, D);
+        if (DROP) ring.fetch(stage, 1, i, static_cast<const T*>(a.residual) + row * a.ld_res, col, D);
+      }
+    }
+    copies_commit();
+  };
+  if (VEC) {
+    ring.clear(S);
+#pragma unroll
+    for (int s = 0; s + 1 < S; ++s) fetch(first + s * stride, s);
+  }
   float wv[NV][8], bv[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    col[i] = ((i * W + rg.sub) * 32 + lane) * 8;
-    load_param8<T>(a.weight, a.param_fp32, col[i], D, wv[i]);
-    load_param8<T>(a.bias, a.param_fp32, col[i], D, bv[i]);
+    load_param8<T, VEC>(a.weight, a.param_fp32, base[i], lane, D, wv[i]);
+    load_param8<T, VEC>(a.bias, a.param_fp32, base[i], lane, D, bv[i]);
   }
   Generator gen{};
   if (DROP) gen = load_generator(a.rng, a.site);
   const float inv_d = 1.0f / D;
-  for (int64_t row = (int64_t)blockIdx.x * R + group; row < a.M; row += (int64_t)gridDim.x * R) {
+  int stage = 0;
+  for (int64_t row = first; row < a.M; row += stride) {
     T* y = static_cast<T*>(a.y) + row * D;
     T* h = DROP ? static_cast<T*>(a.h_out) + row * D : nullptr;
     const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
     const T* res = DROP ? static_cast<const T*>(a.residual) + row * a.ld_res : nullptr;
     const bool pad = padding_row(a, (int)row);
+    if (VEC) {
+      fetch(row + (S - 1) * stride, stage == 0 ? S - 1 : stage - 1);
+      copies_wait<S - 1>();
+    }
     float v[NV][8];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
+    auto input = [&](int tensor, const T* p, int i, float (&f)[8]) {
       Vec8<T> r;
-      if (DROP) {
-        load8<T, VEC>(res, col[i], D, r);
-        unpack(r, v[i]);
-        if (!pad) {
+      if (VEC)
+        ring.read(stage, tensor, i, r);
+      else
+        load8<T, VEC>(p, base[i], lane, D, r);
+      unpack(r, f);
+    };
+    if (DROP) {
+      uint32_t keep = 0;
+      if (!pad && !a.drop_all)
+        keep = keep_row<NV, VEC>(gen, (uint64_t)row * a.groups, base, lane, a.threshold << 16);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        input(1, res, i, v[i]);
+        if (!pad && !a.drop_all) {
           float f[8];
-          load8<T, VEC>(x, col[i], D, r);
-          unpack(r, f);
-          const uint32_t keep = keep_bits(gen, (uint64_t)row * a.groups + (col[i] >> 3), a.threshold);
+          input(0, x, i, f);
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            if (keep >> k & 1) v[i][k] = fmaf(f[k], a.factor, v[i][k]);
+            if (keep & (1u << (8 * i + k))) v[i][k] = fmaf(f[k], a.factor, v[i][k]);
         }
-        store8<T, VEC>(h, col[i], D, v[i]);
-      } else if (!pad) {
-        load8<T, VEC>(x, col[i], D, r);
-        unpack(r, v[i]);
+        store8<T, VEC>(h, base[i], lane, D, v[i]);
       }
+    } else if (!pad) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) input(0, x, i, v[i]);
     }
+    stage = stage + 1 == S ? 0 : stage + 1;
     if (pad) {
       const float zero[8] = {};
 #pragma unroll
-      for (int i = 0; i < NV; ++i) store8<T, VEC>(y, col[i], D, zero);
+      for (int i = 0; i < NV; ++i) store8<T, VEC>(y, base[i], lane, D, zero);
       continue;
     }
     float s = 0.f, none = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s += col[i] + k < D ? v[i][k] : 0.f;
+      for (int k = 0; k < 8; ++k) s += v[i][k];    // columns past D are zero
     row_sum2(rg, s, none);
     const float mean = s * inv_d;
     float sq = 0.f;
@@ -272,7 +380,7 @@ __global__ void __launch_bounds__(256) ln_fwd_kernel(RowArgs a) {
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float d = col[i] + k < D ? v[i][k] - mean : 0.f;
+        const float d = column<VEC>(base[i], lane, k) < D ? v[i][k] - mean : 0.f;
         sq = fmaf(d, d, sq);
       }
     row_sum2(rg, sq, none);
@@ -282,7 +390,7 @@ __global__ void __launch_bounds__(256) ln_fwd_kernel(RowArgs a) {
       float o[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) o[k] = fmaf((v[i][k] - mean) * rstd, wv[i][k], bv[i][k]);
-      store8<T, VEC>(y, col[i], D, o);
+      store8<T, VEC>(y, base[i], lane, D, o);
     }
   }
 }
@@ -295,54 +403,94 @@ __global__ void __launch_bounds__(256) ln_fwd_kernel(RowArgs a) {
 template <typename T, int NV, bool VEC, bool DROP>
 __global__ void __launch_bounds__(256) ln_bwd_kernel(RowArgs a) {
   __shared__ float2 exchange[8][2 * kMaxRowWarps];
-  extern __shared__ float combine[];               // [2][D] with more than one row group a CTA
+  extern __shared__ uint4 ring_slots[];            // the ring, then [2][D] for the CTA's sums
+  constexpr int TENSORS = DROP ? 3 : 2, S = ring_stages(Ring<T, NV, TENSORS>::WORDS);
+  const Ring<T, NV, TENSORS> ring{ring_slots};
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W, R = (blockDim.x >> 5) / W;
   const int group = warp / W;
   RowGroup rg{W, warp - group * W, 1 + group, exchange[group], 0};
   const int D = a.D;
-  int col[NV];
+  int base[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) base[i] = (i * W + rg.sub) * 256;
+  const int64_t stride = (int64_t)gridDim.x * R, first = (int64_t)blockIdx.x * R + group;
+  auto fetch = [&](int64_t row, int stage) {
+    if (VEC && row < a.M) {
+      const bool pad = padding_row(a, (int)row);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int col = base[i] + lane * 8;
+        if (!pad) {
+          ring.fetch(stage, 0, i, static_cast<const T*>(a.x) + row * a.ld_x, col, D);
+          ring.fetch(stage, 1, i, static_cast<const T*>(a.dy) + row * a.ld_dy, col, D);
+        }
+        if (DROP && a.dh) ring.fetch(stage, TENSORS - 1, i, static_cast<const T*>(a.dh) + row * a.ld_dh, col, D);
+      }
+    }
+    copies_commit();
+  };
+  if (VEC) {
+    ring.clear(S);                                 // and zeros stand in for a missing dh
+#pragma unroll
+    for (int s = 0; s + 1 < S; ++s) fetch(first + s * stride, s);
+  }
   float wv[NV][8], dw[NV][8], db[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    col[i] = ((i * W + rg.sub) * 32 + lane) * 8;
-    load_param8<T>(a.weight, a.param_fp32, col[i], D, wv[i]);
+    load_param8<T, VEC>(a.weight, a.param_fp32, base[i], lane, D, wv[i]);
 #pragma unroll
     for (int k = 0; k < 8; ++k) dw[i][k] = db[i][k] = 0.f;
   }
   Generator gen{};
   if (DROP) gen = load_generator(a.rng, a.site);
   const float inv_d = 1.0f / D;
-  for (int64_t row = (int64_t)blockIdx.x * R + group; row < a.M; row += (int64_t)gridDim.x * R) {
+  int stage = 0;
+  for (int64_t row = first; row < a.M; row += stride) {
     T* dx = static_cast<T*>(a.dx) + row * D;
     T* dres = DROP ? static_cast<T*>(a.dres) + row * D : nullptr;
-    const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
-    const T* dy = static_cast<const T*>(a.dy) + row * a.ld_dy;
-    const T* dh = DROP && a.dh ? static_cast<const T*>(a.dh) + row * a.ld_dh : nullptr;
-    if (padding_row(a, (int)row)) {
+    const bool pad = padding_row(a, (int)row);
+    if (VEC) {
+      fetch(row + (S - 1) * stride, stage == 0 ? S - 1 : stage - 1);
+      copies_wait<S - 1>();
+    }
+    const int here = stage;
+    stage = stage + 1 == S ? 0 : stage + 1;
+    auto input = [&](int tensor, const void* p, int64_t ld, int i, Vec8<T>& r) {
+      if (VEC)
+        ring.read(here, tensor, i, r);
+      else
+        load8<T, VEC>(static_cast<const T*>(p) + row * ld, base[i], lane, D, r);
+    };
+    auto input_dh = [&](int i, float (&f)[8]) {
+      if (VEC || a.dh) {
+        Vec8<T> r;
+        input(TENSORS - 1, a.dh, a.ld_dh, i, r);
+        unpack(r, f);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = 0.f;
+      }
+    };
+    if (pad) {
       const float zero[8] = {};
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        store8<T, VEC>(dx, col[i], D, zero);
+        store8<T, VEC>(dx, base[i], lane, D, zero);
         if (DROP) {
-          float f[8] = {};
-          if (dh) {
-            Vec8<T> r;
-            load8<T, VEC>(dh, col[i], D, r);
-            unpack(r, f);
-          }
-          store8<T, VEC>(dres, col[i], D, f);
+          float f[8];
+          input_dh(i, f);
+          store8<T, VEC>(dres, base[i], lane, D, f);
         }
       }
       continue;
     }
-    Vec8<T> xr[NV], gr[NV], hr[NV];
+    Vec8<T> xr[NV], gr[NV];
+    float s = 0.f, s0 = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      load8<T, VEC>(x, col[i], D, xr[i]);
-      load8<T, VEC>(dy, col[i], D, gr[i]);
-      if (DROP && dh) load8<T, VEC>(dh, col[i], D, hr[i]);
+      input(0, a.x, a.ld_x, i, xr[i]);
+      input(1, a.dy, a.ld_dy, i, gr[i]);
     }
-    float s = 0.f, s0 = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float f[8], g[8];
@@ -364,14 +512,17 @@ __global__ void __launch_bounds__(256) ln_bwd_kernel(RowArgs a) {
       unpack(gr[i], g);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float d = col[i] + k < D ? f[k] - mean : 0.f;
+        const float d = column<VEC>(base[i], lane, k) < D ? f[k] - mean : 0.f;
         s1 = fmaf(d, d, s1);
         s2 = fmaf(g[k] * wv[i][k], d, s2);
       }
     }
     row_sum2(rg, s1, s2);
     const float rstd = rsqrtf(fmaf(s1, inv_d, a.eps));
-    const float c1 = s0 * inv_d, c2 = rstd * rstd * (s2 * inv_d);
+    const float c1 = rstd * (s0 * inv_d), c2 = rstd * rstd * rstd * (s2 * inv_d);
+    uint32_t keep = 0;
+    if (DROP && !a.drop_all)
+      keep = keep_row<NV, VEC>(gen, (uint64_t)row * a.groups, base, lane, a.threshold << 16);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float f[8], g[8], o[8];
@@ -380,24 +531,22 @@ __global__ void __launch_bounds__(256) ln_bwd_kernel(RowArgs a) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float d = f[k] - mean;
-        o[k] = rstd * (fmaf(g[k], wv[i][k], -c1) - d * c2);
+        o[k] = fmaf(g[k] * wv[i][k], rstd, -fmaf(d, c2, c1));
         dw[i][k] = fmaf(g[k], d * rstd, dw[i][k]);
         db[i][k] += g[k];
       }
       if (DROP) {
-        if (dh) {
-          unpack(hr[i], f);
+        input_dh(i, f);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) o[k] += f[k];
-        }
-        store8<T, VEC>(dres, col[i], D, o);
-        const uint32_t keep = keep_bits(gen, (uint64_t)row * a.groups + (col[i] >> 3), a.threshold);
+        for (int k = 0; k < 8; ++k) o[k] += f[k];
+        store8<T, VEC>(dres, base[i], lane, D, o);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = keep >> k & 1 ? o[k] * a.factor : 0.f;
+        for (int k = 0; k < 8; ++k) o[k] = keep & (1u << (8 * i + k)) ? o[k] * a.factor : 0.f;
       }
-      store8<T, VEC>(dx, col[i], D, o);
+      store8<T, VEC>(dx, base[i], lane, D, o);
     }
   }
+  float* combine = reinterpret_cast<float*>(ring_slots + (VEC ? S * ring.WORDS * blockDim.x : 0));
   float* out = a.partials + (int64_t)blockIdx.x * 2 * D;
   for (int g = 0; g < R; ++g) {
     if (R > 1) __syncthreads();
@@ -406,7 +555,7 @@ __global__ void __launch_bounds__(256) ln_bwd_kernel(RowArgs a) {
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int c = col[i] + k;
+        const int c = column<VEC>(base[i], lane, k);
         if (c >= D) continue;
         float sw = dw[i][k], sb = db[i][k];
         if (g > 0) {
@@ -424,57 +573,97 @@ __global__ void __launch_bounds__(256) ln_bwd_kernel(RowArgs a) {
   }
 }
 
-// dw and db: the sums over the CTAs' partial rows, in a fixed order.  32 columns a CTA, 8 warps striding the rows.
+// dw and db: the sums over the CTAs' partial rows, in a fixed order.  32 columns a CTA, 32 warps striding the rows.
 template <typename T>
-__global__ void __launch_bounds__(256) ln_param_grad_kernel(const float* __restrict__ partials, int rows, int D,
-                                                            void* dweight, void* dbias, int fp32) {
-  __shared__ float part[8][33];
+__global__ void __launch_bounds__(1024) ln_param_grad_kernel(const float* __restrict__ partials, int rows, int D,
+                                                             void* dweight, void* dbias, int fp32) {
+  __shared__ float part[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;            // column of [dw | db]
   float s = 0.f;
   if (c < 2 * D)
-    for (int r = warp; r < rows; r += 8) s += __ldg(partials + (int64_t)r * 2 * D + c);
+    for (int r = warp; r < rows; r += 32) s += __ldg(partials + (int64_t)r * 2 * D + c);
   part[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && c < 2 * D) {
-    s = 0.f;
+  s = part[lane][warp];                            // warp w adds column w
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += part[i][lane];
-    void* dst = c < D ? dweight : dbias;
-    const int k = c < D ? c : c - D;
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int k = blockIdx.x * 32 + warp;
+  if (lane == 0 && k < 2 * D) {
+    void* dst = k < D ? dweight : dbias;
+    const int at = k < D ? k : k - D;
     if (fp32)
-      static_cast<float*>(dst)[k] = s;
+      static_cast<float*>(dst)[at] = s;
     else
-      static_cast<T*>(dst)[k] = from_f32<T>(s);
+      static_cast<T*>(dst)[at] = from_f32<T>(s);
   }
 }
 
-// out = residual + dropout(x), one group of eight columns a thread.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) dropout_kernel(RowArgs a, int64_t n) {
-  const Generator gen = load_generator(a.rng, a.site);
+// out = residual + dropout(x): a thread takes four groups of eight columns, so that their loads are under way
+// together.  FLAT (dense 16-byte aligned tensors without lengths): group g lies at element 8 g.  `n` groups from
+// `group0` on, fewer than 2^31.
+constexpr int kDropUnroll = 4;
+
+template <typename T, bool VEC, bool FLAT, bool RES>
+__global__ void __launch_bounds__(256) dropout_kernel(RowArgs a, int64_t group0, uint32_t n) {
   const int D = a.D;
-  const int64_t step = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
-    const int64_t r = i / a.groups;
-    const int col = (int)(i - r * a.groups) * 8;
-    const int64_t row = r;
-    float v[8] = {};
-    Vec8<T> q;
-    if (a.residual) {
-      load8<T, VEC>(static_cast<const T*>(a.residual) + row * a.ld_res, col, D, q);
-      unpack(q, v);
-    }
-    if (!padding_row(a, (int)row)) {
+  const uint32_t block0 = blockIdx.x * (256u * kDropUnroll) + threadIdx.x;
+  Vec8<T> xq[kDropUnroll], rq[kDropUnroll];
+  bool there[kDropUnroll], use[kDropUnroll];
+  int64_t row[kDropUnroll];
+  int col[kDropUnroll];
+  auto get = [&](const void* p, int64_t ld, int u, Vec8<T>& q) {
+    if (VEC) {
+      const T* src = static_cast<const T*>(p) + (FLAT ? (group0 + block0 + u * 256u) * 8 : row[u] * ld + col[u]);
+#pragma unroll
+      for (int i = 0; i < Vec8<T>::Q; ++i) q.q[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+    } else {
       float f[8];
-      load8<T, VEC>(static_cast<const T*>(a.x) + row * a.ld_x, col, D, q);
-      unpack(q, f);
-      const uint32_t keep = keep_bits(gen, (uint64_t)row * a.groups + (col >> 3), a.threshold);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = col[u] + k < D ? to_f32(static_cast<const T*>(p)[row[u] * ld + col[u] + k]) : 0.f;
+      pack(f, q);
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < kDropUnroll; ++u) {
+    const uint32_t g = block0 + u * 256u;
+    there[u] = g < n;
+    use[u] = there[u] && !a.drop_all;
+    if (!FLAT && there[u]) {
+      const uint32_t r = g / (uint32_t)a.groups;   // group0 begins a row
+      row[u] = group0 / a.groups + r;
+      col[u] = (int)(g - r * (uint32_t)a.groups) * 8;
+      use[u] = use[u] && !padding_row(a, (int)row[u]);
+    }
+    if (use[u]) get(a.x, a.ld_x, u, xq[u]);
+    if (RES && there[u]) get(a.residual, a.ld_res, u, rq[u]);
+  }
+  const Generator gen = load_generator(a.rng, a.site);
+#pragma unroll
+  for (int u = 0; u < kDropUnroll; ++u) {
+    if (!there[u]) continue;
+    const uint64_t group = group0 + block0 + u * 256u;
+    float v[8] = {};
+    if (RES) unpack(rq[u], v);
+    if (use[u]) {
+      float f[8];
+      unpack(xq[u], f);
+      const uint32_t keep = keep_bits(gen, group, a.threshold << 16);
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (keep >> k & 1) v[k] = fmaf(f[k], a.factor, v[k]);
+        if (keep & (1u << k)) v[k] = RES ? fmaf(f[k], a.factor, v[k]) : f[k] * a.factor;
     }
-    store8<T, VEC>(static_cast<T*>(a.y) + row * D, col, D, v);
+    T* dst = static_cast<T*>(a.y) + (FLAT ? (int64_t)group * 8 : row[u] * D + col[u]);
+    if (VEC) {
+      Vec8<T> q;
+      pack(v, q);
+#pragma unroll
+      for (int i = 0; i < Vec8<T>::Q; ++i) *(reinterpret_cast<uint4*>(dst) + i) = q.q[i];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (col[u] + k < D) dst[k] = from_f32<T>(v[k]);
+    }
   }
 }
 
@@ -508,19 +697,27 @@ bool vec_ok(const RowArgs& a, int size) {
 template <typename T, int NV, bool VEC, bool DROP>
 int launch_fwd(const RowArgs& a, const RowShape& s, cudaStream_t stream) {
   const int R = s.warps / s.W;
-  const int64_t want = (a.M + R - 1) / R;
-  const int grid = (int)(want < 4 * device_sm_count() ? want : 4 * device_sm_count());
-  ln_fwd_kernel<T, NV, VEC, DROP><<<grid, s.warps * 32, 0, stream>>>(a);
+  const int64_t want = (a.M + R - 1) / R, most = 2 * device_sm_count();
+  constexpr int words = Ring<T, NV, DROP ? 2 : 1>::WORDS;
+  const size_t smem = VEC ? sizeof(uint4) * ring_stages(words) * words * s.warps * 32 : 0;
+  auto* kernel = ln_fwd_kernel<T, NV, VEC, DROP>;
+  if (smem > 48 * 1024)
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
+  kernel<<<(int)(want < most ? want : most), s.warps * 32, smem, stream>>>(a);
   return (int)cudaGetLastError();
 }
 
 template <typename T, int NV, bool VEC, bool DROP>
 int launch_bwd(const RowArgs& a, const RowShape& s, cudaStream_t stream) {
   const int R = s.warps / s.W;
-  const size_t smem = R > 1 ? (size_t)2 * a.D * sizeof(float) : 0;
-  ln_bwd_kernel<T, NV, VEC, DROP><<<(int)a.partial_rows, s.warps * 32, smem, stream>>>(a);
-  if (cudaError_t e = cudaGetLastError()) return (int)e;
-  return 0;
+  constexpr int words = Ring<T, NV, DROP ? 3 : 2>::WORDS;
+  const size_t smem = (VEC ? sizeof(uint4) * ring_stages(words) * words * s.warps * 32 : 0) +
+                      (R > 1 ? (size_t)2 * a.D * sizeof(float) : 0);
+  auto* kernel = ln_bwd_kernel<T, NV, VEC, DROP>;
+  if (smem > 48 * 1024)
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
+  kernel<<<(int)a.partial_rows, s.warps * 32, smem, stream>>>(a);
+  return (int)cudaGetLastError();
 }
 
 template <typename T, bool VEC, bool DROP>
@@ -535,21 +732,30 @@ int launch_rows(const RowArgs& a, bool bwd, cudaStream_t stream) {
   }
 }
 
+template <typename T, bool RES>
+int launch_dropout(const RowArgs& a, bool vec, cudaStream_t stream) {
+  const bool flat = vec && !a.lengths && (a.ld_x == a.D || a.M == 1) && (!RES || a.ld_res == a.D || a.M == 1);
+  const int64_t rows_a_time = (int64_t)0x7fffffff / a.groups;    // whole rows, a 32-bit count of groups a launch
+  for (int64_t row0 = 0; row0 < a.M; row0 += rows_a_time) {
+    const int64_t rows = a.M - row0 < rows_a_time ? a.M - row0 : rows_a_time;
+    const uint32_t n = (uint32_t)(rows * a.groups);
+    const int grid = (int)((n + 256u * kDropUnroll - 1) / (256u * kDropUnroll));
+    const int64_t group0 = row0 * a.groups;
+    if (flat)
+      dropout_kernel<T, true, true, RES><<<grid, 256, 0, stream>>>(a, group0, n);
+    else if (vec)
+      dropout_kernel<T, true, false, RES><<<grid, 256, 0, stream>>>(a, group0, n);
+    else
+      dropout_kernel<T, false, false, RES><<<grid, 256, 0, stream>>>(a, group0, n);
+    if (cudaError_t e = cudaGetLastError()) return (int)e;
+  }
+  return 0;
+}
+
 template <typename T>
 int launch_typed(const RowArgs& a, int op, cudaStream_t stream) {
   const bool vec = vec_ok(a, sizeof(T));
-  if (op == kRowDropout) {
-    // the grid's thread index counts groups in 64 bits
-    const int64_t n = a.M * a.groups;
-    const int64_t want = (n + 255) / 256;
-    const int64_t most = 16 * (int64_t)device_sm_count();
-    const int grid = (int)(want < most ? want : most);
-    if (vec)
-      dropout_kernel<T, true><<<grid, 256, 0, stream>>>(a, n);
-    else
-      dropout_kernel<T, false><<<grid, 256, 0, stream>>>(a, n);
-    return (int)cudaGetLastError();
-  }
+  if (op == kRowDropout) return a.residual ? launch_dropout<T, true>(a, vec, stream) : launch_dropout<T, false>(a, vec, stream);
   const bool drop = op == kRowDropNorm || op == kRowDropNormGrad, bwd = op == kRowNormGrad || op == kRowDropNormGrad;
   if (a.M > 0) {
     const int rc = drop ? (vec ? launch_rows<T, true, true>(a, bwd, stream) : launch_rows<T, false, true>(a, bwd, stream))
@@ -558,8 +764,8 @@ int launch_typed(const RowArgs& a, int op, cudaStream_t stream) {
     if (rc) return rc;
   }
   if (bwd) {
-    ln_param_grad_kernel<T><<<(2 * a.D + 31) / 32, 256, 0, stream>>>(a.partials, (int)a.partial_rows, a.D, a.dweight,
-                                                                     a.dbias, a.param_fp32);
+    ln_param_grad_kernel<T><<<(2 * a.D + 31) / 32, 1024, 0, stream>>>(a.partials, (int)a.partial_rows, a.D, a.dweight,
+                                                                      a.dbias, a.param_fp32);
     return (int)cudaGetLastError();
   }
   return 0;
@@ -567,11 +773,12 @@ int launch_typed(const RowArgs& a, int op, cudaStream_t stream) {
 
 }  // namespace rows_impl
 
+// CTAs of the backward pass, a partial row each: one an SM (the ring and the sums in registers fill it)
 int row_partial_rows(int64_t M, int D) {
   const rows_impl::RowShape s = rows_impl::row_shape(D);
   const int R = s.warps / s.W;
   const int64_t want = (M + R - 1) / R;
-  return (int)(want < 2 * device_sm_count() ? want : 2 * device_sm_count());
+  return (int)(want < device_sm_count() ? want : device_sm_count());
 }
 
 int launch_row_op(const RowArgs& args, int op, int dtype, cudaStream_t stream) {

@@ -127,7 +127,8 @@ def test_layer_norm_op_matches_inference_kernel():
 
 
 def test_strides_and_alignment():
-    """Row strides, a tensor off the 16-byte grid, transposed and broadcast inputs, a zero-stride weight."""
+    """Row strides, a tensor off the 16-byte grid, transposed and broadcast inputs, a zero-stride weight.  Rows off the
+    grid are added up in another order than those on it: within the bounds, not the same bits."""
     B, T, D = 2, 5, 64
     w, b = rand(3, (D,), F32, 0.2, 1.0), rand(4, (D,), F32)
     wide = rand(1, (B, T, 2 * D), BF)
@@ -136,18 +137,30 @@ def test_strides_and_alignment():
              rand(6, (B, D, T), BF).transpose(1, 2), rand(7, (1, 1, D), BF).expand(B, T, D), wide[:, ::2, :D]]
     for i, x in enumerate(cases):
         dense = x.contiguous().clone()
-        dy = rand(8, x.shape, BF)
-        assert torch.equal(tr.layer_norm(x, w, b), tr.layer_norm(dense, w, b)), i
-        for got, want in zip(tr.layer_norm_backward(x, x, w), tr.layer_norm_backward(dense, dense, w)):
-            assert torch.equal(got, want), i
-        rng = rng_of()
+        dy, rng = rand(8, x.shape, BF), rng_of()
+        ref, r = R.layer_norm(x, w, b, EPS)
+        close(tr.layer_norm(x, w, b), ref, norm_bound(BF, ref, x, w, b, r), i)
+        for g, at in ((dy, x), (x, dy)):
+            rdx, rdw, rdb, r, xh = R.layer_norm_backward(g, at, w, EPS)
+            dx, dw, db = tr.layer_norm_backward(g, at, w)
+            close(dx, rdx, grads_bound(BF, rdx, g, at, w, r, None), i)
+            bw, bb = param_bounds(F32, rdw, rdb, g, at, r, xh, None)
+            close(dw, rdw, bw, i)
+            close(db, rdb, bb, i)
+            fx, fres, fw, fb = tr.dropout_add_layer_norm_backward(g, at, at, w, rng, 0.3)
+            total = rdx + at.double().cpu()
+            bound = rounded(BF, total) + grads_bound(F32, rdx, g, at, w, r, None) + E * total.abs()
+            close(fres, total, bound, i)
+            want = torch.where(R.keep_mask(x.shape, int(rng[0]), int(rng[1]), 0, 0.3), total * R.factor(0.3, 1.0), 0.0)
+            close(fx, want, R.factor(0.3, 1.0) * bound + rounded(BF, want), i)
+            assert torch.equal(fw, dw) and torch.equal(fb, db), i
         assert torch.equal(tr.dropout_add(x, rng, 0.3, residual=x), tr.dropout_add(dense, rng, 0.3, residual=dense)), i
-        for got, want in zip(tr.dropout_add_layer_norm(x, x, w, b, rng, 0.3),
-                             tr.dropout_add_layer_norm(dense, dense, w, b, rng, 0.3)):
-            assert torch.equal(got, want), i
-        for got, want in zip(tr.dropout_add_layer_norm_backward(dy, x, x, w, rng, 0.3),
-                             tr.dropout_add_layer_norm_backward(dy, dense, dense, w, rng, 0.3)):
-            assert torch.equal(got, want), i
+        y, h = tr.dropout_add_layer_norm(x, x, w, b, rng, 0.3)
+        assert torch.equal(h, tr.dropout_add(x, rng, 0.3, residual=x)), i
+        rh = R.dropout_add(x, x, int(rng[0]), int(rng[1]), 0, 0.3, 1.0)
+        ry, r = R.layer_norm(rh, w, b, EPS)
+        extra = 8 * E * row_max(rh) * r * w.double().cpu().abs() * (2 + r * row_max(rh))
+        close(y, ry, norm_bound(BF, ry, rh, w, b, r) + extra, i)
     one = torch.ones(1, device=DEV).expand(D)
     assert torch.equal(tr.layer_norm(wide[..., :D], one, one), tr.layer_norm(wide[..., :D], one.clone(), one.clone()))
 
