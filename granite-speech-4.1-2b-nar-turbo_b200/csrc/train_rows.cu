@@ -37,55 +37,76 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 
-__device__ __forceinline__ void unpack(const Vec8<__nv_bfloat16>& r, float (&f)[8]) {
+// fp32 pairs, two lanes an instruction (sm_100)
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+__device__ __forceinline__ void unpack(const Vec8<__nv_bfloat16>& r, float2 (&f)[4]) {
   const uint32_t w[4] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w};
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    f[2 * k] = bf16lo_to_f32(w[k]);
-    f[2 * k + 1] = bf16hi_to_f32(w[k]);
-  }
+  for (int k = 0; k < 4; ++k) f[k] = make_float2(bf16lo_to_f32(w[k]), bf16hi_to_f32(w[k]));
 }
-__device__ __forceinline__ void unpack(const Vec8<__half>& r, float (&f)[8]) {
+__device__ __forceinline__ void unpack(const Vec8<__half>& r, float2 (&f)[4]) {
   const uint32_t w[4] = {r.q[0].x, r.q[0].y, r.q[0].z, r.q[0].w};
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-    f[2 * k] = p.x;
-    f[2 * k + 1] = p.y;
-  }
+  for (int k = 0; k < 4; ++k) f[k] = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
 }
-__device__ __forceinline__ void unpack(const Vec8<float>& r, float (&f)[8]) {
+__device__ __forceinline__ void unpack(const Vec8<float>& r, float2 (&f)[4]) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    f[4 * k] = __uint_as_float(r.q[k].x);
-    f[4 * k + 1] = __uint_as_float(r.q[k].y);
-    f[4 * k + 2] = __uint_as_float(r.q[k].z);
-    f[4 * k + 3] = __uint_as_float(r.q[k].w);
+    f[2 * k] = make_float2(__uint_as_float(r.q[k].x), __uint_as_float(r.q[k].y));
+    f[2 * k + 1] = make_float2(__uint_as_float(r.q[k].z), __uint_as_float(r.q[k].w));
   }
 }
-__device__ __forceinline__ void pack(const float (&f)[8], Vec8<__nv_bfloat16>& r) {
-  r.q[0] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                      pack_bf16x2(f[6], f[7]));
+__device__ __forceinline__ void pack(const float2 (&f)[4], Vec8<__nv_bfloat16>& r) {
+  r.q[0] = make_uint4(pack_bf16x2(f[0].x, f[0].y), pack_bf16x2(f[1].x, f[1].y), pack_bf16x2(f[2].x, f[2].y),
+                      pack_bf16x2(f[3].x, f[3].y));
 }
-__device__ __forceinline__ void pack(const float (&f)[8], Vec8<__half>& r) {
+__device__ __forceinline__ void pack(const float2 (&f)[4], Vec8<__half>& r) {
   uint32_t w[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const __half2 h = __floats2half2_rn(f[2 * k], f[2 * k + 1]);
+    const __half2 h = __float22half2_rn(f[k]);
     w[k] = *reinterpret_cast<const uint32_t*>(&h);
   }
   r.q[0] = make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ void pack(const float (&f)[8], Vec8<float>& r) {
+__device__ __forceinline__ void pack(const float2 (&f)[4], Vec8<float>& r) {
 #pragma unroll
   for (int k = 0; k < 2; ++k)
-    r.q[k] = make_uint4(__float_as_uint(f[4 * k]), __float_as_uint(f[4 * k + 1]), __float_as_uint(f[4 * k + 2]),
-                        __float_as_uint(f[4 * k + 3]));
+    r.q[k] = make_uint4(__float_as_uint(f[2 * k].x), __float_as_uint(f[2 * k].y), __float_as_uint(f[2 * k + 1].x),
+                        __float_as_uint(f[2 * k + 1].y));
+}
+
+// the same as single values (the CTC kernels)
+template <typename T>
+__device__ __forceinline__ void unpack(const Vec8<T>& r, float (&f)[8]) {
+  float2 p[4];
+  unpack(r, p);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    f[2 * k] = p[k].x;
+    f[2 * k + 1] = p[k].y;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void pack(const float (&f)[8], Vec8<T>& r) {
+  const float2 p[4] = {{f[0], f[1]}, {f[2], f[3]}, {f[4], f[5]}, {f[6], f[7]}};
+  pack(p, r);
 }
 
 // A warp's block of 256 columns: lane l holds eight of them.  VEC (rows aligned to 16 bytes, D % 8 == 0): columns
 // 8 l .. 8 l + 7, one 16-byte word of a 16-bit type.  Otherwise columns l + 32 k, so that single elements still make
-// whole 32-byte sectors (eight neighbours a lane cost 8 times the L2 writes: 80 -> 23 us at 11376 x 1001 fp16).
+// whole 32-byte sectors.
 template <bool VEC>
 __device__ __forceinline__ int column(int base, int lane, int k) {
   return VEC ? base + lane * 8 + k : base + k * 32 + lane;
@@ -111,7 +132,7 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, int base, int l
 }
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* __restrict__ row, int base, int lane, int D, const float (&f)[8]) {
+__device__ __forceinline__ void store8(T* __restrict__ row, int base, int lane, int D, const float2 (&f)[4]) {
   if (VEC) {
     const int col = base + lane * 8;
     if (col >= D) return;
@@ -123,19 +144,29 @@ __device__ __forceinline__ void store8(T* __restrict__ row, int base, int lane, 
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int col = column<VEC>(base, lane, k);
-      if (col < D) row[col] = from_f32<T>(f[k]);
+      if (col < D) row[col] = from_f32<T>(k & 1 ? f[k / 2].y : f[k / 2].x);
     }
   }
 }
 
 // The lane's columns of weight or bias as fp32; `fp32`: stored as fp32, else as T.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_param8(const void* p, int fp32, int base, int lane, int D, float (&f)[8]) {
+__device__ __forceinline__ void load_param8(const void* p, int fp32, int base, int lane, int D, float2 (&f)[4]) {
+  float v[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const int c = column<VEC>(base, lane, k);
-    f[k] = c >= D ? 0.f : fp32 ? __ldg(static_cast<const float*>(p) + c) : to_f32(static_cast<const T*>(p)[c]);
+    v[k] = c >= D ? 0.f : fp32 ? __ldg(static_cast<const float*>(p) + c) : to_f32(static_cast<const T*>(p)[c]);
   }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) f[k] = make_float2(v[2 * k], v[2 * k + 1]);
+}
+
+// v where the column is inside the row, else 0
+template <bool VEC>
+__device__ __forceinline__ float2 inside(float v, int base, int lane, int k, int D) {
+  if (VEC) return both(base + lane * 8 < D ? v : 0.f);
+  return make_float2(column<VEC>(base, lane, 2 * k) < D ? v : 0.f, column<VEC>(base, lane, 2 * k + 1) < D ? v : 0.f);
 }
 
 __device__ __forceinline__ void copy16(void* smem, const void* gmem) {
@@ -270,19 +301,43 @@ __device__ __forceinline__ void row_sum2(RowGroup& g, float& a, float& b) {
   }
 }
 
+__device__ __forceinline__ float row_sum(RowGroup& g, float a) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  if (g.W > 1) {
+    float2* s = g.slot + g.phase * kMaxRowWarps;
+    g.phase ^= 1;
+    if ((threadIdx.x & 31) == 0) s[g.sub].x = a;
+    asm volatile("bar.sync %0, %1;" ::"r"(g.bar), "r"(g.W * 32) : "memory");
+    a = 0.f;
+    for (int i = 0; i < g.W; ++i) a += s[i].x;
+  }
+  return a;
+}
+
 __device__ __forceinline__ bool padding_row(const RowArgs& a, int row) {
   if (a.lengths == nullptr) return false;
   const int b = row / a.T;
   return row - b * a.T >= __ldg(a.lengths + b);
 }
 
-// Rows under way a warp: what the SM's shared memory holds for two CTAs (forward, short rows) or one.
-__host__ __device__ constexpr int ring_stages(int words) { return words <= 4 ? 4 : words <= 16 ? 3 : 2; }
+// Rows under way a warp: as many as leave two CTAs an SM (one where a lane holds 32 columns of fp32)
+__host__ __device__ constexpr int ring_stages(int words) { return words <= 6 ? 4 : words <= 8 ? 3 : 2; }
+
+// The kept ones of eight elements, the others 0 (chosen, not multiplied: a dropped infinity is gone).  `keep`: bits
+// 8 i + k.
+__device__ __forceinline__ void keep8(uint32_t keep, int i, float2 (&f)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    f[k].x = keep & (1u << (8 * i + 2 * k)) ? f[k].x : 0.f;
+    f[k].y = keep & (2u << (8 * i + 2 * k)) ? f[k].y : 0.f;
+  }
+}
 
 // LayerNorm forward; DROP: of h = residual + dropout(x), which is stored too.  W warps a row, NV blocks of 256 columns
 // a warp: a row stays in registers between the two passes of its statistics, its weights for all rows of the warp.
 template <typename T, int NV, bool VEC, bool DROP>
-__global__ void __launch_bounds__(256, 2) ln_fwd_kernel(RowArgs a) {
+__global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_fwd_kernel(RowArgs a) {
   __shared__ float2 exchange[8][2 * kMaxRowWarps];
   extern __shared__ uint4 ring_slots[];
   constexpr int TENSORS = DROP ? 2 : 1, S = ring_stages(Ring<T, NV, TENSORS>::WORDS);
@@ -312,7 +367,7 @@ __global__ void __launch_bounds__(256, 2) ln_fwd_kernel(RowArgs a) {
 #pragma unroll
     for (int s = 0; s + 1 < S; ++s) fetch(first + s * stride, s);
   }
-  float wv[NV][8], bv[NV][8];
+  float2 wv[NV][4], bv[NV][4];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     load_param8<T, VEC>(a.weight, a.param_fp32, base[i], lane, D, wv[i]);
@@ -324,72 +379,67 @@ __global__ void __launch_bounds__(256, 2) ln_fwd_kernel(RowArgs a) {
   int stage = 0;
   for (int64_t row = first; row < a.M; row += stride) {
     T* y = static_cast<T*>(a.y) + row * D;
-    T* h = DROP ? static_cast<T*>(a.h_out) + row * D : nullptr;
-    const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
-    const T* res = DROP ? static_cast<const T*>(a.residual) + row * a.ld_res : nullptr;
     const bool pad = padding_row(a, (int)row);
     if (VEC) {
       fetch(row + (S - 1) * stride, stage == 0 ? S - 1 : stage - 1);
       copies_wait<S - 1>();
     }
-    float v[NV][8];
-    auto input = [&](int tensor, const T* p, int i, float (&f)[8]) {
+    float2 v[NV][4];
+    auto input = [&](int tensor, const void* p, int64_t ld, int i, float2 (&f)[4]) {
       Vec8<T> r;
       if (VEC)
         ring.read(stage, tensor, i, r);
       else
-        load8<T, VEC>(p, base[i], lane, D, r);
+        load8<T, VEC>(static_cast<const T*>(p) + row * ld, base[i], lane, D, r);
       unpack(r, f);
     };
     if (DROP) {
+      const bool add = !pad && !a.drop_all;
       uint32_t keep = 0;
-      if (!pad && !a.drop_all)
-        keep = keep_row<NV, VEC>(gen, (uint64_t)row * a.groups, base, lane, a.threshold << 16);
+      if (add) keep = keep_row<NV, VEC>(gen, (uint64_t)row * a.groups, base, lane, a.threshold << 16);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        input(1, res, i, v[i]);
-        if (!pad && !a.drop_all) {
-          float f[8];
-          input(0, x, i, f);
+        input(1, a.residual, a.ld_res, i, v[i]);
+        if (add) {
+          float2 f[4];
+          input(0, a.x, a.ld_x, i, f);
+          keep8(keep, i, f);
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (keep & (1u << (8 * i + k))) v[i][k] = fmaf(f[k], a.factor, v[i][k]);
+          for (int k = 0; k < 4; ++k) v[i][k] = ffma2(f[k], both(a.factor), v[i][k]);
         }
-        store8<T, VEC>(h, base[i], lane, D, v[i]);
+        store8<T, VEC>(static_cast<T*>(a.h_out) + row * D, base[i], lane, D, v[i]);
       }
     } else if (!pad) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) input(0, x, i, v[i]);
+      for (int i = 0; i < NV; ++i) input(0, a.x, a.ld_x, i, v[i]);
     }
     stage = stage + 1 == S ? 0 : stage + 1;
     if (pad) {
-      const float zero[8] = {};
+      const float2 zero[4] = {};
 #pragma unroll
       for (int i = 0; i < NV; ++i) store8<T, VEC>(y, base[i], lane, D, zero);
       continue;
     }
-    float s = 0.f, none = 0.f;
+    float2 acc = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s += v[i][k];    // columns past D are zero
-    row_sum2(rg, s, none);
-    const float mean = s * inv_d;
-    float sq = 0.f;
+      for (int k = 0; k < 4; ++k) acc = add2(acc, v[i][k]);    // columns past D are zero
+    const float mean = row_sum(rg, acc.x + acc.y) * inv_d;
+    acc = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float d = column<VEC>(base[i], lane, k) < D ? v[i][k] - mean : 0.f;
-        sq = fmaf(d, d, sq);
+      for (int k = 0; k < 4; ++k) {
+        v[i][k] = add2(v[i][k], inside<VEC>(-mean, base[i], lane, k, D));
+        acc = ffma2(v[i][k], v[i][k], acc);
       }
-    row_sum2(rg, sq, none);
-    const float rstd = rsqrtf(fmaf(sq, inv_d, a.eps));
+    const float rstd = rsqrtf(fmaf(row_sum(rg, acc.x + acc.y), inv_d, a.eps));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float o[8];
+      float2 o[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) o[k] = fmaf((v[i][k] - mean) * rstd, wv[i][k], bv[i][k]);
+      for (int k = 0; k < 4; ++k) o[k] = ffma2(mul2(v[i][k], both(rstd)), wv[i][k], bv[i][k]);
       store8<T, VEC>(y, base[i], lane, D, o);
     }
   }
@@ -401,9 +451,9 @@ __global__ void __launch_bounds__(256, 2) ln_fwd_kernel(RowArgs a) {
 // lane keeps the running sums of its columns' dw and db over all rows of its warp; the CTA adds its row groups in
 // order and leaves one partial row, so no sum depends on the order of arrival.
 template <typename T, int NV, bool VEC, bool DROP>
-__global__ void __launch_bounds__(256) ln_bwd_kernel(RowArgs a) {
+__global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_bwd_kernel(RowArgs a) {
   __shared__ float2 exchange[8][2 * kMaxRowWarps];
-  extern __shared__ uint4 ring_slots[];            // the ring, then [2][D] for the CTA's sums
+  extern __shared__ uint4 ring_slots[];            // the ring; at the end [2][D], the CTA's sums
   constexpr int TENSORS = DROP ? 3 : 2, S = ring_stages(Ring<T, NV, TENSORS>::WORDS);
   const Ring<T, NV, TENSORS> ring{ring_slots};
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W, R = (blockDim.x >> 5) / W;
@@ -434,12 +484,12 @@ __global__ void __launch_bounds__(256) ln_bwd_kernel(RowArgs a) {
 #pragma unroll
     for (int s = 0; s + 1 < S; ++s) fetch(first + s * stride, s);
   }
-  float wv[NV][8], dw[NV][8], db[NV][8];
+  float2 wv[NV][4], dw[NV][4], db[NV][4];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     load_param8<T, VEC>(a.weight, a.param_fp32, base[i], lane, D, wv[i]);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) dw[i][k] = db[i][k] = 0.f;
+    for (int k = 0; k < 4; ++k) dw[i][k] = db[i][k] = both(0.f);
   }
   Generator gen{};
   if (DROP) gen = load_generator(a.rng, a.site);
@@ -455,121 +505,118 @@ __global__ void __launch_bounds__(256) ln_bwd_kernel(RowArgs a) {
     }
     const int here = stage;
     stage = stage + 1 == S ? 0 : stage + 1;
-    auto input = [&](int tensor, const void* p, int64_t ld, int i, Vec8<T>& r) {
+    auto input = [&](int tensor, const void* p, int64_t ld, int i, float2 (&f)[4]) {
+      Vec8<T> r;
       if (VEC)
         ring.read(here, tensor, i, r);
       else
         load8<T, VEC>(static_cast<const T*>(p) + row * ld, base[i], lane, D, r);
+      unpack(r, f);
     };
-    auto input_dh = [&](int i, float (&f)[8]) {
+    auto input_dh = [&](int i, float2 (&f)[4]) {
       if (VEC || a.dh) {
-        Vec8<T> r;
-        input(TENSORS - 1, a.dh, a.ld_dh, i, r);
-        unpack(r, f);
+        input(TENSORS - 1, a.dh, a.ld_dh, i, f);
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] = 0.f;
+        for (int k = 0; k < 4; ++k) f[k] = both(0.f);
       }
     };
     if (pad) {
-      const float zero[8] = {};
+      const float2 zero[4] = {};
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         store8<T, VEC>(dx, base[i], lane, D, zero);
         if (DROP) {
-          float f[8];
+          float2 f[4];
           input_dh(i, f);
           store8<T, VEC>(dres, base[i], lane, D, f);
         }
       }
       continue;
     }
-    Vec8<T> xr[NV], gr[NV];
-    float s = 0.f, s0 = 0.f;
+    float2 x[NV][4], g[NV][4], sx = both(0.f), s0 = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      input(0, a.x, a.ld_x, i, xr[i]);
-      input(1, a.dy, a.ld_dy, i, gr[i]);
+      input(0, a.x, a.ld_x, i, x[i]);
+      input(1, a.dy, a.ld_dy, i, g[i]);
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      float f[8], g[8];
-      unpack(xr[i], f);
-      unpack(gr[i], g);
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {                // columns past D are zero in x and dy
-        s += f[k];
-        s0 = fmaf(g[k], wv[i][k], s0);
+      for (int k = 0; k < 4; ++k) {                // columns past D are zero in x and dy
+        sx = add2(sx, x[i][k]);
+        s0 = ffma2(g[i][k], wv[i][k], s0);
       }
-    }
-    row_sum2(rg, s, s0);
-    const float mean = s * inv_d;
-    float s1 = 0.f, s2 = 0.f;
+    float sum_x = sx.x + sx.y, sum_g = s0.x + s0.y;
+    row_sum2(rg, sum_x, sum_g);
+    const float mean = sum_x * inv_d;
+    float2 s1 = both(0.f), s2 = both(0.f);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      float f[8], g[8];
-      unpack(xr[i], f);
-      unpack(gr[i], g);
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float d = column<VEC>(base[i], lane, k) < D ? f[k] - mean : 0.f;
-        s1 = fmaf(d, d, s1);
-        s2 = fmaf(g[k] * wv[i][k], d, s2);
+      for (int k = 0; k < 4; ++k) {
+        x[i][k] = add2(x[i][k], inside<VEC>(-mean, base[i], lane, k, D));
+        s1 = ffma2(x[i][k], x[i][k], s1);
+        s2 = ffma2(mul2(g[i][k], wv[i][k]), x[i][k], s2);
       }
-    }
-    row_sum2(rg, s1, s2);
-    const float rstd = rsqrtf(fmaf(s1, inv_d, a.eps));
-    const float c1 = rstd * (s0 * inv_d), c2 = rstd * rstd * rstd * (s2 * inv_d);
+    float sum_dd = s1.x + s1.y, sum_gd = s2.x + s2.y;
+    row_sum2(rg, sum_dd, sum_gd);
+    const float rstd = rsqrtf(fmaf(sum_dd, inv_d, a.eps));
+    const float2 r2 = both(rstd), c1 = both(-rstd * (sum_g * inv_d));
+    const float2 c2 = both(-rstd * rstd * rstd * (sum_gd * inv_d));
     uint32_t keep = 0;
     if (DROP && !a.drop_all)
       keep = keep_row<NV, VEC>(gen, (uint64_t)row * a.groups, base, lane, a.threshold << 16);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float f[8], g[8], o[8];
-      unpack(xr[i], f);
-      unpack(gr[i], g);
+      float2 o[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float d = f[k] - mean;
-        o[k] = fmaf(g[k] * wv[i][k], rstd, -fmaf(d, c2, c1));
-        dw[i][k] = fmaf(g[k], d * rstd, dw[i][k]);
-        db[i][k] += g[k];
+      for (int k = 0; k < 4; ++k) {
+        const float2 gr = mul2(g[i][k], r2);
+        o[k] = ffma2(gr, wv[i][k], ffma2(x[i][k], c2, c1));
+        dw[i][k] = ffma2(gr, x[i][k], dw[i][k]);
+        db[i][k] = add2(db[i][k], g[i][k]);
       }
       if (DROP) {
+        float2 f[4];
         input_dh(i, f);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] += f[k];
+        for (int k = 0; k < 4; ++k) o[k] = add2(o[k], f[k]);
         store8<T, VEC>(dres, base[i], lane, D, o);
+        keep8(keep, i, o);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = keep & (1u << (8 * i + k)) ? o[k] * a.factor : 0.f;
+        for (int k = 0; k < 4; ++k) o[k] = mul2(o[k], both(a.factor));
       }
       store8<T, VEC>(dx, base[i], lane, D, o);
     }
   }
-  float* combine = reinterpret_cast<float*>(ring_slots + (VEC ? S * ring.WORDS * blockDim.x : 0));
+  float* combine = reinterpret_cast<float*>(ring_slots);       // the ring is done with
+  copies_wait<0>();
+  if (R > 1) __syncthreads();
   float* out = a.partials + (int64_t)blockIdx.x * 2 * D;
   for (int g = 0; g < R; ++g) {
-    if (R > 1) __syncthreads();
-    if (group != g) continue;
+    if (group == g) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+      for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int c = column<VEC>(base[i], lane, k);
-        if (c >= D) continue;
-        float sw = dw[i][k], sb = db[i][k];
-        if (g > 0) {
-          sw += combine[c];
-          sb += combine[D + c];
+        for (int k = 0; k < 8; ++k) {
+          const int c = column<VEC>(base[i], lane, k);
+          if (c >= D) continue;
+          float sw = k & 1 ? dw[i][k / 2].y : dw[i][k / 2].x, sb = k & 1 ? db[i][k / 2].y : db[i][k / 2].x;
+          if (g > 0) {
+            sw += combine[c];
+            sb += combine[D + c];
+          }
+          if (g + 1 < R) {
+            combine[c] = sw;
+            combine[D + c] = sb;
+          } else {
+            out[c] = sw;
+            out[D + c] = sb;
+          }
         }
-        if (g + 1 < R) {
-          combine[c] = sw;
-          combine[D + c] = sb;
-        } else {
-          out[c] = sw;
-          out[D + c] = sb;
-        }
-      }
+    }
+    if (g + 1 < R) __syncthreads();
   }
 }
 
@@ -643,15 +690,14 @@ __global__ void __launch_bounds__(256) dropout_kernel(RowArgs a, int64_t group0,
   for (int u = 0; u < kDropUnroll; ++u) {
     if (!there[u]) continue;
     const uint64_t group = group0 + block0 + u * 256u;
-    float v[8] = {};
+    float2 v[4] = {};
     if (RES) unpack(rq[u], v);
     if (use[u]) {
-      float f[8];
+      float2 f[4];
       unpack(xq[u], f);
-      const uint32_t keep = keep_bits(gen, group, a.threshold << 16);
+      keep8(keep_bits(gen, group, a.threshold << 16), 0, f);
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (keep & (1u << k)) v[k] = RES ? fmaf(f[k], a.factor, v[k]) : f[k] * a.factor;
+      for (int k = 0; k < 4; ++k) v[k] = RES ? ffma2(f[k], both(a.factor), v[k]) : mul2(f[k], both(a.factor));
     }
     T* dst = static_cast<T*>(a.y) + (FLAT ? (int64_t)group * 8 : row[u] * D + col[u]);
     if (VEC) {
@@ -662,23 +708,22 @@ __global__ void __launch_bounds__(256) dropout_kernel(RowArgs a, int64_t group0,
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (col[u] + k < D) dst[k] = from_f32<T>(v[k]);
+        if (col[u] + k < D) dst[k] = from_f32<T>(k & 1 ? v[k / 2].y : v[k / 2].x);
     }
   }
 }
 
-// A row's warps and vectors a lane: the fewest warps that hold the row in four vectors (32 columns) a lane.
+// A row's warps and blocks of 256 columns a warp.  Two blocks, 16 columns a lane, leave 16 warps an SM beside the
+// weights and the sums of their gradients in registers (one warp with four blocks a row: 8 warps, 100 us instead of
+// 6x us at 73728 x 1024 backward); the widest rows take four.
 struct RowShape {
   int W, NV, warps;
 };
 RowShape row_shape(int D) {
-  const int vec = (D + 255) / 256;                 // vectors of 256 columns a warp
-  RowShape s;
-  s.W = 1;
-  while (s.W * 4 < vec) s.W *= 2;
-  s.NV = (vec + s.W - 1) / s.W;
-  s.NV = s.NV == 3 ? 4 : s.NV;
-  s.warps = 8;
+  const int blocks = (D + 255) / 256;
+  RowShape s{1, blocks == 1 ? 1 : 2, 8};
+  while (s.W < 8 && s.W * s.NV < blocks) s.W *= 2;
+  if (s.W * s.NV < blocks) s.NV = 4;
   return s;
 }
 
@@ -701,7 +746,7 @@ int launch_fwd(const RowArgs& a, const RowShape& s, cudaStream_t stream) {
   constexpr int words = Ring<T, NV, DROP ? 2 : 1>::WORDS;
   const size_t smem = VEC ? sizeof(uint4) * ring_stages(words) * words * s.warps * 32 : 0;
   auto* kernel = ln_fwd_kernel<T, NV, VEC, DROP>;
-  if (smem > 48 * 1024)
+  if (smem > 32 * 1024)                            // with the static part, more than a launch gets unasked
     if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
   kernel<<<(int)(want < most ? want : most), s.warps * 32, smem, stream>>>(a);
   return (int)cudaGetLastError();
@@ -711,10 +756,10 @@ template <typename T, int NV, bool VEC, bool DROP>
 int launch_bwd(const RowArgs& a, const RowShape& s, cudaStream_t stream) {
   const int R = s.warps / s.W;
   constexpr int words = Ring<T, NV, DROP ? 3 : 2>::WORDS;
-  const size_t smem = (VEC ? sizeof(uint4) * ring_stages(words) * words * s.warps * 32 : 0) +
-                      (R > 1 ? (size_t)2 * a.D * sizeof(float) : 0);
+  const size_t ring = VEC ? sizeof(uint4) * ring_stages(words) * words * s.warps * 32 : 0;
+  const size_t sums = R > 1 ? (size_t)2 * a.D * sizeof(float) : 0, smem = ring > sums ? ring : sums;
   auto* kernel = ln_bwd_kernel<T, NV, VEC, DROP>;
-  if (smem > 48 * 1024)
+  if (smem > 32 * 1024)                            // with the static part, more than a launch gets unasked
     if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
   kernel<<<(int)a.partial_rows, s.warps * 32, smem, stream>>>(a);
   return (int)cudaGetLastError();
@@ -773,12 +818,12 @@ int launch_typed(const RowArgs& a, int op, cudaStream_t stream) {
 
 }  // namespace rows_impl
 
-// CTAs of the backward pass, a partial row each: one an SM (the ring and the sums in registers fill it)
+// CTAs of the backward pass, a partial row each: as many as are resident
 int row_partial_rows(int64_t M, int D) {
   const rows_impl::RowShape s = rows_impl::row_shape(D);
   const int R = s.warps / s.W;
-  const int64_t want = (M + R - 1) / R;
-  return (int)(want < device_sm_count() ? want : device_sm_count());
+  const int64_t want = (M + R - 1) / R, most = (s.NV < 4 ? 2 : 1) * device_sm_count();
+  return (int)(want < most ? want : most);
 }
 
 int launch_row_op(const RowArgs& args, int op, int dtype, cudaStream_t stream) {

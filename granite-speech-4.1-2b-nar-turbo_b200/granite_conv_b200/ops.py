@@ -37,7 +37,6 @@ import torch
 from . import _lib, training
 
 KERNEL_SIZE = 15
-LAYERNORM_WIDTHS = (256, 512, 1024, 2048)     # of the inference kernel (gsn_layernorm_bf16)
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -286,13 +285,6 @@ def layer_norm_op(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, eps
     """nn.LayerNorm over the last dim of x [..., D] (the block's post_norm, conformer.py:199, :209), differentiable; x
     bf16, fp16 or fp32, weight and bias fp32 or of x's type, D <= 8192.  lengths (int [B] beside x [B, T, D]): padding
     frames are not read and give 0."""
-    _require_cuda("granite::layer_norm", x, weight, bias)
-    D = x.shape[-1]
-    if (lengths is None and x.dtype == weight.dtype == bias.dtype == torch.bfloat16 and D in LAYERNORM_WIDTHS
-            and weight.is_contiguous() and bias.is_contiguous()
-            and not (weight.data_ptr() | bias.data_ptr() | x.data_ptr()) & 15):
-        x2 = x.contiguous().view(-1, D)
-        return layernorm(x2, weight, bias, eps).view(x.shape)
     return training._layer_norm(x, weight, bias, eps, lengths)
 
 

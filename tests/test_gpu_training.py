@@ -13,6 +13,7 @@ import pytest
 import torch
 
 import train_ref as R
+from granite_conv_b200 import ops
 from granite_conv_b200 import training as tr
 
 pytestmark = pytest.mark.gpu
@@ -120,10 +121,13 @@ def test_layer_norm_many_rows():
     assert all(torch.equal(a, c) for a, c in zip(out, again))
 
 
-def test_layer_norm_op_matches_inference_kernel():
-    """granite::layer_norm keeps the inference kernel where it ran before; the new one gives the same bits there."""
+def test_layer_norm_keeps_the_inference_kernel():
+    """What granite::layer_norm took before keeps its kernel and its bits, with and without a gradient to record."""
     x, w, b = rand(1, (2, 37, 1024), BF), rand(2, (1024,), BF, 0.1, 1.0), rand(3, (1024,), BF)
-    assert torch.equal(torch.ops.granite.layer_norm(x, w, b, EPS), tr.layer_norm(x, w, b, EPS))
+    old = ops.layernorm(x.view(-1, 1024), w, b, EPS).view(x.shape)
+    assert torch.equal(torch.ops.granite.layer_norm(x, w, b, EPS), old)
+    assert torch.equal(tr.layer_norm(x, w, b), old)
+    assert torch.equal(tr.layer_norm(x.requires_grad_(), w, b).detach(), old)
 
 
 def test_strides_and_alignment():
@@ -509,7 +513,7 @@ def test_training_step_against_formulas():
     share = 1.0 / (tl.double().cpu().clamp(min=1) * B)
     value = (rl * share).sum() + 1e-3 * h.square().mean()
     rgrads = torch.autograd.grad([logits, h], ref, [rg * share[:, None, None], 2e-3 * h.detach() / h.numel()])
-    assert abs(float(loss.detach()) - float(value)) < 1e-4 * abs(float(value))
+    assert abs(float(loss.detach()) - float(value.detach())) < 1e-4 * abs(float(value.detach()))
     for name, got, want in zip(("ff", "x", *par), grads, rgrads):
         # fp32 throughout: chain, norm and products leave about (64 T + D) roundings of the largest entry
         bound = (64 * T + 4 * D + 300) * E * want.abs().max() * 8
