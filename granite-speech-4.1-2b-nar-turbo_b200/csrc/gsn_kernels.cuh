@@ -177,7 +177,8 @@ struct RowArgs {
   int64_t M = 0;
   int D = 0, T = 0, groups = 0;  // groups = ceil(D / 8)
   float eps = 0.f;
-  int W = 1;                     // set by the launcher
+  int W = 1;                     // set by the launcher, as are the next two
+  uint32_t div_factor = 0, div_shift = 0;
 };
 int row_partial_rows(int64_t M, int D);
 int launch_row_op(const RowArgs& args, int op, int dtype, cudaStream_t stream);

@@ -271,54 +271,56 @@ __device__ __forceinline__ uint32_t keep_row(const Generator& g, uint64_t row_gr
 // ---- a row's warps ---------------------------------------------------------------------------------------------------
 constexpr int kMaxRowWarps = 8;
 
-// Sums of two values over the W warps of a row, the same in every lane and in the same order on every run.  `slot`
-// points at this row group's [2][kMaxRowWarps] exchange; it alternates, so one barrier a reduction is enough: a warp
-// that writes slot k again has passed the barrier behind the reads of it.
+// Sums over the W warps of a row, the same in every lane and in the same order on every run.  `slot` points at this row
+// group's exchange, [2 phases][2 values][8 warps], zeros where there is no warp; the phases alternate, so one barrier a
+// reduction is enough: a warp that writes a phase again has passed the barrier behind the reads of it.
 struct RowGroup {
   int W, sub, bar;
-  float2* slot;
+  float* slot;
   int phase;
 };
 
-__device__ __forceinline__ void row_sum2(RowGroup& g, float& a, float& b) {
+template <int N>
+__device__ __forceinline__ void row_sums(RowGroup& g, float (&v)[N]) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    b += __shfl_xor_sync(0xffffffffu, b, o);
-  }
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
   if (g.W > 1) {
-    float2* s = g.slot + g.phase * kMaxRowWarps;
-    g.phase ^= 1;
-    if ((threadIdx.x & 31) == 0) s[g.sub] = make_float2(a, b);
+    float* s = g.slot + g.phase;
+    g.phase ^= 2 * kMaxRowWarps;
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[i * kMaxRowWarps + g.sub] = v[i];
     asm volatile("bar.sync %0, %1;" ::"r"(g.bar), "r"(g.W * 32) : "memory");
-    a = 0.f;
-    b = 0.f;
-    for (int i = 0; i < g.W; ++i) {
-      const float2 v = s[i];
-      a += v.x;
-      b += v.y;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float4 lo = *reinterpret_cast<const float4*>(s + i * kMaxRowWarps);
+      v[i] = (lo.x + lo.y) + (lo.z + lo.w);
+      if (g.W > 4) {
+        const float4 hi = *reinterpret_cast<const float4*>(s + i * kMaxRowWarps + 4);
+        v[i] += (hi.x + hi.y) + (hi.z + hi.w);
+      }
     }
   }
 }
 
-__device__ __forceinline__ float row_sum(RowGroup& g, float a) {
+// The sum of a lane's pairs in four chains: a single one would wait for its own additions.
+template <int NV, typename F>
+__device__ __forceinline__ float2 lane_sum(F term) {
+  float2 c[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-  if (g.W > 1) {
-    float2* s = g.slot + g.phase * kMaxRowWarps;
-    g.phase ^= 1;
-    if ((threadIdx.x & 31) == 0) s[g.sub].x = a;
-    asm volatile("bar.sync %0, %1;" ::"r"(g.bar), "r"(g.W * 32) : "memory");
-    a = 0.f;
-    for (int i = 0; i < g.W; ++i) a += s[i].x;
-  }
-  return a;
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) c[k] = term(i, k, c[k]);
+  return add2(add2(c[0], c[1]), add2(c[2], c[3]));
 }
 
-__device__ __forceinline__ bool padding_row(const RowArgs& a, int row) {
+// row / T by a multiplication (the launcher sets the factor), for row < 2^31
+__device__ __forceinline__ bool padding_row(const RowArgs& a, uint32_t row) {
   if (a.lengths == nullptr) return false;
-  const int b = row / a.T;
-  return row - b * a.T >= __ldg(a.lengths + b);
+  const uint32_t b = (__umulhi(a.div_factor, row) + row) >> a.div_shift;
+  return (int)(row - b * (uint32_t)a.T) >= __ldg(a.lengths + b);
 }
 
 // Rows under way a warp: as many as leave two CTAs an SM (one where a lane holds 32 columns of fp32)
@@ -338,35 +340,45 @@ __device__ __forceinline__ void keep8(uint32_t keep, int i, float2 (&f)[4]) {
 // a warp: a row stays in registers between the two passes of its statistics, its weights for all rows of the warp.
 template <typename T, int NV, bool VEC, bool DROP>
 __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_fwd_kernel(RowArgs a) {
-  __shared__ float2 exchange[8][2 * kMaxRowWarps];
+  __shared__ __align__(16) float exchange[8][4 * kMaxRowWarps];
   extern __shared__ uint4 ring_slots[];
   constexpr int TENSORS = DROP ? 2 : 1, S = ring_stages(Ring<T, NV, TENSORS>::WORDS);
   const Ring<T, NV, TENSORS> ring{ring_slots};
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W, R = (blockDim.x >> 5) / W;
   const int group = warp / W;
+  (&exchange[0][0])[threadIdx.x] = 0.f;
   RowGroup rg{W, warp - group * W, 1 + group, exchange[group], 0};
   const int D = a.D;
   int base[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) base[i] = (i * W + rg.sub) * 256;
-  const int64_t stride = (int64_t)gridDim.x * R, first = (int64_t)blockIdx.x * R + group;
-  auto fetch = [&](int64_t row, int stage) {
-    if (VEC && row < a.M) {
-      const bool pad = padding_row(a, (int)row);
+  const uint32_t M = (uint32_t)a.M, stride = gridDim.x * R, first = blockIdx.x * R + group;
+  uint32_t ahead = first, pads = 0;                // the row to fetch next; bit s: stage s holds a padding row
+  const T* x_ahead = static_cast<const T*>(a.x) + first * a.ld_x;
+  const T* res_ahead = DROP ? static_cast<const T*>(a.residual) + first * a.ld_res : nullptr;
+  auto fetch = [&](int stage) {
+    pads &= ~(1u << stage);
+    if (ahead < M) {
+      const bool pad = padding_row(a, ahead);
+      pads |= (pad ? 1u : 0u) << stage;
+      if (VEC) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int col = base[i] + lane * 8;
-        if (!pad && !(DROP && a.drop_all)) ring.fetch(stage, 0, i, static_cast<const T*>(a.x) + row * a.ld_x, col, D);
-        if (DROP) ring.fetch(stage, 1, i, static_cast<const T*>(a.residual) + row * a.ld_res, col, D);
+        for (int i = 0; i < NV; ++i) {
+          const int col = base[i] + lane * 8;
+          if (!pad && !(DROP && a.drop_all)) ring.fetch(stage, 0, i, x_ahead, col, D);
+          if (DROP) ring.fetch(stage, 1, i, res_ahead, col, D);
+        }
+        x_ahead += stride * a.ld_x;
+        if (DROP) res_ahead += stride * a.ld_res;
       }
     }
-    copies_commit();
+    ahead += stride;
+    if (VEC) copies_commit();
   };
-  if (VEC) {
-    ring.clear(S);
+  if (VEC) ring.clear(S);
 #pragma unroll
-    for (int s = 0; s + 1 < S; ++s) fetch(first + s * stride, s);
-  }
+  for (int s = 0; s + 1 < S; ++s) fetch(s);
+  __syncthreads();                                 // the exchange is cleared
   float2 wv[NV][4], bv[NV][4];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -377,20 +389,18 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_fwd_kernel(RowArgs a) 
   if (DROP) gen = load_generator(a.rng, a.site);
   const float inv_d = 1.0f / D;
   int stage = 0;
-  for (int64_t row = first; row < a.M; row += stride) {
-    T* y = static_cast<T*>(a.y) + row * D;
-    const bool pad = padding_row(a, (int)row);
-    if (VEC) {
-      fetch(row + (S - 1) * stride, stage == 0 ? S - 1 : stage - 1);
-      copies_wait<S - 1>();
-    }
+  for (uint32_t row = first; row < M; row += stride) {
+    T* y = static_cast<T*>(a.y) + (int64_t)row * D;
+    fetch(stage == 0 ? S - 1 : stage - 1);
+    const bool pad = pads >> stage & 1;
+    if (VEC) copies_wait<S - 1>();
     float2 v[NV][4];
     auto input = [&](int tensor, const void* p, int64_t ld, int i, float2 (&f)[4]) {
       Vec8<T> r;
       if (VEC)
         ring.read(stage, tensor, i, r);
       else
-        load8<T, VEC>(static_cast<const T*>(p) + row * ld, base[i], lane, D, r);
+        load8<T, VEC>(static_cast<const T*>(p) + (int64_t)row * ld, base[i], lane, D, r);
       unpack(r, f);
     };
     if (DROP) {
@@ -407,7 +417,7 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_fwd_kernel(RowArgs a) 
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[i][k] = ffma2(f[k], both(a.factor), v[i][k]);
         }
-        store8<T, VEC>(static_cast<T*>(a.h_out) + row * D, base[i], lane, D, v[i]);
+        store8<T, VEC>(static_cast<T*>(a.h_out) + (int64_t)row * D, base[i], lane, D, v[i]);
       }
     } else if (!pad) {
 #pragma unroll
@@ -420,21 +430,18 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_fwd_kernel(RowArgs a) 
       for (int i = 0; i < NV; ++i) store8<T, VEC>(y, base[i], lane, D, zero);
       continue;
     }
-    float2 acc = both(0.f);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc = add2(acc, v[i][k]);    // columns past D are zero
-    const float mean = row_sum(rg, acc.x + acc.y) * inv_d;
-    acc = both(0.f);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        v[i][k] = add2(v[i][k], inside<VEC>(-mean, base[i], lane, k, D));
-        acc = ffma2(v[i][k], v[i][k], acc);
-      }
-    const float rstd = rsqrtf(fmaf(row_sum(rg, acc.x + acc.y), inv_d, a.eps));
+    // columns past D are zero
+    float2 acc = lane_sum<NV>([&](int i, int k, float2 c) { return add2(c, v[i][k]); });
+    float sum[1] = {acc.x + acc.y};
+    row_sums(rg, sum);
+    const float mean = sum[0] * inv_d;
+    acc = lane_sum<NV>([&](int i, int k, float2 c) {
+      v[i][k] = add2(v[i][k], inside<VEC>(-mean, base[i], lane, k, D));
+      return ffma2(v[i][k], v[i][k], c);
+    });
+    sum[0] = acc.x + acc.y;
+    row_sums(rg, sum);
+    const float rstd = rsqrtf(fmaf(sum[0], inv_d, a.eps));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float2 o[4];
@@ -452,38 +459,50 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_fwd_kernel(RowArgs a) 
 // order and leaves one partial row, so no sum depends on the order of arrival.
 template <typename T, int NV, bool VEC, bool DROP>
 __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_bwd_kernel(RowArgs a) {
-  __shared__ float2 exchange[8][2 * kMaxRowWarps];
+  __shared__ __align__(16) float exchange[8][4 * kMaxRowWarps];
   extern __shared__ uint4 ring_slots[];            // the ring; at the end [2][D], the CTA's sums
   constexpr int TENSORS = DROP ? 3 : 2, S = ring_stages(Ring<T, NV, TENSORS>::WORDS);
   const Ring<T, NV, TENSORS> ring{ring_slots};
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W, R = (blockDim.x >> 5) / W;
   const int group = warp / W;
+  (&exchange[0][0])[threadIdx.x] = 0.f;
   RowGroup rg{W, warp - group * W, 1 + group, exchange[group], 0};
   const int D = a.D;
   int base[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) base[i] = (i * W + rg.sub) * 256;
-  const int64_t stride = (int64_t)gridDim.x * R, first = (int64_t)blockIdx.x * R + group;
-  auto fetch = [&](int64_t row, int stage) {
-    if (VEC && row < a.M) {
-      const bool pad = padding_row(a, (int)row);
+  const uint32_t M = (uint32_t)a.M, stride = gridDim.x * R, first = blockIdx.x * R + group;
+  uint32_t ahead = first, pads = 0;                // the row to fetch next; bit s: stage s holds a padding row
+  const T* x_ahead = static_cast<const T*>(a.x) + first * a.ld_x;
+  const T* dy_ahead = static_cast<const T*>(a.dy) + first * a.ld_dy;
+  const T* dh_ahead = DROP && a.dh ? static_cast<const T*>(a.dh) + first * a.ld_dh : nullptr;
+  auto fetch = [&](int stage) {
+    pads &= ~(1u << stage);
+    if (ahead < M) {
+      const bool pad = padding_row(a, ahead);
+      pads |= (pad ? 1u : 0u) << stage;
+      if (VEC) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int col = base[i] + lane * 8;
-        if (!pad) {
-          ring.fetch(stage, 0, i, static_cast<const T*>(a.x) + row * a.ld_x, col, D);
-          ring.fetch(stage, 1, i, static_cast<const T*>(a.dy) + row * a.ld_dy, col, D);
+        for (int i = 0; i < NV; ++i) {
+          const int col = base[i] + lane * 8;
+          if (!pad) {
+            ring.fetch(stage, 0, i, x_ahead, col, D);
+            ring.fetch(stage, 1, i, dy_ahead, col, D);
+          }
+          if (DROP && dh_ahead) ring.fetch(stage, TENSORS - 1, i, dh_ahead, col, D);
         }
-        if (DROP && a.dh) ring.fetch(stage, TENSORS - 1, i, static_cast<const T*>(a.dh) + row * a.ld_dh, col, D);
+        x_ahead += stride * a.ld_x;
+        dy_ahead += stride * a.ld_dy;
+        if (DROP && dh_ahead) dh_ahead += stride * a.ld_dh;
       }
     }
-    copies_commit();
+    ahead += stride;
+    if (VEC) copies_commit();
   };
-  if (VEC) {
-    ring.clear(S);                                 // and zeros stand in for a missing dh
+  if (VEC) ring.clear(S);                          // and zeros stand in for a missing dh
 #pragma unroll
-    for (int s = 0; s + 1 < S; ++s) fetch(first + s * stride, s);
-  }
+  for (int s = 0; s + 1 < S; ++s) fetch(s);
+  __syncthreads();                                 // the exchange is cleared
   float2 wv[NV][4], dw[NV][4], db[NV][4];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -495,14 +514,12 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_bwd_kernel(RowArgs a) 
   if (DROP) gen = load_generator(a.rng, a.site);
   const float inv_d = 1.0f / D;
   int stage = 0;
-  for (int64_t row = first; row < a.M; row += stride) {
-    T* dx = static_cast<T*>(a.dx) + row * D;
-    T* dres = DROP ? static_cast<T*>(a.dres) + row * D : nullptr;
-    const bool pad = padding_row(a, (int)row);
-    if (VEC) {
-      fetch(row + (S - 1) * stride, stage == 0 ? S - 1 : stage - 1);
-      copies_wait<S - 1>();
-    }
+  for (uint32_t row = first; row < M; row += stride) {
+    T* dx = static_cast<T*>(a.dx) + (int64_t)row * D;
+    T* dres = DROP ? static_cast<T*>(a.dres) + (int64_t)row * D : nullptr;
+    fetch(stage == 0 ? S - 1 : stage - 1);
+    const bool pad = pads >> stage & 1;
+    if (VEC) copies_wait<S - 1>();
     const int here = stage;
     stage = stage + 1 == S ? 0 : stage + 1;
     auto input = [&](int tensor, const void* p, int64_t ld, int i, float2 (&f)[4]) {
@@ -510,7 +527,7 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_bwd_kernel(RowArgs a) 
       if (VEC)
         ring.read(here, tensor, i, r);
       else
-        load8<T, VEC>(static_cast<const T*>(p) + row * ld, base[i], lane, D, r);
+        load8<T, VEC>(static_cast<const T*>(p) + (int64_t)row * ld, base[i], lane, D, r);
       unpack(r, f);
     };
     auto input_dh = [&](int i, float2 (&f)[4]) {
@@ -534,36 +551,28 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_bwd_kernel(RowArgs a) 
       }
       continue;
     }
-    float2 x[NV][4], g[NV][4], sx = both(0.f), s0 = both(0.f);
+    float2 x[NV][4], g[NV][4];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       input(0, a.x, a.ld_x, i, x[i]);
       input(1, a.dy, a.ld_dy, i, g[i]);
     }
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {                // columns past D are zero in x and dy
-        sx = add2(sx, x[i][k]);
-        s0 = ffma2(g[i][k], wv[i][k], s0);
-      }
-    float sum_x = sx.x + sx.y, sum_g = s0.x + s0.y;
-    row_sum2(rg, sum_x, sum_g);
-    const float mean = sum_x * inv_d;
-    float2 s1 = both(0.f), s2 = both(0.f);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        x[i][k] = add2(x[i][k], inside<VEC>(-mean, base[i], lane, k, D));
-        s1 = ffma2(x[i][k], x[i][k], s1);
-        s2 = ffma2(mul2(g[i][k], wv[i][k]), x[i][k], s2);
-      }
-    float sum_dd = s1.x + s1.y, sum_gd = s2.x + s2.y;
-    row_sum2(rg, sum_dd, sum_gd);
-    const float rstd = rsqrtf(fmaf(sum_dd, inv_d, a.eps));
-    const float2 r2 = both(rstd), c1 = both(-rstd * (sum_g * inv_d));
-    const float2 c2 = both(-rstd * rstd * rstd * (sum_gd * inv_d));
+    // columns past D are zero in x and dy
+    float2 p = lane_sum<NV>([&](int i, int k, float2 c) { return add2(c, x[i][k]); });
+    float2 q = lane_sum<NV>([&](int i, int k, float2 c) { return ffma2(g[i][k], wv[i][k], c); });
+    float sum[2] = {p.x + p.y, q.x + q.y};
+    row_sums(rg, sum);
+    const float mean = sum[0] * inv_d, mean_g = sum[1] * inv_d;
+    p = lane_sum<NV>([&](int i, int k, float2 c) {
+      x[i][k] = add2(x[i][k], inside<VEC>(-mean, base[i], lane, k, D));
+      return ffma2(x[i][k], x[i][k], c);
+    });
+    q = lane_sum<NV>([&](int i, int k, float2 c) { return ffma2(mul2(g[i][k], wv[i][k]), x[i][k], c); });
+    sum[0] = p.x + p.y;
+    sum[1] = q.x + q.y;
+    row_sums(rg, sum);
+    const float rstd = rsqrtf(fmaf(sum[0], inv_d, a.eps));
+    const float2 r2 = both(rstd), c1 = both(-rstd * mean_g), c2 = both(-rstd * rstd * rstd * (sum[1] * inv_d));
     uint32_t keep = 0;
     if (DROP && !a.drop_all)
       keep = keep_row<NV, VEC>(gen, (uint64_t)row * a.groups, base, lane, a.threshold << 16);
@@ -680,7 +689,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(RowArgs a, int64_t group0,
       const uint32_t r = g / (uint32_t)a.groups;   // group0 begins a row
       row[u] = group0 / a.groups + r;
       col[u] = (int)(g - r * (uint32_t)a.groups) * 8;
-      use[u] = use[u] && !padding_row(a, (int)row[u]);
+      use[u] = use[u] && !padding_row(a, (uint32_t)row[u]);
     }
     if (use[u]) get(a.x, a.ld_x, u, xq[u]);
     if (RES && there[u]) get(a.residual, a.ld_res, u, rq[u]);
@@ -798,8 +807,12 @@ int launch_dropout(const RowArgs& a, bool vec, cudaStream_t stream) {
 }
 
 template <typename T>
-int launch_typed(const RowArgs& a, int op, cudaStream_t stream) {
+int launch_typed(RowArgs a, int op, cudaStream_t stream) {
   const bool vec = vec_ok(a, sizeof(T));
+  if (a.lengths) {                                 // row / T = (umulhi(factor, row) + row) >> shift
+    while (((uint64_t)1 << a.div_shift) < (uint64_t)a.T) ++a.div_shift;
+    a.div_factor = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << a.div_shift) - a.T)) / a.T + 1);
+  }
   if (op == kRowDropout) return a.residual ? launch_dropout<T, true>(a, vec, stream) : launch_dropout<T, false>(a, vec, stream);
   const bool drop = op == kRowDropNorm || op == kRowDropNormGrad, bwd = op == kRowNormGrad || op == kRowDropNormGrad;
   if (a.M > 0) {
