@@ -104,27 +104,32 @@ __device__ __forceinline__ void pack(const float (&f)[8], Vec8<T>& r) {
   pack(p, r);
 }
 
-// A warp's block of 256 columns: lane l holds eight of them.  VEC (rows aligned to 16 bytes, D % 8 == 0): columns
-// 8 l .. 8 l + 7, one 16-byte word of a 16-bit type.  Otherwise columns l + 32 k, so that single elements still make
-// whole 32-byte sectors.
-template <bool VEC>
+// A warp's block of 256 columns: lane l holds eight of them.  VEC (rows aligned to 16 bytes, D % 8 == 0): of a 16-bit
+// type columns 8 l .. 8 l + 7, of fp32 columns 4 l .. 4 l + 3 and 128 further on: one and two 16-byte words, a warp's
+// words without a gap.  Otherwise columns l + 32 k, so that single elements still make whole 32-byte sectors.
+template <typename T, bool VEC>
 __device__ __forceinline__ int column(int base, int lane, int k) {
-  return VEC ? base + lane * 8 + k : base + k * 32 + lane;
+  if (!VEC) return base + k * 32 + lane;
+  return sizeof(T) == 2 ? base + lane * 8 + k : base + (k >> 2) * 128 + lane * 4 + (k & 3);
 }
+// the first column of 16-byte word q (VEC)
+template <typename T>
+__device__ __forceinline__ int word_column(int base, int lane, int q) { return column<T, true>(base, lane, q * 4); }
 
 // columns past D read as zero
 template <typename T, bool VEC>
 __device__ __forceinline__ void load8(const T* __restrict__ row, int base, int lane, int D, Vec8<T>& r) {
   if (VEC) {
-    const int col = base + lane * 8;
 #pragma unroll
-    for (int i = 0; i < Vec8<T>::Q; ++i)
-      r.q[i] = col < D ? __ldg(reinterpret_cast<const uint4*>(row + col) + i) : make_uint4(0, 0, 0, 0);
+    for (int q = 0; q < Vec8<T>::Q; ++q) {
+      const int col = word_column<T>(base, lane, q);
+      r.q[q] = col < D ? __ldg(reinterpret_cast<const uint4*>(row + col)) : make_uint4(0, 0, 0, 0);
+    }
   } else {
     float f[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int col = column<VEC>(base, lane, k);
+      const int col = column<T, VEC>(base, lane, k);
       f[k] = col < D ? to_f32(row[col]) : 0.f;
     }
     pack(f, r);                     // exact: the values are of type T
@@ -134,16 +139,17 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, int base, int l
 template <typename T, bool VEC>
 __device__ __forceinline__ void store8(T* __restrict__ row, int base, int lane, int D, const float2 (&f)[4]) {
   if (VEC) {
-    const int col = base + lane * 8;
-    if (col >= D) return;
     Vec8<T> r;
     pack(f, r);
 #pragma unroll
-    for (int i = 0; i < Vec8<T>::Q; ++i) *(reinterpret_cast<uint4*>(row + col) + i) = r.q[i];
+    for (int q = 0; q < Vec8<T>::Q; ++q) {
+      const int col = word_column<T>(base, lane, q);
+      if (col < D) *reinterpret_cast<uint4*>(row + col) = r.q[q];
+    }
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int col = column<VEC>(base, lane, k);
+      const int col = column<T, VEC>(base, lane, k);
       if (col < D) row[col] = from_f32<T>(k & 1 ? f[k / 2].y : f[k / 2].x);
     }
   }
@@ -155,18 +161,18 @@ __device__ __forceinline__ void load_param8(const void* p, int fp32, int base, i
   float v[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const int c = column<VEC>(base, lane, k);
+    const int c = column<T, VEC>(base, lane, k);
     v[k] = c >= D ? 0.f : fp32 ? __ldg(static_cast<const float*>(p) + c) : to_f32(static_cast<const T*>(p)[c]);
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) f[k] = make_float2(v[2 * k], v[2 * k + 1]);
 }
 
-// v where the column is inside the row, else 0
-template <bool VEC>
+// v where the columns of pair k are inside the row, else 0
+template <typename T, bool VEC>
 __device__ __forceinline__ float2 inside(float v, int base, int lane, int k, int D) {
-  if (VEC) return both(base + lane * 8 < D ? v : 0.f);
-  return make_float2(column<VEC>(base, lane, 2 * k) < D ? v : 0.f, column<VEC>(base, lane, 2 * k + 1) < D ? v : 0.f);
+  if (VEC) return both(column<T, true>(base, lane, 2 * k) < D ? v : 0.f);
+  return make_float2(column<T, VEC>(base, lane, 2 * k) < D ? v : 0.f, column<T, VEC>(base, lane, 2 * k + 1) < D ? v : 0.f);
 }
 
 __device__ __forceinline__ void copy16(void* smem, const void* gmem) {
@@ -182,11 +188,13 @@ struct Ring {
   __device__ __forceinline__ uint4* at(int stage, int tensor, int i) const {
     return slots + ((stage * TENSORS + tensor) * NV + i) * Q * blockDim.x + threadIdx.x;
   }
-  __device__ __forceinline__ void fetch(int stage, int tensor, int i, const T* row, int col, int D) const {
+  __device__ __forceinline__ void fetch(int stage, int tensor, int i, const T* row, int base, int lane, int D) const {
     uint4* dst = at(stage, tensor, i);
-    if (col < D)
 #pragma unroll
-      for (int q = 0; q < Q; ++q) copy16(dst + q * blockDim.x, reinterpret_cast<const uint4*>(row + col) + q);
+    for (int q = 0; q < Q; ++q) {
+      const int col = word_column<T>(base, lane, q);
+      if (col < D) copy16(dst + q * blockDim.x, row + col);
+    }
   }
   __device__ __forceinline__ void read(int stage, int tensor, int i, Vec8<T>& r) const {
     const uint4* src = at(stage, tensor, i);
@@ -250,16 +258,24 @@ __device__ __forceinline__ uint32_t keep_bits(const Generator& g, uint64_t group
 }
 
 // The keep bits of a lane's elements of NV blocks, eight a block: bit 8 i + k.  The generator's groups are neighbours,
-// so without VEC a lane's elements belong to eight groups, drawn by eight lanes.
-template <int NV, bool VEC>
+// so fp32's two halves belong to two groups, single elements to eight, each drawn by another lane.
+template <typename T, int NV, bool VEC>
 __device__ __forceinline__ uint32_t keep_row(const Generator& g, uint64_t row_group, const int (&base)[NV], int lane,
                                              uint32_t threshold16) {
   static_assert(NV <= 4, "eight bits a block in one word");
   uint32_t own = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) own |= keep_bits(g, row_group + (base[i] >> 3) + lane, threshold16) << (8 * i);
-  if (VEC) return own;
+  if (VEC && sizeof(T) == 2) return own;
   uint32_t bits = 0;
+  if (VEC) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {                  // columns base + 128 q + 4 l: group 16 q + l / 2, its half l % 2
+      const uint32_t w = __shfl_sync(0xffffffffu, own, 16 * q + (lane >> 1)) >> (4 * (lane & 1));
+      bits |= (w & 0x0F0F0F0Fu) << (4 * q);
+    }
+    return bits;
+  }
 #pragma unroll
   for (int k = 0; k < 8; ++k) {                    // column base + 32 k + lane: group 4 k + lane / 8, its bit lane % 8
     const uint32_t w = __shfl_sync(0xffffffffu, own, 4 * k + (lane >> 3)) >> (lane & 7);
@@ -364,9 +380,8 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_fwd_kernel(RowArgs a) 
       if (VEC) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          const int col = base[i] + lane * 8;
-          if (!pad && !(DROP && a.drop_all)) ring.fetch(stage, 0, i, x_ahead, col, D);
-          if (DROP) ring.fetch(stage, 1, i, res_ahead, col, D);
+          if (!pad && !(DROP && a.drop_all)) ring.fetch(stage, 0, i, x_ahead, base[i], lane, D);
+          if (DROP) ring.fetch(stage, 1, i, res_ahead, base[i], lane, D);
         }
         x_ahead += stride * a.ld_x;
         if (DROP) res_ahead += stride * a.ld_res;
@@ -406,7 +421,7 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_fwd_kernel(RowArgs a) 
     if (DROP) {
       const bool add = !pad && !a.drop_all;
       uint32_t keep = 0;
-      if (add) keep = keep_row<NV, VEC>(gen, (uint64_t)row * a.groups, base, lane, a.threshold << 16);
+      if (add) keep = keep_row<T, NV, VEC>(gen, (uint64_t)row * a.groups, base, lane, a.threshold << 16);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         input(1, a.residual, a.ld_res, i, v[i]);
@@ -436,7 +451,7 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_fwd_kernel(RowArgs a) 
     row_sums(rg, sum);
     const float mean = sum[0] * inv_d;
     acc = lane_sum<NV>([&](int i, int k, float2 c) {
-      v[i][k] = add2(v[i][k], inside<VEC>(-mean, base[i], lane, k, D));
+      v[i][k] = add2(v[i][k], inside<T, VEC>(-mean, base[i], lane, k, D));
       return ffma2(v[i][k], v[i][k], c);
     });
     sum[0] = acc.x + acc.y;
@@ -484,12 +499,11 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_bwd_kernel(RowArgs a) 
       if (VEC) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          const int col = base[i] + lane * 8;
           if (!pad) {
-            ring.fetch(stage, 0, i, x_ahead, col, D);
-            ring.fetch(stage, 1, i, dy_ahead, col, D);
+            ring.fetch(stage, 0, i, x_ahead, base[i], lane, D);
+            ring.fetch(stage, 1, i, dy_ahead, base[i], lane, D);
           }
-          if (DROP && dh_ahead) ring.fetch(stage, TENSORS - 1, i, dh_ahead, col, D);
+          if (DROP && dh_ahead) ring.fetch(stage, TENSORS - 1, i, dh_ahead, base[i], lane, D);
         }
         x_ahead += stride * a.ld_x;
         dy_ahead += stride * a.ld_dy;
@@ -564,7 +578,7 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_bwd_kernel(RowArgs a) 
     row_sums(rg, sum);
     const float mean = sum[0] * inv_d, mean_g = sum[1] * inv_d;
     p = lane_sum<NV>([&](int i, int k, float2 c) {
-      x[i][k] = add2(x[i][k], inside<VEC>(-mean, base[i], lane, k, D));
+      x[i][k] = add2(x[i][k], inside<T, VEC>(-mean, base[i], lane, k, D));
       return ffma2(x[i][k], x[i][k], c);
     });
     q = lane_sum<NV>([&](int i, int k, float2 c) { return ffma2(mul2(g[i][k], wv[i][k]), x[i][k], c); });
@@ -575,7 +589,7 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_bwd_kernel(RowArgs a) 
     const float2 r2 = both(rstd), c1 = both(-rstd * mean_g), c2 = both(-rstd * rstd * rstd * (sum[1] * inv_d));
     uint32_t keep = 0;
     if (DROP && !a.drop_all)
-      keep = keep_row<NV, VEC>(gen, (uint64_t)row * a.groups, base, lane, a.threshold << 16);
+      keep = keep_row<T, NV, VEC>(gen, (uint64_t)row * a.groups, base, lane, a.threshold << 16);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float2 o[4];
@@ -609,7 +623,7 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_bwd_kernel(RowArgs a) 
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const int c = column<VEC>(base[i], lane, k);
+          const int c = column<T, VEC>(base[i], lane, k);
           if (c >= D) continue;
           float sw = k & 1 ? dw[i][k / 2].y : dw[i][k / 2].x, sb = k & 1 ? db[i][k / 2].y : db[i][k / 2].x;
           if (g > 0) {
