@@ -222,31 +222,53 @@ struct Generator {
   uint32_t k0, k1, offset, site;
 };
 
-__device__ __forceinline__ uint4 philox(const Generator& g, uint64_t group) {
-  uint32_t c0 = (uint32_t)group, c1 = (uint32_t)(group >> 32), c2 = g.offset, c3 = g.site;
-  uint32_t k0 = g.k0, k1 = g.k1;
-#pragma unroll
-  for (int i = 0; i < 10; ++i) {
-    const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
-    c1 = (uint32_t)b;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
-    c3 = (uint32_t)a;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
-  }
-  return make_uint4(c0, c1, c2, c3);
-}
-
 __device__ __forceinline__ Generator load_generator(const int64_t* rng, uint32_t site) {
   const uint64_t seed = (uint64_t)__ldg(reinterpret_cast<const long long*>(rng));
   const uint64_t offset = (uint64_t)__ldg(reinterpret_cast<const long long*>(rng) + 1);
   return Generator{(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)offset, site};
 }
 
-// bit j: element j of the group is kept (its 16-bit number is not below the threshold, given shifted up by 16)
-__device__ __forceinline__ uint32_t keep_bits(const Generator& g, uint64_t group, uint32_t threshold16) {
-  const uint4 r = philox(g, group);
+// the eight numbers of N groups at a time, round by round: the keys of a round are formed once
+template <int N>
+__device__ __forceinline__ void philox(const Generator& g, const uint64_t (&group)[N], uint4 (&out)[N]) {
+  uint32_t c0[N], c1[N], c2[N], c3[N], k0 = g.k0, k1 = g.k1;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    c0[n] = (uint32_t)group[n];
+    c1[n] = (uint32_t)(group[n] >> 32);
+    c2[n] = g.offset;
+    c3[n] = g.site;
+  }
+#pragma unroll
+  for (int i = 0; i < 10; ++i) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const uint64_t a = (uint64_t)0xD2511F53u * c0[n], b = (uint64_t)0xCD9E8D57u * c2[n];
+      c0[n] = (uint32_t)(b >> 32) ^ c1[n] ^ k0;
+      c1[n] = (uint32_t)b;
+      c2[n] = (uint32_t)(a >> 32) ^ c3[n] ^ k1;
+      c3[n] = (uint32_t)a;
+    }
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) out[n] = make_uint4(c0[n], c1[n], c2[n], c3[n]);
+}
+
+// The kept ones of a group's eight elements in their order, the others 0 (chosen, not multiplied: a dropped infinity is
+// gone).  An element is kept where its 16-bit number is not below the threshold, given shifted up by 16.
+__device__ __forceinline__ void keep8(const uint4& r, uint32_t threshold16, float2 (&f)[4]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    f[k].x = (w[k] << 16) >= threshold16 ? f[k].x : 0.f;
+    f[k].y = w[k] >= threshold16 ? f[k].y : 0.f;
+  }
+}
+
+// the same as bits, number j in bit j
+__device__ __forceinline__ uint32_t keep_bits(const uint4& r, uint32_t threshold16) {
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
   uint32_t bits = 0;
 #pragma unroll
@@ -257,32 +279,56 @@ __device__ __forceinline__ uint32_t keep_bits(const Generator& g, uint64_t group
   return bits;
 }
 
-// The keep bits of a lane's elements of NV blocks, eight a block: bit 8 i + k.  The generator's groups are neighbours,
-// so fp32's two halves belong to two groups, single elements to eight, each drawn by another lane.
+// Which of a lane's elements of NV blocks are kept.  The generator's groups are neighbours, so a 16-bit type's eight
+// elements a block are a group; fp32's two halves belong to two groups and single elements to eight, drawn by other
+// lanes: there the answers travel as bits, 8 i + k.
 template <typename T, int NV, bool VEC>
-__device__ __forceinline__ uint32_t keep_row(const Generator& g, uint64_t row_group, const int (&base)[NV], int lane,
-                                             uint32_t threshold16) {
-  static_assert(NV <= 4, "eight bits a block in one word");
-  uint32_t own = 0;
+struct Kept {
+  static constexpr bool OWN = VEC && sizeof(T) == 2;
+  uint4 drawn[OWN ? NV : 1];
+  uint32_t bits;
+
+  __device__ __forceinline__ void draw(const Generator& g, uint64_t row_group, const int (&base)[NV], int lane,
+                                       uint32_t threshold16) {
+    static_assert(NV <= 4, "eight bits a block in one word");
+    uint64_t group[NV];
+    uint4 r[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) own |= keep_bits(g, row_group + (base[i] >> 3) + lane, threshold16) << (8 * i);
-  if (VEC && sizeof(T) == 2) return own;
-  uint32_t bits = 0;
-  if (VEC) {
+    for (int i = 0; i < NV; ++i) group[i] = row_group + (base[i] >> 3) + lane;
+    philox(g, group, r);
+    if (OWN) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {                  // columns base + 128 q + 4 l: group 16 q + l / 2, its half l % 2
-      const uint32_t w = __shfl_sync(0xffffffffu, own, 16 * q + (lane >> 1)) >> (4 * (lane & 1));
-      bits |= (w & 0x0F0F0F0Fu) << (4 * q);
+      for (int i = 0; i < NV; ++i) drawn[OWN ? i : 0] = r[i];
+      return;
     }
-    return bits;
-  }
+    uint32_t own = 0;
+    bits = 0;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {                    // column base + 32 k + lane: group 4 k + lane / 8, its bit lane % 8
-    const uint32_t w = __shfl_sync(0xffffffffu, own, 4 * k + (lane >> 3)) >> (lane & 7);
-    bits |= (w & 0x01010101u) << k;
+    for (int i = 0; i < NV; ++i) own |= keep_bits(r[i], threshold16) << (8 * i);
+    if (VEC) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {                // columns base + 128 q + 4 l: group 16 q + l / 2, its half l % 2
+        const uint32_t w = __shfl_sync(0xffffffffu, own, 16 * q + (lane >> 1)) >> (4 * (lane & 1));
+        bits |= (w & 0x0F0F0F0Fu) << (4 * q);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {                // column base + 32 k + lane: group 4 k + lane / 8, its bit lane % 8
+        const uint32_t w = __shfl_sync(0xffffffffu, own, 4 * k + (lane >> 3)) >> (lane & 7);
+        bits |= (w & 0x01010101u) << k;
+      }
+    }
   }
-  return bits;
-}
+
+  __device__ __forceinline__ void apply(int i, uint32_t threshold16, float2 (&f)[4]) const {
+    if (OWN) return keep8(drawn[OWN ? i : 0], threshold16, f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f[k].x = bits & (1u << (8 * i + 2 * k)) ? f[k].x : 0.f;
+      f[k].y = bits & (2u << (8 * i + 2 * k)) ? f[k].y : 0.f;
+    }
+  }
+};
 
 // ---- a row's warps ---------------------------------------------------------------------------------------------------
 constexpr int kMaxRowWarps = 8;
@@ -341,16 +387,6 @@ __device__ __forceinline__ bool padding_row(const RowArgs& a, uint32_t row) {
 
 // Rows under way a warp: as many as leave two CTAs an SM (one where a lane holds 32 columns of fp32)
 __host__ __device__ constexpr int ring_stages(int words) { return words <= 6 ? 4 : words <= 8 ? 3 : 2; }
-
-// The kept ones of eight elements, the others 0 (chosen, not multiplied: a dropped infinity is gone).  `keep`: bits
-// 8 i + k.
-__device__ __forceinline__ void keep8(uint32_t keep, int i, float2 (&f)[4]) {
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    f[k].x = keep & (1u << (8 * i + 2 * k)) ? f[k].x : 0.f;
-    f[k].y = keep & (2u << (8 * i + 2 * k)) ? f[k].y : 0.f;
-  }
-}
 
 // LayerNorm forward; DROP: of h = residual + dropout(x), which is stored too.  W warps a row, NV blocks of 256 columns
 // a warp: a row stays in registers between the two passes of its statistics, its weights for all rows of the warp.
@@ -420,15 +456,15 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_fwd_kernel(RowArgs a) 
     };
     if (DROP) {
       const bool add = !pad && !a.drop_all;
-      uint32_t keep = 0;
-      if (add) keep = keep_row<T, NV, VEC>(gen, (uint64_t)row * a.groups, base, lane, a.threshold << 16);
+      Kept<T, NV, VEC> kept;
+      if (add) kept.draw(gen, (uint64_t)row * a.groups, base, lane, a.threshold << 16);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         input(1, a.residual, a.ld_res, i, v[i]);
         if (add) {
           float2 f[4];
           input(0, a.x, a.ld_x, i, f);
-          keep8(keep, i, f);
+          kept.apply(i, a.threshold << 16, f);
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[i][k] = ffma2(f[k], both(a.factor), v[i][k]);
         }
@@ -587,9 +623,8 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_bwd_kernel(RowArgs a) 
     row_sums(rg, sum);
     const float rstd = rsqrtf(fmaf(sum[0], inv_d, a.eps));
     const float2 r2 = both(rstd), c1 = both(-rstd * mean_g), c2 = both(-rstd * rstd * rstd * (sum[1] * inv_d));
-    uint32_t keep = 0;
-    if (DROP && !a.drop_all)
-      keep = keep_row<T, NV, VEC>(gen, (uint64_t)row * a.groups, base, lane, a.threshold << 16);
+    Kept<T, NV, VEC> kept;
+    if (DROP && !a.drop_all) kept.draw(gen, (uint64_t)row * a.groups, base, lane, a.threshold << 16);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float2 o[4];
@@ -606,7 +641,12 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_bwd_kernel(RowArgs a) 
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = add2(o[k], f[k]);
         store8<T, VEC>(dres, base[i], lane, D, o);
-        keep8(keep, i, o);
+        if (a.drop_all) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[k] = both(0.f);
+        } else {
+          kept.apply(i, a.threshold << 16, o);
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = mul2(o[k], both(a.factor));
       }
@@ -680,8 +720,8 @@ __global__ void __launch_bounds__(256) dropout_kernel(RowArgs a, int64_t group0,
   const uint32_t block0 = blockIdx.x * (256u * kDropUnroll) + threadIdx.x;
   Vec8<T> xq[kDropUnroll], rq[kDropUnroll];
   bool there[kDropUnroll], use[kDropUnroll];
-  int64_t row[kDropUnroll];
-  int col[kDropUnroll];
+  int64_t row[kDropUnroll] = {};
+  int col[kDropUnroll] = {};
   auto get = [&](const void* p, int64_t ld, int u, Vec8<T>& q) {
     if (VEC) {
       const T* src = static_cast<const T*>(p) + (FLAT ? (group0 + block0 + u * 256u) * 8 : row[u] * ld + col[u]);
@@ -709,16 +749,21 @@ __global__ void __launch_bounds__(256) dropout_kernel(RowArgs a, int64_t group0,
     if (RES && there[u]) get(a.residual, a.ld_res, u, rq[u]);
   }
   const Generator gen = load_generator(a.rng, a.site);
+  uint64_t groups[kDropUnroll];
+  uint4 drawn[kDropUnroll];
+#pragma unroll
+  for (int u = 0; u < kDropUnroll; ++u) groups[u] = group0 + block0 + u * 256u;
+  philox(gen, groups, drawn);
 #pragma unroll
   for (int u = 0; u < kDropUnroll; ++u) {
     if (!there[u]) continue;
-    const uint64_t group = group0 + block0 + u * 256u;
+    const uint64_t group = groups[u];
     float2 v[4] = {};
     if (RES) unpack(rq[u], v);
     if (use[u]) {
       float2 f[4];
       unpack(xq[u], f);
-      keep8(keep_bits(gen, group, a.threshold << 16), 0, f);
+      keep8(drawn[u], a.threshold << 16, f);
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] = RES ? ffma2(f[k], both(a.factor), v[k]) : mul2(f[k], both(a.factor));
     }
