@@ -89,6 +89,42 @@ int check_ctc(const char* name, int B, int T, int V, int S, int64_t ld_b, int64_
   return B == 0 ? -1 : 0;
 }
 
+CtcArgs ctc_args(const void* logits, int64_t ld_b, int64_t ld_t, const int32_t* targets, const int32_t* input_lengths,
+                 const int32_t* target_lengths, int B, int T, int V, int S, int blank, int zero_infinity) {
+  CtcArgs a;
+  a.logits = logits;
+  a.ld_b = ld_b;
+  a.ld_t = ld_t;
+  a.targets = targets;
+  a.input_lengths = input_lengths;
+  a.target_lengths = target_lengths;
+  a.B = B;
+  a.T = T;
+  a.V = V;
+  a.S = S;
+  a.blank = blank;
+  a.zero_infinity = zero_infinity;
+  a.pitch = ctc_pitch(S);
+  a.state_pitch = ctc_state_pitch(S);
+  return a;
+}
+
+// what the forward pass leaves for the backward pass, in one buffer
+int set_state(const char* name, CtcArgs& a, void* state, size_t bytes) {
+  const size_t need = gsn_ctc_loss_state_bytes(a.B, a.T, a.S);
+  if (bytes < need) return fail(GSN_ERR_WORKSPACE, "%s: state %zu < %zu bytes", name, bytes, need);
+  if (!state || !aligned(state, 16)) return fail(GSN_ERR_INVALID_ARG, "%s: state must be 16-byte aligned", name);
+  char* p = static_cast<char*>(state);
+  a.raw_loss = (float*)p;
+  p += align256(a.B * sizeof(float));
+  a.stats = (float2*)p;
+  p += align256((size_t)a.B * a.T * sizeof(float2));
+  a.order = (int2*)p;
+  p += align256((size_t)a.B * a.pitch * sizeof(int2));
+  a.post = (float*)p;
+  return 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -221,7 +257,12 @@ int gsn_dropout_add_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* dh
   return finish(launch_row_op(a, kRowDropNormGrad, dtype, (cudaStream_t)stream), name);
 }
 
-int gsn_ctc_loss_pitch(int S) { return S < 0 ? 0 : ctc_pitch(S); }
+size_t gsn_ctc_loss_state_bytes(int B, int T, int S) {
+  if (B <= 0 || T < 0 || S < 0 || S > kMaxCtcLabels) return 0;
+  const size_t frames = (size_t)B * T, pitch = ctc_pitch(S);
+  return align256(B * sizeof(float)) + align256(frames * sizeof(float2)) + align256(B * pitch * sizeof(int2)) +
+         align256(frames * pitch * sizeof(float));
+}
 
 size_t gsn_ctc_loss_workspace_bytes(int B, int T, int S, int gradient) {
   if (B <= 0 || T < 0 || S < 0 || S > kMaxCtcLabels) return 0;
@@ -233,39 +274,19 @@ size_t gsn_ctc_loss_workspace_bytes(int B, int T, int S, int gradient) {
 
 int gsn_ctc_loss_fwd(const void* logits, int64_t ld_b, int64_t ld_t, const int32_t* targets,
                      const int32_t* input_lengths, const int32_t* target_lengths, int B, int T, int V, int S, int blank,
-                     int zero_infinity, int gradient, int dtype, float* loss, float* raw_loss, float* stats,
-                     float* posteriors, int32_t* order, void* workspace, size_t workspace_bytes, gsn_stream_t stream) {
+                     int zero_infinity, int gradient, int dtype, float* loss, void* state, size_t state_bytes,
+                     void* workspace, size_t workspace_bytes, gsn_stream_t stream) {
   const char* name = "gsn_ctc_loss_fwd";
   if (int rc = check_ctc(name, B, T, V, S, ld_b, ld_t, blank, dtype)) return rc < 0 ? ok() : rc;
-  if (!input_lengths || !target_lengths || !loss || !raw_loss || !order || (S > 0 && !targets) ||
-      (T > 0 && (!logits || !stats || !posteriors)))
+  if (!input_lengths || !target_lengths || !loss || (S > 0 && !targets) || (T > 0 && !logits))
     return fail(GSN_ERR_INVALID_ARG, "%s: null pointer", name);
-  if (!aligned(logits, type_size(dtype)) || !aligned(stats, 8) || !aligned(posteriors, 16) || !aligned(order, 8))
-    return fail(GSN_ERR_UNSUPPORTED,
-                "%s: logits must be aligned to their type, stats and order to 8, posteriors to 16 bytes", name);
+  if (!aligned(logits, type_size(dtype))) return fail(GSN_ERR_UNSUPPORTED, "%s: logits are not aligned to their type", name);
+  CtcArgs a = ctc_args(logits, ld_b, ld_t, targets, input_lengths, target_lengths, B, T, V, S, blank, zero_infinity);
+  if (int rc = set_state(name, a, state, state_bytes)) return rc;
   const size_t need = gsn_ctc_loss_workspace_bytes(B, T, S, gradient);
   if (workspace_bytes < need) return fail(GSN_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", name, workspace_bytes, need);
   if (!workspace || !aligned(workspace, 16)) return fail(GSN_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", name);
-  CtcArgs a;
-  a.logits = logits;
-  a.ld_b = ld_b;
-  a.ld_t = ld_t;
-  a.targets = targets;
-  a.input_lengths = input_lengths;
-  a.target_lengths = target_lengths;
-  a.B = B;
-  a.T = T;
-  a.V = V;
-  a.S = S;
-  a.blank = blank;
-  a.zero_infinity = zero_infinity;
-  a.pitch = ctc_pitch(S);
-  a.state_pitch = ctc_state_pitch(S);
   a.loss = loss;
-  a.raw_loss = raw_loss;
-  a.stats = (float2*)stats;
-  a.post = posteriors;
-  a.order = (int2*)order;
   char* ws = static_cast<char*>(workspace);
   a.bad = (int*)ws;
   ws += align256((size_t)B * sizeof(int));
@@ -278,36 +299,17 @@ int gsn_ctc_loss_fwd(const void* logits, int64_t ld_b, int64_t ld_t, const int32
 
 int gsn_ctc_loss_bwd(const float* dloss, const void* logits, int64_t ld_b, int64_t ld_t, const int32_t* targets,
                      const int32_t* input_lengths, const int32_t* target_lengths, int B, int T, int V, int S, int blank,
-                     int zero_infinity, int dtype, const float* raw_loss, const float* stats, const float* posteriors,
-                     const int32_t* order, void* dlogits, gsn_stream_t stream) {
+                     int zero_infinity, int dtype, const void* state, size_t state_bytes, void* dlogits,
+                     gsn_stream_t stream) {
   const char* name = "gsn_ctc_loss_bwd";
   if (int rc = check_ctc(name, B, T, V, S, ld_b, ld_t, blank, dtype)) return rc < 0 ? ok() : rc;
   if (T == 0) return ok();
-  if (!dloss || !logits || !input_lengths || !target_lengths || (S > 0 && !targets) || !raw_loss || !stats ||
-      !posteriors || !order || !dlogits)
+  if (!dloss || !logits || !input_lengths || !target_lengths || (S > 0 && !targets) || !dlogits)
     return fail(GSN_ERR_INVALID_ARG, "%s: null pointer", name);
-  if (!aligned(logits, type_size(dtype)) || !aligned(dlogits, type_size(dtype)) || !aligned(stats, 8) ||
-      !aligned(order, 8))
-    return fail(GSN_ERR_UNSUPPORTED, "%s: logits and dlogits must be aligned to their type, stats and order to 8 bytes",
-                name);
-  CtcArgs a;
-  a.logits = logits;
-  a.ld_b = ld_b;
-  a.ld_t = ld_t;
-  a.targets = targets;
-  a.input_lengths = input_lengths;
-  a.target_lengths = target_lengths;
-  a.B = B;
-  a.T = T;
-  a.V = V;
-  a.S = S;
-  a.blank = blank;
-  a.zero_infinity = zero_infinity;
-  a.pitch = ctc_pitch(S);
-  a.raw_loss = const_cast<float*>(raw_loss);
-  a.stats = (float2*)const_cast<float*>(stats);
-  a.post = const_cast<float*>(posteriors);
-  a.order = (int2*)const_cast<int32_t*>(order);
+  if (!aligned(logits, type_size(dtype)) || !aligned(dlogits, type_size(dtype)))
+    return fail(GSN_ERR_UNSUPPORTED, "%s: logits and dlogits are not aligned to their type", name);
+  CtcArgs a = ctc_args(logits, ld_b, ld_t, targets, input_lengths, target_lengths, B, T, V, S, blank, zero_infinity);
+  if (int rc = set_state(name, a, const_cast<void*>(state), state_bytes)) return rc;
   a.dloss = dloss;
   a.dlogits = dlogits;
   return finish(launch_ctc_grad(a, dtype, (cudaStream_t)stream), name);

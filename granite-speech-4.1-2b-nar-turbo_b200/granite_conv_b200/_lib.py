@@ -96,12 +96,12 @@ SIGNATURES = {
                                               _vp, _u32, _f64, _f64, _vp, _i32, _vp]),
     "gsn_dropout_add_layer_norm_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i32,
                                               _f32, _i32, _i32, _vp, _u32, _f64, _f64, _vp, _i32, _vp, _sz, _vp]),
-    "gsn_ctc_loss_pitch": (_i32, [_i32]),
+    "gsn_ctc_loss_state_bytes": (_sz, [_i32, _i32, _i32]),
     "gsn_ctc_loss_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32]),
     "gsn_ctc_loss_fwd": (_i32, [_vp, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _fp,
-                                _fp, _fp, _fp, _vp, _vp, _sz, _vp]),
-    "gsn_ctc_loss_bwd": (_i32, [_fp, _vp, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _fp, _fp,
-                                _fp, _vp, _vp, _vp]),
+                                _vp, _sz, _vp, _sz, _vp]),
+    "gsn_ctc_loss_bwd": (_i32, [_fp, _vp, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp,
+                                _sz, _vp, _vp]),
     "gsn_interleave_glu_rows": (_i32, [_vp, _vp, _i32, _i64, _vp]),
     "gsn_device_status": (_i32, [ctypes.POINTER(_i32), _i32, _vp]),
     "gsn_selftest_bounded_wait": (_i32, [_u64, _vp]),

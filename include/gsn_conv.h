@@ -400,26 +400,25 @@ int gsn_dropout_add_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* dh
  * target_lengths int32 [B] on the device; S <= 2000, T <= 16384.
  * gsn_ctc_loss_fwd: loss[b] = -log p(targets[b, :target_lengths[b]] | softmax(logits[b, :input_lengths[b]])), inf where
  *   no alignment exists (0 with zero_infinity), NaN where a length lies outside [0, T] or [0, S], a label outside
- *   [0, V), or a valid frame holds NaN, +inf or nothing but -inf.  raw_loss [B], stats [B, T, 2], posteriors [B, T, P]
- *   (fp32; P = gsn_ctc_loss_pitch(S)) and order (int32 [B, P, 2]) are buffers that the backward pass reads; it may be
- *   called after a forward pass with gradient != 0.  A class of the transcript, the blank among them, whose logit lies
- *   more than 690 below the largest of them counts as impossible in that frame.
- *   workspace: gsn_ctc_loss_workspace_bytes(B, T, S, gradient) bytes, 16-byte aligned.
+ *   [0, V), or a valid frame holds NaN, +inf or nothing but -inf.  state: gsn_ctc_loss_state_bytes(B, T, S) bytes that
+ *   the backward pass reads; it may be called after a forward pass with gradient != 0.  A class of the transcript, the
+ *   blank among them, whose logit lies more than 690 below the largest of them counts as impossible in that frame.
+ *   workspace: gsn_ctc_loss_workspace_bytes(B, T, S, gradient) bytes.  Both 16-byte aligned.
  * gsn_ctc_loss_bwd: dlogits [B, T, V] dense, dloss[b] * d loss[b] / d logits; 0 in padding frames, for utterances
  *   without an alignment 0 with zero_infinity and NaN without, NaN for the others whose loss is NaN. */
-int gsn_ctc_loss_pitch(int S);
+size_t gsn_ctc_loss_state_bytes(int B, int T, int S);
 
 size_t gsn_ctc_loss_workspace_bytes(int B, int T, int S, int gradient);
 
 int gsn_ctc_loss_fwd(const void* logits, int64_t ld_b, int64_t ld_t, const int32_t* targets,
                      const int32_t* input_lengths, const int32_t* target_lengths, int B, int T, int V, int S, int blank,
-                     int zero_infinity, int gradient, int dtype, float* loss, float* raw_loss, float* stats,
-                     float* posteriors, int32_t* order, void* workspace, size_t workspace_bytes, gsn_stream_t stream);
+                     int zero_infinity, int gradient, int dtype, float* loss, void* state, size_t state_bytes,
+                     void* workspace, size_t workspace_bytes, gsn_stream_t stream);
 
 int gsn_ctc_loss_bwd(const float* dloss, const void* logits, int64_t ld_b, int64_t ld_t, const int32_t* targets,
                      const int32_t* input_lengths, const int32_t* target_lengths, int B, int T, int V, int S, int blank,
-                     int zero_infinity, int dtype, const float* raw_loss, const float* stats, const float* posteriors,
-                     const int32_t* order, void* dlogits, gsn_stream_t stream);
+                     int zero_infinity, int dtype, const void* state, size_t state_bytes, void* dlogits,
+                     gsn_stream_t stream);
 
 /* ---- whole module without any allocation ------------------------------------------------------------------
  * No counterpart in the reference.  For callers that cannot allocate device memory where they run the module —

@@ -70,7 +70,7 @@ def test_ctc_entry_points_refuse_bad_calls():
     L = _lib.lib()
 
     def fwd(B=2, T=5, V=7, S=3, ld_t=7, blank=0, dtype=0, logits=P, targets=P, ws=None, nbytes=0):
-        return L.gsn_ctc_loss_fwd(logits, 35, ld_t, targets, P, P, B, T, V, S, blank, 0, 1, dtype, P, P, P, P, P, ws,
+        return L.gsn_ctc_loss_fwd(logits, 35, ld_t, targets, P, P, B, T, V, S, blank, 0, 1, dtype, P, P, 1 << 20, ws,
                                   nbytes, None)
 
     assert fwd(B=-1) == 1 and fwd(V=0) == 1 and fwd(S=-1) == 1
@@ -79,14 +79,16 @@ def test_ctc_entry_points_refuse_bad_calls():
     assert fwd(logits=None) == 1 and fwd(targets=None) == 1 and fwd(logits=ODD) == 2
     need = L.gsn_ctc_loss_workspace_bytes(2, 5, 3, 1)
     assert need > L.gsn_ctc_loss_workspace_bytes(2, 5, 3, 0) > 0 and L.gsn_ctc_loss_workspace_bytes(0, 5, 3, 1) == 0
-    assert all(L.gsn_ctc_loss_pitch(s) == training._ctc_pitch(s) for s in range(9))
     assert fwd(ws=P, nbytes=need - 1) == 5
     assert fwd(B=0, logits=None, targets=None) == 0
 
-    def bwd(dloss=P, out=P, T=5):
-        return L.gsn_ctc_loss_bwd(dloss, P, 35, 7, P, P, P, 2, T, 7, 3, 0, 0, 0, P, P, P, P, out, None)
+    state = L.gsn_ctc_loss_state_bytes(2, 5, 3)
+
+    def bwd(dloss=P, out=P, T=5, st=P, nbytes=state):
+        return L.gsn_ctc_loss_bwd(dloss, P, 35, 7, P, P, P, 2, T, 7, 3, 0, 0, 0, st, nbytes, out, None)
 
     assert bwd(dloss=None) == 1 and bwd(out=None) == 1 and bwd(out=ODD) == 2 and bwd(dloss=None, T=0) == 0
+    assert bwd(nbytes=state - 1) == 5 and bwd(st=None) == 1 and bwd(st=ctypes.c_void_p(264)) == 1
 
 
 def test_functions_refuse_cpu_tensors():
