@@ -180,30 +180,32 @@ __device__ __forceinline__ void copy16(void* smem, const void* gmem) {
 }
 
 // Rows under way: each thread copies the 16-byte words that it will itself read, some rows ahead, so the loads need
-// neither registers nor a barrier.  TENSORS inputs of NV vectors a lane; slots [stage][tensor][vector][word][thread].
+// neither registers nor a barrier.  TENSORS inputs of NV blocks a lane; slots [stage][tensor][block][word][thread].
+constexpr int kRowThreads = 256;
+
 template <typename T, int NV, int TENSORS>
 struct Ring {
-  static constexpr int Q = Vec8<T>::Q, WORDS = TENSORS * NV * Q;
-  uint4* slots;                                    // shared memory, stages * WORDS * blockDim.x
-  __device__ __forceinline__ uint4* at(int stage, int tensor, int i) const {
-    return slots + ((stage * TENSORS + tensor) * NV + i) * Q * blockDim.x + threadIdx.x;
+  static constexpr int Q = Vec8<T>::Q, WORDS = TENSORS * NV * Q, STAGE = WORDS * kRowThreads;
+  uint4* slots;                                    // this thread's first, in shared memory
+  static __device__ __forceinline__ constexpr int at(int tensor, int i, int q) {
+    return ((tensor * NV + i) * Q + q) * kRowThreads;
   }
   __device__ __forceinline__ void fetch(int stage, int tensor, int i, const T* row, int base, int lane, int D) const {
-    uint4* dst = at(stage, tensor, i);
+    uint4* dst = slots + stage * STAGE;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int col = word_column<T>(base, lane, q);
-      if (col < D) copy16(dst + q * blockDim.x, row + col);
+      if (col < D) copy16(dst + at(tensor, i, q), row + col);
     }
   }
   __device__ __forceinline__ void read(int stage, int tensor, int i, Vec8<T>& r) const {
-    const uint4* src = at(stage, tensor, i);
+    const uint4* src = slots + stage * STAGE;
 #pragma unroll
-    for (int q = 0; q < Q; ++q) r.q[q] = src[q * blockDim.x];
+    for (int q = 0; q < Q; ++q) r.q[q] = src[at(tensor, i, q)];
   }
   // columns past D are never copied: zeros, once
   __device__ __forceinline__ void clear(int stages) const {
-    for (int i = 0; i < stages * WORDS; ++i) slots[i * blockDim.x + threadIdx.x] = make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < stages * WORDS; ++i) slots[i * kRowThreads] = make_uint4(0, 0, 0, 0);
   }
 };
 
@@ -391,12 +393,12 @@ __host__ __device__ constexpr int ring_stages(int words) { return words <= 6 ? 4
 // LayerNorm forward; DROP: of h = residual + dropout(x), which is stored too.  W warps a row, NV blocks of 256 columns
 // a warp: a row stays in registers between the two passes of its statistics, its weights for all rows of the warp.
 template <typename T, int NV, bool VEC, bool DROP>
-__global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_fwd_kernel(RowArgs a) {
+__global__ void __launch_bounds__(kRowThreads, NV < 4 ? 2 : 1) ln_fwd_kernel(RowArgs a) {
   __shared__ __align__(16) float exchange[8][4 * kMaxRowWarps];
   extern __shared__ uint4 ring_slots[];
   constexpr int TENSORS = DROP ? 2 : 1, S = ring_stages(Ring<T, NV, TENSORS>::WORDS);
-  const Ring<T, NV, TENSORS> ring{ring_slots};
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W, R = (blockDim.x >> 5) / W;
+  const Ring<T, NV, TENSORS> ring{ring_slots + threadIdx.x};
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W, R = (kRowThreads >> 5) / W;
   const int group = warp / W;
   (&exchange[0][0])[threadIdx.x] = 0.f;
   RowGroup rg{W, warp - group * W, 1 + group, exchange[group], 0};
@@ -509,12 +511,12 @@ __global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_fwd_kernel(RowArgs a) 
 // lane keeps the running sums of its columns' dw and db over all rows of its warp; the CTA adds its row groups in
 // order and leaves one partial row, so no sum depends on the order of arrival.
 template <typename T, int NV, bool VEC, bool DROP>
-__global__ void __launch_bounds__(256, NV < 4 ? 2 : 1) ln_bwd_kernel(RowArgs a) {
+__global__ void __launch_bounds__(kRowThreads, NV < 4 ? 2 : 1) ln_bwd_kernel(RowArgs a) {
   __shared__ __align__(16) float exchange[8][4 * kMaxRowWarps];
   extern __shared__ uint4 ring_slots[];            // the ring; at the end [2][D], the CTA's sums
   constexpr int TENSORS = DROP ? 3 : 2, S = ring_stages(Ring<T, NV, TENSORS>::WORDS);
-  const Ring<T, NV, TENSORS> ring{ring_slots};
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W, R = (blockDim.x >> 5) / W;
+  const Ring<T, NV, TENSORS> ring{ring_slots + threadIdx.x};
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W, R = (kRowThreads >> 5) / W;
   const int group = warp / W;
   (&exchange[0][0])[threadIdx.x] = 0.f;
   RowGroup rg{W, warp - group * W, 1 + group, exchange[group], 0};
@@ -812,11 +814,11 @@ int launch_fwd(const RowArgs& a, const RowShape& s, cudaStream_t stream) {
   const int R = s.warps / s.W;
   const int64_t want = (a.M + R - 1) / R, most = 2 * device_sm_count();
   constexpr int words = Ring<T, NV, DROP ? 2 : 1>::WORDS;
-  const size_t smem = VEC ? sizeof(uint4) * ring_stages(words) * words * s.warps * 32 : 0;
+  const size_t smem = VEC ? sizeof(uint4) * ring_stages(words) * words * kRowThreads : 0;
   auto* kernel = ln_fwd_kernel<T, NV, VEC, DROP>;
   if (smem > 32 * 1024)                            // with the static part, more than a launch gets unasked
     if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
-  kernel<<<(int)(want < most ? want : most), s.warps * 32, smem, stream>>>(a);
+  kernel<<<(int)(want < most ? want : most), kRowThreads, smem, stream>>>(a);
   return (int)cudaGetLastError();
 }
 
@@ -824,12 +826,12 @@ template <typename T, int NV, bool VEC, bool DROP>
 int launch_bwd(const RowArgs& a, const RowShape& s, cudaStream_t stream) {
   const int R = s.warps / s.W;
   constexpr int words = Ring<T, NV, DROP ? 3 : 2>::WORDS;
-  const size_t ring = VEC ? sizeof(uint4) * ring_stages(words) * words * s.warps * 32 : 0;
+  const size_t ring = VEC ? sizeof(uint4) * ring_stages(words) * words * kRowThreads : 0;
   const size_t sums = R > 1 ? (size_t)2 * a.D * sizeof(float) : 0, smem = ring > sums ? ring : sums;
   auto* kernel = ln_bwd_kernel<T, NV, VEC, DROP>;
   if (smem > 32 * 1024)                            // with the static part, more than a launch gets unasked
     if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
-  kernel<<<(int)a.partial_rows, s.warps * 32, smem, stream>>>(a);
+  kernel<<<(int)a.partial_rows, kRowThreads, smem, stream>>>(a);
   return (int)cudaGetLastError();
 }
 
