@@ -121,6 +121,32 @@ def test_layer_norm_many_rows():
     assert all(torch.equal(a, c) for a, c in zip(out, again))
 
 
+def test_many_utterances():
+    """More utterances than a walk takes at once, lengths from zero up and out of range, both operators and directions."""
+    B, T, D = 2500, 3, 40
+    g = np.random.default_rng(5)
+    given = g.integers(-1, T + 2, B)
+    given[:3] = (0, T, 2 ** 31 - 1)
+    lengths = np.clip(given, 0, T).tolist()
+    lens = torch.tensor(given, dtype=torch.int32, device=DEV)
+    x, dy, res = rand(1, (B, T, D), BF), rand(2, (B, T, D), BF), rand(5, (B, T, D), BF)
+    w, b = rand(3, (D,), F32, 0.2, 1.0), rand(4, (D,), F32)
+    ref, r = R.layer_norm(x, w, b, EPS, lengths)
+    close(tr.layer_norm(x, w, b, EPS, lens), ref, norm_bound(BF, ref, x, w, b, r))
+    rdx, rdw, rdb, r, xh = R.layer_norm_backward(dy, x, w, EPS, lengths)
+    bw, bb = param_bounds(F32, rdw, rdb, dy, x, r, xh, lengths)
+    dx, dw, db = tr.layer_norm_backward(dy, x, w, EPS, lens)
+    close(dx, rdx, grads_bound(BF, rdx, dy, x, w, r, lengths))
+    close(dw, rdw, bw)
+    close(db, rdb, bb)
+    y, h = tr.dropout_add_layer_norm(x, res, w, b, rng_of(), 0.2, lengths=lens)
+    assert torch.equal(h, tr.dropout_add(x, rng_of(), 0.2, residual=res, lengths=lens))
+    pad = R.padding(x.shape, lengths).to(DEV)
+    assert torch.equal(h.masked_select(pad), res.masked_select(pad)) and not y.masked_select(pad).any()
+    out = tr.dropout_add_layer_norm_backward(dy, res, h, w, rng_of(), 0.2, lengths=lens)
+    assert torch.equal(out[1].masked_select(pad), res.masked_select(pad)) and not out[0].masked_select(pad).any()
+
+
 def test_layer_norm_keeps_the_inference_kernel():
     """What granite::layer_norm took before keeps its kernel and its bits, with and without a gradient to record."""
     x, w, b = rand(1, (2, 37, 1024), BF), rand(2, (1024,), BF, 0.1, 1.0), rand(3, (1024,), BF)
