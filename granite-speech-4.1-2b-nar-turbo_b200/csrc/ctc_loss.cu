@@ -335,7 +335,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 
   const int dir = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int n = __ldg(a.input_lengths + b), len = __ldg(a.target_lengths + b);
-  const bool bad = __ldg(a.bad + b) || n < 0 || n > a.T;
+  kernel_wait_ahead();
+  const bool bad = a.bad[b] || n < 0 || n > a.T;
   if (bad || n == 0) {                             // both CTAs of the cluster leave here
     if (dir == 0 && tid == 0) {
       const float raw = bad ? NAN : len == 0 ? 0.f : INFINITY;
@@ -401,7 +402,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 
   // the frames' normalisers, by the warp that has the time
   double norm = 0.0;
   if (dir == 0 && producer)
-    for (int t = lane; t < n; t += 32) norm += (double)__ldg(a.norms + frame0 + t);
+    for (int t = lane; t < n; t += 32) norm += (double)a.norms[frame0 + t];
   __syncthreads();
 
   const int h = (n + 1) / 2, n1 = dir ? n - h : h;  // this side's frames before the meeting
@@ -928,6 +929,8 @@ __global__ void __launch_bounds__(WARP_ROW ? kRowThreads : kCtaThreads) ctc_grad
   if (tid < 32) grad_labels<T, F>(a, p, x, g, frame, count, b, tid);
 }
 
+constexpr size_t kMostSmem = 227 * 1024 - 1024;  // a CTA's, less the static part
+
 template <int NP, int H, int NBUF, bool GRAD>
 int launch_lattice(const CtcArgs& a, cudaStream_t stream) {
   constexpr int HL = halo_lanes<NP, H>(), NS = 2 * NP;
@@ -935,9 +938,9 @@ int launch_lattice(const CtcArgs& a, cudaStream_t stream) {
   const size_t smem = (size_t)NBUF * H * a.pitch * 4 + (GRAD ? (size_t)NBUF * H * a.state_pitch * 4 : 0) +
                       (size_t)2 * nw * HL * NS * sizeof(float2) + (GRAD ? (size_t)2 * H * (nw * 32 + 4) * 4 : 0);
   auto* kernel = ctc_lattice_kernel<NP, H, NBUF, GRAD>;
-  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
-  kernel<<<dim3(2, a.B), (nw + 1) * 32, smem, stream>>>(a, nw);
-  return (int)cudaGetLastError();
+  static std::atomic<uint64_t> allowed{0};
+  if (int rc = allow_smem((const void*)kernel, kMostSmem, allowed)) return rc;
+  return launch_behind(kernel, dim3(2, a.B), (nw + 1) * 32, smem, stream, a, nw);
 }
 
 // Pairs a lane: as few as four warps hold (one a scheduler of the SM, so that a step issues in the least time), then

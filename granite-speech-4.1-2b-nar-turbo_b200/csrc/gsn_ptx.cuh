@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace gsn {
 
 // ------------------------------------------------------------------------------------------------------------
@@ -452,6 +454,39 @@ __device__ __forceinline__ void tmem_wait_ld_dep(uint32_t (&a)[16], uint32_t (&b
         "+r"(b[10]), "+r"(b[11]), "+r"(b[12]), "+r"(b[13]), "+r"(b[14]), "+r"(b[15])
       :
       : "memory");
+}
+
+// ------------------------------------------------------------------------------------------------------------
+// A kernel launched by launch_behind() may begin before the one ahead of it in the stream has ended, where that one
+// has let it (kernel_let_next): its blocks then stand ready, and nothing of the other's output is read before
+// kernel_wait_ahead(), which returns when the kernel ahead has ended and its writes are visible.
+__device__ __forceinline__ void kernel_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void kernel_wait_ahead() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... P, typename... A>
+int launch_behind(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, A... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
+// Raises a kernel's limit of dynamic shared memory once a device; `done` is the caller's, one bit a device.
+inline int allow_smem(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return (int)e;
+  const uint64_t bit = (uint64_t)1 << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return 0;
+  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes)) return (int)e;
+  if (dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return 0;
 }
 
 // ------------------------------------------------------------------------------------------------------------

@@ -514,6 +514,7 @@ template <typename T, int NV, bool VEC, bool DROP>
 __global__ void __launch_bounds__(kRowThreads, NV < 4 ? 2 : 1) ln_bwd_kernel(RowArgs a) {
   __shared__ __align__(16) float exchange[8][4 * kMaxRowWarps];
   extern __shared__ uint4 ring_slots[];            // the ring; at the end [2][D], the CTA's sums
+  kernel_let_next();                               // the sums' kernel stands ready
   constexpr int TENSORS = DROP ? 3 : 2, S = ring_stages(Ring<T, NV, TENSORS>::WORDS);
   const Ring<T, NV, TENSORS> ring{ring_slots + threadIdx.x};
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, W = a.W, R = (kRowThreads >> 5) / W;
@@ -692,6 +693,7 @@ __global__ void __launch_bounds__(1024) ln_param_grad_kernel(const float* __rest
   __shared__ float part[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;            // column of [dw | db]
+  kernel_wait_ahead();
   float s = 0.f;
   if (c < 2 * D)
     for (int r = warp; r < rows; r += 32) s += __ldg(partials + (int64_t)r * 2 * D + c);
@@ -809,6 +811,8 @@ bool vec_ok(const RowArgs& a, int size) {
   return true;
 }
 
+constexpr size_t kMostSums = (size_t)2 * (kMaxRowWidth / 2) * sizeof(float);     // R > 1: half the widest row
+
 template <typename T, int NV, bool VEC, bool DROP>
 int launch_fwd(const RowArgs& a, const RowShape& s, cudaStream_t stream) {
   const int R = s.warps / s.W;
@@ -816,8 +820,9 @@ int launch_fwd(const RowArgs& a, const RowShape& s, cudaStream_t stream) {
   constexpr int words = Ring<T, NV, DROP ? 2 : 1>::WORDS;
   const size_t smem = VEC ? sizeof(uint4) * ring_stages(words) * words * kRowThreads : 0;
   auto* kernel = ln_fwd_kernel<T, NV, VEC, DROP>;
+  static std::atomic<uint64_t> allowed{0};         // an instantiation's need does not change beyond its sums' 64 KB
   if (smem > 32 * 1024)                            // with the static part, more than a launch gets unasked
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
+    if (int rc = allow_smem((const void*)kernel, smem > kMostSums ? smem : kMostSums, allowed)) return rc;
   kernel<<<(int)(want < most ? want : most), kRowThreads, smem, stream>>>(a);
   return (int)cudaGetLastError();
 }
@@ -829,8 +834,9 @@ int launch_bwd(const RowArgs& a, const RowShape& s, cudaStream_t stream) {
   const size_t ring = VEC ? sizeof(uint4) * ring_stages(words) * words * kRowThreads : 0;
   const size_t sums = R > 1 ? (size_t)2 * a.D * sizeof(float) : 0, smem = ring > sums ? ring : sums;
   auto* kernel = ln_bwd_kernel<T, NV, VEC, DROP>;
+  static std::atomic<uint64_t> allowed{0};         // an instantiation's need does not change beyond its sums' 64 KB
   if (smem > 32 * 1024)                            // with the static part, more than a launch gets unasked
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return (int)e;
+    if (int rc = allow_smem((const void*)kernel, smem > kMostSums ? smem : kMostSums, allowed)) return rc;
   kernel<<<(int)a.partial_rows, kRowThreads, smem, stream>>>(a);
   return (int)cudaGetLastError();
 }
@@ -883,9 +889,8 @@ int launch_typed(RowArgs a, int op, cudaStream_t stream) {
     if (rc) return rc;
   }
   if (bwd) {
-    ln_param_grad_kernel<T><<<(2 * a.D + 31) / 32, 1024, 0, stream>>>(a.partials, (int)a.partial_rows, a.D, a.dweight,
-                                                                      a.dbias, a.param_fp32);
-    return (int)cudaGetLastError();
+    return launch_behind(ln_param_grad_kernel<T>, dim3((2 * a.D + 31) / 32), 1024, 0, stream, a.partials,
+                         (int)a.partial_rows, a.D, a.dweight, a.dbias, a.param_fp32);
   }
   return 0;
 }

@@ -150,8 +150,7 @@ def _layer_norm_backward(dy, x, weight, eps, lengths):
     D = x.shape[-1]
     dx = _dense(x)
     M = dx.numel() // D
-    dw = weight.new_empty((D,))
-    db = weight.new_empty((D,))
+    dw, db = _dense(weight), _dense(weight)
     with _on(x.device):
         xr, ld_x = _rows(x)
         gr, ld_g = _rows(dy)
@@ -294,8 +293,7 @@ def _dropout_add_layer_norm_backward(dy, dh, h, weight, rng, p, scale, site, eps
     dx = _dense(h)
     dres = _dense(h)
     M = dx.numel() // D
-    dw = weight.new_empty((D,))
-    db = weight.new_empty((D,))
+    dw, db = _dense(weight), _dense(weight)
     with _on(h.device):
         hr, ld_h = _rows(h)
         gr, ld_g = _rows(dy)
