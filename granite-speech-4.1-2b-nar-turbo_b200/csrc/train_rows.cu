@@ -298,16 +298,20 @@ struct Kept {
 #pragma unroll
     for (int i = 0; i < NV; ++i) group[i] = row_group + (base[i] >> 3) + lane;
     philox(g, group, r);
-    if (OWN) {
+    if constexpr (OWN) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) drawn[OWN ? i : 0] = r[i];
-      return;
+      for (int i = 0; i < NV; ++i) drawn[i] = r[i];
+    } else {
+      to_bits(r, lane, threshold16);
     }
+  }
+
+  __device__ __forceinline__ void to_bits(const uint4 (&r)[NV], int lane, uint32_t threshold16) {
     uint32_t own = 0;
     bits = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) own |= keep_bits(r[i], threshold16) << (8 * i);
-    if (VEC) {
+    if constexpr (VEC) {
 #pragma unroll
       for (int q = 0; q < 2; ++q) {                // columns base + 128 q + 4 l: group 16 q + l / 2, its half l % 2
         const uint32_t w = __shfl_sync(0xffffffffu, own, 16 * q + (lane >> 1)) >> (4 * (lane & 1));
@@ -323,7 +327,7 @@ struct Kept {
   }
 
   __device__ __forceinline__ void apply(int i, uint32_t threshold16, float2 (&f)[4]) const {
-    if (OWN) return keep8(drawn[OWN ? i : 0], threshold16, f);
+    if constexpr (OWN) return keep8(drawn[i], threshold16, f);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       f[k].x = bits & (1u << (8 * i + 2 * k)) ? f[k].x : 0.f;
@@ -696,7 +700,7 @@ __global__ void __launch_bounds__(1024) ln_param_grad_kernel(const float* __rest
   kernel_wait_ahead();
   float s = 0.f;
   if (c < 2 * D)
-    for (int r = warp; r < rows; r += 32) s += __ldg(partials + (int64_t)r * 2 * D + c);
+    for (int r = warp; r < rows; r += 32) s += __ldcg(partials + (int64_t)r * 2 * D + c);
   part[warp][lane] = s;
   __syncthreads();
   s = part[lane][warp];                            // warp w adds column w
@@ -714,13 +718,14 @@ __global__ void __launch_bounds__(1024) ln_param_grad_kernel(const float* __rest
 }
 
 // out = residual + dropout(x): a thread takes four groups of eight columns, so that their loads are under way
-// together.  FLAT (dense 16-byte aligned tensors without lengths): group g lies at element 8 g.  `n` groups from
-// `group0` on, fewer than 2^31.
+// together.  FLAT (dense 16-byte aligned tensors without lengths): group g lies at element 8 g.  `n` groups from row
+// `row0` on, fewer than 2^31.
 constexpr int kDropUnroll = 4;
 
 template <typename T, bool VEC, bool FLAT, bool RES>
-__global__ void __launch_bounds__(256) dropout_kernel(RowArgs a, int64_t group0, uint32_t n) {
+__global__ void __launch_bounds__(256) dropout_kernel(RowArgs a, int64_t row0, uint32_t n) {
   const int D = a.D;
+  const int64_t group0 = row0 * a.groups;
   const uint32_t block0 = blockIdx.x * (256u * kDropUnroll) + threadIdx.x;
   Vec8<T> xq[kDropUnroll], rq[kDropUnroll];
   bool there[kDropUnroll], use[kDropUnroll];
@@ -744,8 +749,8 @@ __global__ void __launch_bounds__(256) dropout_kernel(RowArgs a, int64_t group0,
     there[u] = g < n;
     use[u] = there[u] && !a.drop_all;
     if (!FLAT && there[u]) {
-      const uint32_t r = g / (uint32_t)a.groups;   // group0 begins a row
-      row[u] = group0 / a.groups + r;
+      const uint32_t r = g / (uint32_t)a.groups;
+      row[u] = row0 + r;
       col[u] = (int)(g - r * (uint32_t)a.groups) * 8;
       use[u] = use[u] && !padding_row(a, (uint32_t)row[u]);
     }
@@ -785,9 +790,39 @@ __global__ void __launch_bounds__(256) dropout_kernel(RowArgs a, int64_t group0,
   }
 }
 
+// The same off the 16-byte grid: a warp takes a block of 256 columns of a row, so that its single elements stay
+// neighbours (eight of a lane's own in a row write every 32-byte sector eight times).
+template <typename T>
+__global__ void __launch_bounds__(256) dropout_block_kernel(RowArgs a) {
+  const int lane = threadIdx.x & 31, D = a.D;
+  const uint32_t blocks = (uint32_t)(D + 255) / 256;
+  const int64_t n = a.M * blocks, step = (int64_t)gridDim.x * 8;
+  const Generator gen = load_generator(a.rng, a.site);
+  for (int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); item < n; item += step) {
+    const int64_t row = blocks == 1 ? item : item / blocks;
+    const int base[1] = {(int)(item - row * blocks) * 256};
+    const bool use = !a.drop_all && !padding_row(a, (uint32_t)row);
+    Vec8<T> xq, rq;
+    if (use) load8<T, false>(static_cast<const T*>(a.x) + row * a.ld_x, base[0], lane, D, xq);
+    if (a.residual) load8<T, false>(static_cast<const T*>(a.residual) + row * a.ld_res, base[0], lane, D, rq);
+    float2 v[4] = {};
+    if (a.residual) unpack(rq, v);
+    if (use) {
+      Kept<T, 1, false> kept;
+      kept.draw(gen, (uint64_t)row * a.groups, base, lane, a.threshold << 16);
+      float2 f[4];
+      unpack(xq, f);
+      kept.apply(0, 0, f);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = ffma2(f[k], both(a.factor), v[k]);
+    }
+    store8<T, false>(static_cast<T*>(a.y) + row * D, base[0], lane, D, v);
+  }
+}
+
 // A row's warps and blocks of 256 columns a warp.  Two blocks, 16 columns a lane, leave 16 warps an SM beside the
-// weights and the sums of their gradients in registers (one warp with four blocks a row: 8 warps, 100 us instead of
-// 6x us at 73728 x 1024 backward); the widest rows take four.
+// weights and the sums of their gradients in registers; the widest rows take four.  At 73728 x 1024 bf16 backward, fused
+// with dropout, two blocks take 123 us and four 122, one block 158; of the odd 11376 x 1001, 36, 51 and 32 us.
 struct RowShape {
   int W, NV, warps;
 };
@@ -820,7 +855,7 @@ int launch_fwd(const RowArgs& a, const RowShape& s, cudaStream_t stream) {
   constexpr int words = Ring<T, NV, DROP ? 2 : 1>::WORDS;
   const size_t smem = VEC ? sizeof(uint4) * ring_stages(words) * words * kRowThreads : 0;
   auto* kernel = ln_fwd_kernel<T, NV, VEC, DROP>;
-  static std::atomic<uint64_t> allowed{0};         // an instantiation's need does not change beyond its sums' 64 KB
+  static std::atomic<uint64_t> allowed{0};         // an instantiation's ring is fixed, its sums are 32 KB at most
   if (smem > 32 * 1024)                            // with the static part, more than a launch gets unasked
     if (int rc = allow_smem((const void*)kernel, smem > kMostSums ? smem : kMostSums, allowed)) return rc;
   kernel<<<(int)(want < most ? want : most), kRowThreads, smem, stream>>>(a);
@@ -834,7 +869,7 @@ int launch_bwd(const RowArgs& a, const RowShape& s, cudaStream_t stream) {
   const size_t ring = VEC ? sizeof(uint4) * ring_stages(words) * words * kRowThreads : 0;
   const size_t sums = R > 1 ? (size_t)2 * a.D * sizeof(float) : 0, smem = ring > sums ? ring : sums;
   auto* kernel = ln_bwd_kernel<T, NV, VEC, DROP>;
-  static std::atomic<uint64_t> allowed{0};         // an instantiation's need does not change beyond its sums' 64 KB
+  static std::atomic<uint64_t> allowed{0};         // an instantiation's ring is fixed, its sums are 32 KB at most
   if (smem > 32 * 1024)                            // with the static part, more than a launch gets unasked
     if (int rc = allow_smem((const void*)kernel, smem > kMostSums ? smem : kMostSums, allowed)) return rc;
   kernel<<<(int)a.partial_rows, kRowThreads, smem, stream>>>(a);
@@ -856,18 +891,25 @@ int launch_rows(const RowArgs& a, bool bwd, cudaStream_t stream) {
 template <typename T, bool RES>
 int launch_dropout(const RowArgs& a, bool vec, cudaStream_t stream) {
   const bool flat = vec && !a.lengths && (a.ld_x == a.D || a.M == 1) && (!RES || a.ld_res == a.D || a.M == 1);
+  // Blocks where they are at least three fifths full.  30 M elements of bf16 without a residual: 53 us in full blocks,
+  // 77 us at D = 150, 113 us at 100, 169 us at 65; eight neighbours a lane 86 to 88 us at any width.
+  const int64_t blocks = (a.D + 255) / 256;
+  if (!vec && (int64_t)a.D * 5 >= blocks * 256 * 3) {
+    const int64_t want = (a.M * blocks + 7) / 8, most = 8 * device_sm_count();
+    dropout_block_kernel<T><<<(int)(want < most ? want : most), 256, 0, stream>>>(a);
+    return (int)cudaGetLastError();
+  }
   const int64_t rows_a_time = (int64_t)0x7fffffff / a.groups;    // whole rows, a 32-bit count of groups a launch
   for (int64_t row0 = 0; row0 < a.M; row0 += rows_a_time) {
     const int64_t rows = a.M - row0 < rows_a_time ? a.M - row0 : rows_a_time;
     const uint32_t n = (uint32_t)(rows * a.groups);
     const int grid = (int)((n + 256u * kDropUnroll - 1) / (256u * kDropUnroll));
-    const int64_t group0 = row0 * a.groups;
     if (flat)
-      dropout_kernel<T, true, true, RES><<<grid, 256, 0, stream>>>(a, group0, n);
+      dropout_kernel<T, true, true, RES><<<grid, 256, 0, stream>>>(a, row0, n);
     else if (vec)
-      dropout_kernel<T, true, false, RES><<<grid, 256, 0, stream>>>(a, group0, n);
+      dropout_kernel<T, true, false, RES><<<grid, 256, 0, stream>>>(a, row0, n);
     else
-      dropout_kernel<T, false, false, RES><<<grid, 256, 0, stream>>>(a, group0, n);
+      dropout_kernel<T, false, false, RES><<<grid, 256, 0, stream>>>(a, row0, n);
     if (cudaError_t e = cudaGetLastError()) return (int)e;
   }
   return 0;

@@ -25,7 +25,7 @@ EPS = 1e-5
 # (shape, lengths): one row, the encoder's width, narrow, odd and ragged widths, several warps a row, the widest
 SHAPES = [((1, 1, 1), None), ((1, 1, 1024), None), ((2, 37, 1024), [37, 11]), ((3, 5, 160), [5, 0, 1]),
           ((2, 9, 7), None), ((2, 9, 257), [9, 3]), ((1, 33, 1001), None), ((2, 17, 2048), None), ((1, 6, 2051), None),
-          ((2, 3, 4096), [3, 1]), ((1, 3, 8192), None), ((1, 2, 8191), None), ((1, 700, 24), None)]
+          ((2, 3, 4096), [3, 1]), ((1, 3, 8192), None), ((1, 2, 8191), None), ((1, 700, 24), None), ((2, 8, 153), [8, 2]), ((2, 8, 155), [3, 8])]
 
 
 def rand(seed, shape, dtype, scale=1.0, shift=0.0):
