@@ -932,9 +932,8 @@ __global__ void __launch_bounds__(WARP_ROW ? kRowThreads : kCtaThreads) ctc_grad
 constexpr size_t kMostSmem = 227 * 1024 - 1024;  // a CTA's, less the static part
 
 template <int NP, int H, int NBUF, bool GRAD>
-int launch_lattice(const CtcArgs& a, cudaStream_t stream) {
+int launch_lattice(const CtcArgs& a, int nw, cudaStream_t stream) {
   constexpr int HL = halo_lanes<NP, H>(), NS = 2 * NP;
-  const int nw = lattice_warps(a.S + 1, NP, HL);
   const size_t smem = (size_t)NBUF * H * a.pitch * 4 + (GRAD ? (size_t)NBUF * H * a.state_pitch * 4 : 0) +
                       (size_t)2 * nw * HL * NS * sizeof(float2) + (GRAD ? (size_t)2 * H * (nw * 32 + 4) * 4 : 0);
   auto* kernel = ctc_lattice_kernel<NP, H, NBUF, GRAD>;
@@ -946,14 +945,25 @@ int launch_lattice(const CtcArgs& a, cudaStream_t stream) {
 // Pairs a lane: as few as four warps hold (one a scheduler of the SM, so that a step issues in the least time), then
 // four pairs and more warps.  Frames a block: 16 where they fit (48 utterances of 1536 frames with 300 labels: 195 us,
 // with 8 frames 252 us: about 500 cycles go into a block's begin and end), fewer where the rows get long.
+struct LatticeShape {
+  int NP, H, nw;
+};
+LatticeShape lattice_shape(int pairs) {
+  if (const int nw = lattice_warps(pairs, 1, halo_lanes<1, 16>()); nw <= 4) return {1, 16, nw};
+  if (const int nw = lattice_warps(pairs, 2, halo_lanes<2, 16>()); nw <= 4) return {2, 16, nw};
+  if (const int nw = lattice_warps(pairs, 3, halo_lanes<3, 16>()); nw <= 4) return {3, 16, nw};
+  if (const int nw = lattice_warps(pairs, 4, halo_lanes<4, 8>()); nw <= 8) return {4, 8, nw};
+  return {4, 4, lattice_warps(pairs, 4, halo_lanes<4, 4>())};
+}
+
 template <bool GRAD>
 int launch_lattice_for(const CtcArgs& a, cudaStream_t stream) {
-  const int pairs = a.S + 1;
-  if (lattice_warps(pairs, 1, halo_lanes<1, 16>()) <= 4) return launch_lattice<1, 16, 2, GRAD>(a, stream);
-  if (lattice_warps(pairs, 2, halo_lanes<2, 16>()) <= 4) return launch_lattice<2, 16, 2, GRAD>(a, stream);
-  if (lattice_warps(pairs, 3, halo_lanes<3, 16>()) <= 4) return launch_lattice<3, 16, 2, GRAD>(a, stream);
-  if (lattice_warps(pairs, 4, halo_lanes<4, 8>()) <= 8) return launch_lattice<4, 8, 2, GRAD>(a, stream);
-  return launch_lattice<4, 4, 2, GRAD>(a, stream);
+  const LatticeShape s = lattice_shape(a.S + 1);
+  if (s.NP == 1) return launch_lattice<1, 16, 2, GRAD>(a, s.nw, stream);
+  if (s.NP == 2) return launch_lattice<2, 16, 2, GRAD>(a, s.nw, stream);
+  if (s.NP == 3) return launch_lattice<3, 16, 2, GRAD>(a, s.nw, stream);
+  if (s.H == 8) return launch_lattice<4, 8, 2, GRAD>(a, s.nw, stream);
+  return launch_lattice<4, 4, 2, GRAD>(a, s.nw, stream);
 }
 
 // utterances [b0, b0 + 65535): a grid's second extent
@@ -1021,8 +1031,7 @@ int ctc_pitch(int S) { return (S + 3 + 3) / 4 * 4; }
 int ctc_state_pitch(int S) {
   using namespace ctc_loss_impl;
   // the states of the pairs, and a reference for every lane of the warps that hold them
-  int warps = lattice_warps(S + 1, 4, halo_lanes<4, 4>());
-  return 2 * ctc_pitch(S) + 32 * (warps > 4 ? warps : 4);
+  return 2 * ctc_pitch(S) + 32 * lattice_shape(S + 1).nw;
 }
 
 int launch_ctc_loss(const CtcArgs& args, int dtype, cudaStream_t stream) {

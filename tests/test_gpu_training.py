@@ -365,7 +365,7 @@ def test_ctc_loss(B, T, V, S, dtype):
     check_ctc(*ctc_case(B * 1000 + T, B, T, V, S, dtype))
 
 
-@pytest.mark.parametrize("S", [79, 80, 207, 208, 329, 330, 900, 967, 968])
+@pytest.mark.parametrize("S", [79, 80, 207, 208, 329, 330, 368, 489, 499, 615, 740, 860, 900, 967, 968])
 def test_ctc_label_counts(S):
     """Around the counts where a lane holds more of them or a block fewer frames; long and short chains beside them."""
     il, tl = [2 * S + 40, S + 30, 17], [S, S // 3, 5]

@@ -159,3 +159,20 @@ def test_keep_mask_probability():
         n = keep.numel()
         assert abs(keep.double().mean().item() - (1 - p)) < 5 * np.sqrt(p * (1 - p) / n) + 2 ** -17
     assert R.keep_mask((3, 9), 1, 0, 0, 0.0).all() and not R.keep_mask((3, 9), 1, 0, 0, 1.0).any()
+
+
+def test_ctc_workspace_holds_every_lane_reference():
+    """A frame's stored states: two words for each of the S + 1 pairs, and one for each lane of the warps that hold them
+    (the first 32 lanes of NP pairs, the others less the lanes that repeat the warp below)."""
+    lib = _lib.lib()
+
+    def warps(pairs, NP, H):
+        halo = -(-H // NP)
+        return 1 if pairs <= 32 * NP else 1 - (32 * NP - pairs) // ((32 - halo) * NP)
+
+    for S in range(0, training.MAX_CTC_LABELS + 1):
+        shapes = [(1, 16, 4), (2, 16, 4), (3, 16, 4), (4, 8, 8), (4, 4, 99)]
+        nw = next(warps(S + 1, NP, H) for NP, H, most in shapes if warps(S + 1, NP, H) <= most)
+        frames = 1000
+        states = lib.gsn_ctc_loss_workspace_bytes(1, frames, S, 1) - lib.gsn_ctc_loss_workspace_bytes(1, frames, S, 0)
+        assert states >= frames * 4 * (2 * (S + 1) + 32 * nw), S
