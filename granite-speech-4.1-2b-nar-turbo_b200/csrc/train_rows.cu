@@ -9,6 +9,8 @@
 //
 // Every one of them moves each tensor once, so HBM bounds it.  Tensors are bf16, fp16 or fp32, all arithmetic is fp32.
 // Rows are M = B * T frames; with lengths, the frames t >= lengths[b] are padding: their x and dy are not read.
+#include <algorithm>
+
 #include "gsn_kernels.cuh"
 #include "gsn_ptx.cuh"
 
@@ -327,11 +329,14 @@ struct Kept {
   }
 
   __device__ __forceinline__ void apply(int i, uint32_t threshold16, float2 (&f)[4]) const {
-    if constexpr (OWN) return keep8(drawn[i], threshold16, f);
+    if constexpr (OWN) {
+      keep8(drawn[i], threshold16, f);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      f[k].x = bits & (1u << (8 * i + 2 * k)) ? f[k].x : 0.f;
-      f[k].y = bits & (2u << (8 * i + 2 * k)) ? f[k].y : 0.f;
+      for (int k = 0; k < 4; ++k) {
+        f[k].x = bits & (1u << (8 * i + 2 * k)) ? f[k].x : 0.f;
+        f[k].y = bits & (2u << (8 * i + 2 * k)) ? f[k].y : 0.f;
+      }
     }
   }
 };
@@ -867,7 +872,7 @@ int launch_bwd(const RowArgs& a, const RowShape& s, cudaStream_t stream) {
   const int R = s.warps / s.W;
   constexpr int words = Ring<T, NV, DROP ? 3 : 2>::WORDS;
   const size_t ring = VEC ? sizeof(uint4) * ring_stages(words) * words * kRowThreads : 0;
-  const size_t sums = R > 1 ? (size_t)2 * a.D * sizeof(float) : 0, smem = ring > sums ? ring : sums;
+  const size_t sums = R > 1 ? (size_t)2 * a.D * sizeof(float) : 0, smem = std::max(ring, sums);
   auto* kernel = ln_bwd_kernel<T, NV, VEC, DROP>;
   static std::atomic<uint64_t> allowed{0};         // an instantiation's ring is fixed, its sums are 32 KB at most
   if (smem > 32 * 1024)                            // with the static part, more than a launch gets unasked

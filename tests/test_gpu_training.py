@@ -653,3 +653,40 @@ def test_functions_refuse_mismatched_tensors():
                  lambda: tr.ctc_loss(x, i[:, None], i[:1], i)):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_functions_record_what_the_ops_record():
+    """The functions' gradients are the dispatcher ops' bit for bit; dropout's gradient has a gradient of its own, those
+    of the norms and of the loss refuse to be differentiated."""
+    ff, x, targets, il, tl = tail_case(80)
+    w, b, rng = rand(81, (x.shape[-1],), F32), rand(82, (x.shape[-1],), F32), rng_of(9, 2)
+    logits = rand(83, (3, 24, 30), BF)
+    o = torch.ops.granite
+    pairs = [
+        (lambda u: tr.layer_norm(u, w, b, EPS, il), lambda u: o.layer_norm(u, w, b, EPS, il), x),
+        (lambda u: tr.dropout_add(u, rng, 0.2, x, 0.5, 3, il), lambda u: o.dropout_add(u, x, rng, 0.2, 0.5, 3, il), ff),
+        (lambda u: tr.dropout_add_layer_norm(ff, u, w, b, rng, 0.2, 0.5, 1, EPS, il),
+         lambda u: o.dropout_add_layer_norm(ff, u, w, b, rng, 0.2, 0.5, 1, EPS, il), x),
+        (lambda u: tr.ctc_loss(u, targets, il, tl), lambda u: o.ctc_loss(u, targets, il, tl, 0, False)[0], logits),
+    ]
+    for function, op, at in pairs:
+        got = []
+        for f in (function, op):
+            u = at.clone().requires_grad_()
+            out = f(u)
+            first = out[0] if isinstance(out, tuple) else out
+            d = torch.linspace(-1.0, 1.0, first.numel(), device=DEV).reshape(first.shape).to(first.dtype)
+            got.append((first.detach(), *torch.autograd.grad(first, u, d)))
+        assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    u = ff.clone().requires_grad_()
+    d = x.clone().requires_grad_()
+    du, = torch.autograd.grad(tr.dropout_add(u, rng, 0.2), u, d, create_graph=True)
+    dd, = torch.autograd.grad(du, d, ff)
+    assert torch.equal(dd, tr.dropout_add(ff, rng, 0.2))
+    for function, _, at in (pairs[0], pairs[2], pairs[3]):
+        u = at.clone().requires_grad_()
+        out = function(u)
+        first = out[0] if isinstance(out, tuple) else out
+        du, = torch.autograd.grad(first.float().square().sum(), u, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(du.float().sum(), u)
