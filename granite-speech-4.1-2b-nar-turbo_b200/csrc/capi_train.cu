@@ -40,19 +40,28 @@ int check_params(const char* name, int D, int dtype, int param_dtype, const void
   return 0;
 }
 
+// of 65536 numbers, those below it drop; what remains is multiplied by the factor
+uint32_t dropout_threshold(double p) { return (uint32_t)nearbyint(p * 65536.0); }
+
+float dropout_factor(double p, double scale) {
+  const uint32_t threshold = dropout_threshold(p);
+  return threshold > 65535u ? 0.f : (float)(scale * 65536.0 / (65536.0 - threshold));
+}
+
 int check_dropout(const char* name, const int64_t* rng, double p, double scale) {
   if (!rng || !aligned(rng, 8)) return fail(GSN_ERR_INVALID_ARG, "%s: rng must be a device int64[2]", name);
   if (!(p >= 0.0 && p <= 1.0)) return fail(GSN_ERR_INVALID_ARG, "%s: p=%g is not a probability", name, p);
-  if (!isfinite(scale)) return fail(GSN_ERR_INVALID_ARG, "%s: scale=%g", name, scale);
+  if (!isfinite(scale) || !isfinite(dropout_factor(p, scale)))
+    return fail(GSN_ERR_INVALID_ARG, "%s: scale=%g with p=%g is not finite in fp32", name, scale, p);
   return 0;
 }
 
 void set_dropout(RowArgs& a, const int64_t* rng, uint32_t site, double p, double scale) {
   a.rng = rng;
   a.site = site;
-  a.threshold = (uint32_t)nearbyint(p * 65536.0);
+  a.threshold = dropout_threshold(p);
   a.drop_all = a.threshold > 65535u;
-  a.factor = !a.drop_all ? (float)(scale * 65536.0 / (65536.0 - a.threshold)) : 0.f;
+  a.factor = dropout_factor(p, scale);
 }
 
 RowArgs row_args(int64_t M, int D, float eps, const int32_t* lengths, int T, int param_dtype) {

@@ -54,6 +54,13 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+def _int32(t: torch.Tensor) -> torch.Tensor:
+    """Dense int32; what int64 holds beyond it stays out of every range."""
+    if t.dtype == torch.int64:
+        t = t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+    return t.contiguous()
+
+
 def _check_device(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
     if not first.is_cuda:
         raise RuntimeError(f"{name}: every tensor must be on a CUDA device (got {first.device}); the kernels have no "
@@ -98,7 +105,7 @@ def _check_lengths(name: str, x: torch.Tensor, lengths: Optional[torch.Tensor]) 
     if x.dim() != 3 or lengths.shape != x.shape[:1] or lengths.dtype not in (torch.int32, torch.int64):
         raise RuntimeError(f"{name}: lengths must be int [B] beside [B, T, D], got {lengths.dtype} "
                            f"{tuple(lengths.shape)} beside {tuple(x.shape)}")
-    return lengths.to(torch.int32).contiguous(), x.shape[1]
+    return _int32(lengths), x.shape[1]
 
 
 def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
@@ -469,7 +476,7 @@ def _ctc_operands(logits, targets, input_lengths, target_lengths):
     if (sv != 1 and V > 1) or (st < V and T > 1):
         logits = logits.contiguous()
         sb, st, _ = logits.stride()
-    i32 = [t.to(torch.int32).contiguous() for t in (targets, input_lengths, target_lengths)]
+    i32 = [_int32(t) for t in (targets, input_lengths, target_lengths)]
     return logits, sb, st if T > 1 else V, i32
 
 

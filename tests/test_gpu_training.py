@@ -690,3 +690,88 @@ def test_functions_record_what_the_ops_record():
         du, = torch.autograd.grad(first.float().square().sum(), u, create_graph=True)
         with pytest.raises(RuntimeError):
             torch.autograd.grad(du.float().sum(), u)
+
+
+# ---- the ends of the ranges ------------------------------------------------------------------------------------------
+def test_ctc_wide_integers():
+    """int64 labels and lengths that int32 does not hold are outside, not what their low halves say."""
+    logits, targets, il, tl = ctc_case(200, 4, 12, 9, 4, F32)
+    targets, il, tl = targets.long(), il.long(), tl.long()
+    targets[1, 2] += 2 ** 32
+    il[2] += 2 ** 32
+    tl[3] -= 2 ** 33
+    loss = tr.ctc_loss(logits, targets, il, tl)
+    assert torch.isfinite(loss[0]) and torch.isnan(loss[1:]).all()
+    x, w = rand(201, (2, 3, 16), BF), torch.ones(16, device=DEV)
+    lengths = torch.tensor([2 ** 32 + 1, -2 ** 32 + 1], device=DEV)
+    y = tr.layer_norm(x, w, w, EPS, lengths)
+    assert torch.equal(y[0], tr.layer_norm(x, w, w, EPS, torch.tensor([3, 0], device=DEV))[0]) and not y[1].any()
+
+
+def test_ctc_one_class():
+    """A vocabulary of the blank alone: the loss is 0 without labels; as a label the blank needs one frame of its own."""
+    logits, targets, il, tl = ctc_case(202, 3, 4, 1, 2, F32, ([4, 4, 1], [0, 2, 2]), labels=[[0, 0]] * 3)
+    check_ctc(logits, targets, il, tl)
+
+
+def test_ctc_more_utterances_than_a_grid_holds():
+    B = 65535 + 9
+    logits, targets, il, tl = ctc_case(203, 7, 3, 5, 2, BF, ([3, 2, 1, 3, 0, 3, 2], [2, 1, 1, 0, 0, 2, 2]))
+    base, grad = check_ctc(logits, targets, il, tl, dloss=torch.ones(7, device=DEV))
+    many = [t.repeat(-(-B // 7), *[1] * (t.dim() - 1))[:B] for t in (logits, targets, il, tl)]
+    x = many[0].requires_grad_()
+    loss = tr.ctc_loss(x, *many[1:])
+    got, = torch.autograd.grad(loss, x, torch.ones(B, device=DEV))
+    # rows of five bf16 logits begin at every alignment, and a row's sum at its first 16-byte boundary: its order, so not
+    # its bits, is the utterance's own.  Both sides lie within check_ctc's bounds (T = 3, V = 5) of the same number.
+    want, wgrad = base.repeat(-(-B // 7))[:B].detach().double(), grad.repeat(-(-B // 7), 1, 1)[:B].double()
+    per_frame = (5 / 256 + 100) * E
+    fin = torch.isfinite(want)
+    assert torch.equal(fin, torch.isfinite(loss)) and torch.equal(want == math.inf, loss == math.inf)
+    assert ((loss.double() - want).abs()[fin] <= (2 * (3 * per_frame + E * want.abs() * (1 + E) + 1e-6))[fin]).all()
+    ok = ~torch.isnan(wgrad)
+    assert torch.equal(ok, ~torch.isnan(got))
+    bound = 2 * (rounded(BF, wgrad) * (1 + 2 ** -8) + per_frame + (3 * 64 + 164) * E)
+    assert ((got.double() - wgrad).abs()[ok] <= bound[ok]).all()
+
+
+def test_ctc_longest_chain():
+    check_ctc(*ctc_case(204, 2, tr.MAX_CTC_FRAMES, 5, 20, F32, ([tr.MAX_CTC_FRAMES, 9001], [20, 13])))
+
+
+def test_elements_past_32_bits():
+    """More elements than an int counts: the last rows and the last utterance as they are alone."""
+    M, D = 2 ** 21 + 104, 1024
+    g = torch.Generator(device=DEV).manual_seed(205)
+    x = torch.randn(M, D, device=DEV, generator=g, dtype=BF)
+    res = torch.randn(M, D, device=DEV, generator=g, dtype=BF)
+    w, b, rng = rand(206, (D,), F32, 0.1, 1.0), rand(207, (D,), F32, 0.1), rng_of(3, 4)
+    last = slice(M - 40, M)
+    y, h = tr.dropout_add_layer_norm(x, res, w, b, rng, 0.0)
+    y1, h1 = tr.dropout_add_layer_norm(x[last], res[last], w, b, rng, 0.0)
+    assert torch.equal(y[last], y1) and torch.equal(h[last], h1)
+    del y, h
+    dx, dres, _, _ = tr.dropout_add_layer_norm_backward(x, res, x, w, rng, 0.0)
+    dx1, dres1, _, _ = tr.dropout_add_layer_norm_backward(x[last], res[last], x[last], w, rng, 0.0)
+    assert torch.equal(dx[last], dx1) and torch.equal(dres[last], dres1)
+    del dx, dres
+    out = tr.dropout_add(x, rng, 0.25, res)
+    kept = out[M - 2:].double().cpu() != res[M - 2:].double().cpu()
+    groups = np.arange((M - 2) * (D // 8), M * (D // 8), dtype=np.uint64)
+    r = R.philox((groups & np.uint64(0xFFFFFFFF), groups >> np.uint64(32), np.full(groups.shape, 4, np.uint64),
+                  np.zeros(groups.shape, np.uint64)), (3, 0))
+    halves = np.stack([(v >> np.uint64(16 * i)) & np.uint64(0xFFFF) for v in r for i in (0, 1)], -1).reshape(2, D)
+    keep = torch.from_numpy(halves >= 16384)
+    # a kept element is the sum rounded, the residual itself only where x is lost beside it
+    assert not (kept & ~keep).any() and (keep & ~kept).sum() < 16
+    del x, res, out
+    B, T, V = 2, 10800, 100352
+    logits = torch.randn(B, T, V, device=DEV, generator=g, dtype=BF).requires_grad_()
+    targets = torch.randint(1, V, (B, 30), device=DEV, generator=g, dtype=torch.int32)
+    il, tl = lens_of([T, T - 7]), lens_of([30, 29])
+    loss = tr.ctc_loss(logits, targets, il, tl)
+    grad, = torch.autograd.grad(loss.sum(), logits)
+    alone = logits[1:].detach().requires_grad_()
+    loss1 = tr.ctc_loss(alone, targets[1:], il[1:], tl[1:])
+    grad1, = torch.autograd.grad(loss1.sum(), alone)
+    assert torch.equal(loss[1:], loss1) and torch.equal(grad[1:], grad1)

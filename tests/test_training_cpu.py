@@ -51,6 +51,7 @@ def test_row_entry_points_refuse_bad_calls():
     assert drop(p=-0.1) == 1 and drop(p=1.1) == 1 and drop(p=float("nan")) == 1
     assert drop(rng=None) == 1 and drop(rng=ctypes.c_void_p(260)) == 1
     assert drop(scale=float("inf")) == 1 and drop(ld_r=8) == 2 and drop(M=0) == 0
+    assert drop(scale=1e39) == 1 and drop(p=0.99998, scale=1e37) == 1 and "fp32" in _lib.last_error()
 
     def both(res=P, h=P, p=0.1):
         return L.gsn_dropout_add_layer_norm_fwd(P, 64, res, 64, P, P, P, h, 4, 64, 1e-5, 0, 2, P, 0, p, 1.0, None, 0,
