@@ -258,7 +258,8 @@ constexpr int kRowThreads = 256;
 constexpr int kWarpRowV = 2048;                  // up to it a warp takes a row, beyond it a CTA
 
 // Frames of one utterance that a warp takes: two, which share what is looked up of the transcript, where that leaves
-// 16 warps an SM; a CTA takes one.
+// 16 warps an SM; a CTA takes one.  48 x 1536 x 348 with 300 labels: rows and gradient 47 and 59 us, with three frames
+// 55 and 71, with four 70 and 75.
 int warp_frames(const CtcArgs& a) { return (int64_t)a.B * a.T >= 32 * device_sm_count() ? 2 : 1; }
 
 // block (frames, utterance); the last block of an utterance plans it
