@@ -548,11 +548,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 
       }
     }
     E = hi;
-    // where nothing but zeros reaches a lane, nothing comes from below within the block either
-    const int lower = __shfl_up_sync(0xffffffffu, E, 1) - E;
-    const bool closed = lane == 0 || E < kZeroBelow;
-    below = __hiloint2double(closed || lower < -1000 ? 0 : (min(lower, 1000) + 1023) << 20, 0);
-    return __all_sync(0xffffffffu, (lo == INT_MAX || hi - lo + span <= kFastSpan) && (closed || lower <= 900)) != 0;
+    // Where nothing but zeros reaches a lane or the one below it, nothing comes from below within the block.  A lane
+    // below that lies further down than the factor reaches still counts: its path can be the one that goes on.
+    const int under = __shfl_up_sync(0xffffffffu, E, 1), lower = under - E;
+    const bool closed = lane == 0 || E < kZeroBelow || under < kZeroBelow, held = lower >= -1000 && lower <= 900;
+    below = __hiloint2double(closed || !held ? 0 : (lower + 1023) << 20, 0);
+    return __all_sync(0xffffffffu, (lo == INT_MAX || hi - lo + span <= kFastSpan) && (closed || held)) != 0;
   };
   auto fast_frames = [&](auto second, int k, const uint32_t* em, const uint32_t* st) {
     constexpr bool SECOND = decltype(second)::value;
