@@ -275,9 +275,9 @@ size_t gsn_ctc_loss_state_bytes(int B, int T, int S) {
 
 size_t gsn_ctc_loss_workspace_bytes(int B, int T, int S, int gradient) {
   if (B <= 0 || T < 0 || S < 0 || S > kMaxCtcLabels) return 0;
-  size_t n = align256((size_t)B * sizeof(int)) + align256((size_t)B * T * sizeof(float)) +
-             align256((size_t)B * 4 * ctc_pitch(S) * sizeof(float2));
-  if (gradient) n += (size_t)B * T * ctc_state_pitch(S) * sizeof(uint32_t);
+  size_t n = 2 * align256((size_t)B * sizeof(int)) + align256((size_t)B * T * sizeof(float)) +
+             align256((size_t)B * 8 * ctc_pitch(S) * sizeof(float2));
+  if (gradient) n += (size_t)B * T * (ctc_state_pitch(S) + ctc_pitch(S)) * sizeof(uint32_t);
   return n;
 }
 
@@ -299,10 +299,15 @@ int gsn_ctc_loss_fwd(const void* logits, int64_t ld_b, int64_t ld_t, const int32
   char* ws = static_cast<char*>(workspace);
   a.bad = (int*)ws;
   ws += align256((size_t)B * sizeof(int));
+  a.again = (int*)ws;
+  ws += align256((size_t)B * sizeof(int));
   a.norms = (float*)ws;
   ws += align256((size_t)B * T * sizeof(float));
   a.exchange = (float2*)ws;
-  if (gradient) a.states = (uint32_t*)(ws + align256((size_t)B * 4 * a.pitch * sizeof(float2)));
+  if (gradient) {
+    a.states = (uint32_t*)(ws + align256((size_t)B * 8 * a.pitch * sizeof(float2)));
+    a.upper = a.states + (size_t)B * T * a.state_pitch;
+  }
   return finish(launch_ctc_loss(a, dtype, (cudaStream_t)stream), name);
 }
 

@@ -41,11 +41,27 @@ __device__ __forceinline__ float pow2i(int d) { return __int_as_float(max(d + 12
 
 // Stored numbers, emissions and states alike, are the high word of an fp64: 11 bits of exponent, 20 of mantissa,
 // rounded to nearest (2^-21, an eighth of an fp32 logit's own step at 10).  0 is zero.  An emission is against the
-// frame's likeliest class of the transcript; a state against its lane's reference exponent, stored beside it.
+// frame's likeliest class of the transcript; a state against its lane's reference exponent, stored beside it.  That
+// holds states down to 2^-kWordSpan of their lane's largest.  Labels that the logits favour in another order than the
+// transcript's lie further apart, and the lower one can carry the whole posterior: such an utterance is walked again
+// with every state's own exponent stored.
 constexpr uint32_t kWordOne = 1u << 20;       // words below it are zeros
+constexpr int kWordSpan = 1000;
 __device__ __forceinline__ uint32_t to_word(float m, int e) {          // m * 2^e, 0 where it leaves the range
   const uint32_t v = ((__float_as_uint(m) + 4u) >> 3) + ((uint32_t)(e + 896) << 20);
-  return e < -1000 ? 0u : v;
+  return e < -kWordSpan ? 0u : v;
+}
+// A state with its own exponent: 20 bits of mantissa and the low 12 of the exponent, its upper 16 apart (0: a zero).
+constexpr int kWideBias = (1 << 28) - (1 << 16);   // exponents from -2^28 + 2^16 to 2^16 as 28 bits
+__device__ __forceinline__ uint32_t to_wide(float m, int e, uint32_t& upper) {
+  const uint32_t bits = __float_as_uint(m), t = ((bits & 0x7FFFFFu) + 4u) >> 3;
+  const int field = e < kZeroBelow ? 0 : e + (int)(bits >> 23) - 127 + (int)(t >> 20) + kWideBias;
+  upper = (uint32_t)field >> 12;
+  return (t << 12) | ((uint32_t)field & 0xFFFu);
+}
+__device__ __forceinline__ float wide_mantissa(uint32_t v) { return __uint_as_float((v >> 12 << 3) | 0x3F800000u); }
+__device__ __forceinline__ int wide_exponent(uint32_t v, uint32_t upper) {
+  return (int)((upper << 12) | (v & 0xFFFu)) - kWideBias;
 }
 // A double in [0, 2^127) cut to fp32, zero below 2^-126: three integer instructions (the conversion instruction from
 // fp64 runs at a sixteenth of their rate or less: with it a frame of three pairs a lane took 455 cycles, not 160).
@@ -168,7 +184,10 @@ __device__ __forceinline__ void plan_utterance(const CtcArgs& a, int b) {
     order[rank] = make_int2(i < len ? i : a.S + 1, v);           // where its posterior lies, its class
   }
   bad = __syncthreads_or(bad);
-  if (threadIdx.x == 0) a.bad[b] = bad;
+  if (threadIdx.x == 0) {
+    a.bad[b] = bad;
+    a.again[b] = 0;
+  }
 }
 
 // exp(a) as a stored word, for a <= 0; 0 (impossible) below kLowest and for NaN (the frame's sum tells of it)
@@ -329,13 +348,14 @@ __host__ __device__ constexpr int lattice_warps(int pairs, int NP, int HL) {
 }
 
 // Four warps at most hold up to three pairs a lane; one more warp fetches the frames and adds up the blanks.
-template <int NP, int H, int NBUF, bool GRAD>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 8 ? 288 : 576)
-    ctc_lattice_kernel(CtcArgs a, int nw) {
+// WIDE: every block on the exponents of its states, and every state stored with its own.  Otherwise true comes back, on
+// both sides, where the utterance has to be walked so for its posteriors: none is written yet, the loss is.
+template <int NP, int H, int NBUF, bool GRAD, bool WIDE>
+__device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
   constexpr int HL = halo_lanes<NP, H>(), NS = 2 * NP;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[NBUF];
-  __shared__ double sums[32];
+  __shared__ double norms_sum;
   __shared__ float zm[32];
   __shared__ int ze[32];
   const int dir = blockIdx.x, b = blockIdx.y;
@@ -349,7 +369,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 
       a.raw_loss[b] = raw;
       a.loss[b] = a.zero_infinity && raw == INFINITY ? 0.f : raw;
     }
-    return;
+    return false;
   }
   const int pitch = a.pitch, spitch = a.state_pitch, brow = nw * 32 + 4;
   const int64_t frame0 = (int64_t)b * a.T;
@@ -413,7 +433,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 
 
   const int h = (n + 1) / 2, n1 = dir ? n - h : h;  // this side's frames before the meeting
   int issued = 0, waited = 0, blocks = 0, parity = 0;
-  bool fail = false;
+  bool fail = false, again = false;
 
   // frames [k, k + cnt) of this side's order are rows lo, lo + 1, ...
   auto issue = [&](int k, int cnt, bool states) {
@@ -473,6 +493,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 
     st += first * spitch;
     [[maybe_unused]] float* post = a.post + frame * pitch;
     [[maybe_unused]] uint32_t* dst = a.states + frame * spitch;
+    [[maybe_unused]] uint32_t* upper = a.upper + frame * pitch;
     [[maybe_unused]] float* bl = blanks + parity * H * brow + tid;
     for (int f = 0; f < cnt; ++f) {
       float pm[NS];
@@ -485,7 +506,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 
         m[s] = pm[s] * word_mantissa(x);
         e[s] = max(pe[s] + (x < kWordOne ? kZeroExp : (int)(x >> 20) - 1023), kZeroExp);
       }
-      if constexpr (SECOND) {
+      if constexpr (SECOND && WIDE) {
+        auto joint = [&](int q, int s, float pm, int pe) {         // with state s (0 blank, 1 label) of the pair q
+          q = max(q, 0);
+          const uint32_t v = st[2 * q + s], u = __ldcg(upper + q) >> (16 * s) & 0xFFFFu;
+          return u == 0 ? 0.f : pm * (wide_mantissa(v) * zinv) * pow2i(wide_exponent(v, u) - zexp + pe);
+        };
+        float blank = 0.f;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          if (j < blanks_here) blank += joint(q0 - j, 0, pm[2 * j], pe[2 * j]);
+          if (j < labels_here) post[slot[j]] = joint(q0 - j - 1, 1, pm[2 * j + 1], pe[2 * j + 1]);
+        }
+        bl[f * brow] = blank;
+        post += step * pitch;
+        upper += step * pitch;
+        st += step * spitch;
+      } else if constexpr (SECOND) {
         const int rh = (int)st[ref_hi] - zexp, rl = (int)st[ref_lo] - zexp;
         float blank = 0.f;
 #pragma unroll
@@ -501,10 +538,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 
         bl[f * brow] = blank;
         post += step * pitch;
         st += step * spitch;
+      } else if constexpr (GRAD && WIDE) {
+#pragma unroll
+        for (int j = 0; j < NP; ++j)
+          if (j < blanks_here) {
+            uint32_t ub, ul;
+            const uint32_t vb = to_wide(m[2 * j], e[2 * j], ub), vl = to_wide(m[2 * j + 1], e[2 * j + 1], ul);
+            *reinterpret_cast<uint2*>(dst + 2 * (i0 + j)) = make_uint2(vb, vl);
+            upper[i0 + j] = ub | ul << 16;
+          }
+        dst += step * spitch;
+        upper += step * pitch;
       } else if constexpr (GRAD) {
         int ref = e[0];
 #pragma unroll
         for (int s = 1; s < NS; ++s) ref = max(ref, e[s]);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) again |= own && e[s] >= kZeroBelow && e[s] < ref - kWordSpan;
 #pragma unroll
         for (int j = 0; j < NP; ++j)
           if (j < blanks_here)
@@ -701,10 +751,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 
         refresh_halo();
         const uint32_t* em = em_ring + buf * H * pitch;
         const uint32_t* st = st_ring + buf * H * spitch;
-        if (cnt == H && fast_block(em))
-          fast_frames(second, k, em, st);
-        else
+        bool fast = false;
+        if constexpr (!WIDE) fast = cnt == H && fast_block(em);
+        if (fast) {
+          if constexpr (!WIDE) fast_frames(second, k, em, st);
+        } else {
           frames(second, k, cnt, em, st);
+        }
         publish_halo();
       }
       fail = __syncthreads_or(!ok);
@@ -729,19 +782,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 
   walk(0, n1, std::false_type{});
 
   // the meeting: Z = sum over the states of this side's sum into them times the other side's value
-  float2* mine = a.exchange + ((int64_t)b * 2 + dir) * 2 * pitch;
-  const float2* theirs = a.exchange + ((int64_t)b * 2 + (dir ^ 1)) * 2 * pitch;
+  // (one place for either walk: the other side may still be at the first one's meeting)
+  float2* mine = a.exchange + (((int64_t)b * 2 + WIDE) * 2 + dir) * 2 * pitch;
+  const float2* theirs = a.exchange + (((int64_t)b * 2 + WIDE) * 2 + (dir ^ 1)) * 2 * pitch;
 #pragma unroll
   for (int j = 0; j < NP; ++j)
     if (j < blanks_here) {
       mine[2 * (i0 + j)] = make_float2(m[2 * j], __int_as_float(e[2 * j]));
       mine[2 * (i0 + j) + 1] = make_float2(m[2 * j + 1], __int_as_float(e[2 * j + 1]));
     }
+  if (again) a.again[b] = 1;                       // any lane's, either side's
   // the states were stored by plain stores and are fetched by bulk copies of the other CTA
   asm volatile("fence.proxy.async;" ::: "memory");
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   asm volatile("fence.proxy.async;" ::: "memory");
-  if (fail) return drain();
+  if (fail) {
+    drain();
+    return false;
+  }
+  if constexpr (!WIDE) again = __ldcg(a.again + b) != 0;
   {
     int top = 2 * kZeroExp;
     float total = 0.f;
@@ -772,7 +831,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 
     if (producer) {
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, d);
-      if (lane == 0) sums[0] = norm;
+      if (lane == 0) norms_sum = norm;
     } else if (lane == 0) {
       zm[w] = total;
       ze[w] = top;
@@ -783,15 +842,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 
     total = 0.f;
     for (int i = 0; i < nw; ++i) total += zm[i] * pow2i(ze[i] - top);
     const bool exists = top > kZeroBelow;
-    if (dir == 0 && tid == 0) {
-      norm = sums[0];
+    if (!WIDE && dir == 0 && tid == 0) {
+      norm = norms_sum;
       float raw = INFINITY;
       if (exists) raw = (float)((norm - (double)top - log2((double)total)) * 0.6931471805599453);
       if (!(norm > -INFINITY)) raw = NAN;          // a frame of NaN, +inf or nothing but -inf
       a.raw_loss[b] = raw;
       a.loss[b] = a.zero_infinity && raw == INFINITY ? 0.f : raw;
     }
-    if (!GRAD || !exists) return;
+    if (!GRAD || !exists) return false;
+    if (!WIDE && again) return true;
     const int bits = __float_as_int(total), k = (bits >> 23) - 127;
     zinv = 1.f / __int_as_float(bits - (k << 23));
     zexp = top + k;
@@ -800,6 +860,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 
     walk(n1, n, std::true_type{});
     if (fail) drain();
   }
+  return false;
+}
+
+// a function of its own: its code beside the other walk's took a fifth of that one's speed
+template <int NP, int H, int NBUF, bool GRAD>
+__device__ __noinline__ void lattice_wide(const CtcArgs& a, int nw) {
+  __syncthreads();                                 // the first walk's shared memory is free
+  lattice_walk<NP, H, NBUF, GRAD, true>(a, nw);
+}
+
+template <int NP, int H, int NBUF, bool GRAD>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 8 ? 288 : 576)
+    ctc_lattice_kernel(const __grid_constant__ CtcArgs a, int nw) {
+  if (lattice_walk<NP, H, NBUF, GRAD, false>(a, nw)) lattice_wide<NP, H, NBUF, GRAD>(a, nw);
 }
 
 // ---- gradient --------------------------------------------------------------------------------------------------------
@@ -936,7 +1010,7 @@ __global__ void __launch_bounds__(WARP_ROW ? kRowThreads : kCtaThreads) ctc_grad
   if (tid < 32) grad_labels<T, F>(a, p, x, g, frame, count, b, tid);
 }
 
-constexpr size_t kMostSmem = 227 * 1024 - 1024;  // a CTA's, less the static part
+constexpr size_t kMostSmem = 227 * 1024 - 1024;  // a CTA's, less the static part (of both walks)
 
 template <int NP, int H, int NBUF, bool GRAD>
 int launch_lattice(const CtcArgs& a, int nw, cudaStream_t stream) {
@@ -989,8 +1063,10 @@ CtcArgs batch_part(const CtcArgs& a, int b0, int size) {
   if (c.loss) c.loss += b0;
   if (c.bad) c.bad += b0;
   if (c.norms) c.norms += frames;
-  if (c.exchange) c.exchange += (int64_t)b0 * 4 * a.pitch;
+  if (c.again) c.again += b0;
+  if (c.exchange) c.exchange += (int64_t)b0 * 8 * a.pitch;
   if (c.states) c.states += frames * a.state_pitch;
+  if (c.upper) c.upper += frames * a.pitch;
   if (c.dloss) c.dloss += b0;
   if (c.dlogits) c.dlogits = static_cast<char*>(a.dlogits) + frames * a.V * size;
   return c;

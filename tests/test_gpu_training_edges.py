@@ -48,3 +48,67 @@ def test_ctc_path_from_a_lane_far_below(S, at, boost, K):
         loss = tr.ctc_loss(logits, targets, il, tl).double().cpu()
         # check_ctc's bound: n frames' normalisers and steps, and the loss's own rounding
         assert abs(loss - ref) <= logits.shape[1] * 100 * E + E * ref + 1e-6, (float(loss), float(ref))
+
+
+def sharp_check(logits, targets, il, tl, blank=0):
+    """check_ctc, and the gradient against what the stored words leave: an emission is rounded by 2^-21 of itself, its
+    exponent (log2 e in fp32, a difference of logits up to 32) by 2^-20, so a posterior, a share of two products of n
+    of them, by less than n 2^-19."""
+    _, grad = check_ctc(logits, targets, il, tl, blank, dloss=torch.ones(logits.shape[0], device=DEV))
+    ref = R.ctc(logits, targets, il, tl, blank, False)[1]
+    d = (grad.double().cpu() - ref).abs()
+    bound = rounded(logits.dtype, ref) + logits.shape[1] * 2.0 ** -19 + (logits.shape[2] / 256 + 100) * E
+    assert (d <= bound).all(), float(d.max())
+
+
+@pytest.mark.parametrize("S,at,K,boost,back", [(100, 44, 100, 15.0, 5), (300, 147, 75, 20.0, 5), (300, 150, 40, 30.0, 3),
+                                               (500, 240, 60, 25.0, 5), (1200, 600, 90, 25.0, 5)])
+def test_ctc_posterior_far_below_its_lane(S, at, K, boost, back):
+    """a and b in one lane, b favoured K frames and a behind it: a's states lie up to 3246 octaves below b's and carry
+    the posterior; words against the lane's largest would drop them."""
+    case = run_case(S, at, [("b", K, boost), ("a", K + back, boost)])
+    sharp_check(*case)
+    sharp_check(*backwards(*case))
+
+
+@pytest.mark.parametrize("S,at", [(60, 24), (100, 45), (300, 148), (500, 243)])
+def test_ctc_posterior_in_a_blank_far_below_its_label(S, at):
+    """The label favoured, then the blank, then the label again: the posterior lies on the blank before it."""
+    case = run_case(S, at, [("a", 80, 20.0), ("blank", 80, 20.0), ("a", 85, 20.0)])
+    sharp_check(*case)
+    sharp_check(*backwards(*case))
+
+
+def test_ctc_utterances_far_apart_beside_others():
+    """Only the utterances that need it are walked with every state's exponent; a captured call does the same."""
+    far = [run_case(100, 44, [("b", 100, 15.0), ("a", 105, 15.0)]), run_case(100, 45, [("a", 80, 20.0), ("blank", 80, 20.0),
+                                                                                      ("a", 85, 20.0)])]
+    plain = ctc_case(31, 3, 560, 13, 100, F32, ([560, 410, 0], [100, 90, 0]))
+    T = 560
+    logits, targets = [plain[0]], [plain[1]]
+    for x, lab, _, _ in far:
+        logits.append(torch.cat([x, torch.full((1, T - x.shape[1], 13), float("nan"), device=DEV)], 1))
+        targets.append(lab)
+    il, tl = (torch.cat([plain[i], *[c[i] for c in far]]) for i in (2, 3))
+    order = torch.tensor([3, 0, 4, 1, 2], device=DEV)
+    case = [t[order].contiguous() for t in (torch.cat(logits), torch.cat(targets), il, tl)]
+    sharp_check(*case)
+
+    def step():
+        x = case[0].detach().requires_grad_()
+        loss = tr.ctc_loss(x, *case[1:])
+        return loss.detach(), torch.autograd.grad(loss, x, torch.ones(5, device=DEV))[0]
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
