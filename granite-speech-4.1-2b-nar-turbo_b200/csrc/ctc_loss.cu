@@ -31,7 +31,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // a state thousands of octaves below its frame's largest can still carry the whole posterior (a confident model and
 // another transcript), so neither fp32 with a scale a frame nor fp64 holds them; the logarithm in fp32 would lose
 // 2^-12 at -4000.  m lies within a few octaves of 1; a zero has e near kZeroExp, so that its terms vanish in any sum.
-//   bounds: a frame's emission is 2^-1020 at the least or impossible, kMaxCtcFrames of them reach -2^24;
+//   bounds: a frame's emission is 2^-15870 at the least or impossible, kMaxCtcFrames of them stay above -2^28;
 //   kZeroExp = -2^29, e is held at or above it, and no sum of three exponents leaves an int.
 constexpr int kZeroExp = -(1 << 29);
 constexpr int kZeroBelow = -(1 << 28);        // exponents below it are zeros
@@ -190,8 +190,28 @@ __device__ __forceinline__ void plan_utterance(const CtcArgs& a, int b) {
   }
 }
 
-// exp(a) as a stored word, for a <= 0; 0 (impossible) below kLowest and for NaN (the frame's sum tells of it)
+// exp(a) as a stored word, for a <= 0; 0 below kLowest and for NaN (the frame's sum tells of it)
 constexpr float kLowest = -690.f;
+// A frame with a class of the transcript below kLowest and not below kImpossible has words of 14 bits of exponent and 18
+// of mantissa, and its span is marked: beyond any block's kFastSpan, so the lattice comes upon it among its slow frames.
+constexpr float kImpossible = -11000.f;
+constexpr int kFarShift = 18, kFarBias = 15872;
+constexpr uint32_t kFarSpan = 1u << 16;
+__device__ __forceinline__ uint32_t far_emission_word(float logit, float best) {
+  const double d = (double)logit - (double)best, a = d * 1.4426950408889634, r = rint(a);
+  if (!(d >= (double)kImpossible)) return 0u;
+  return ((__float_as_uint(ex2_approx((float)(a - r))) + 16u) >> 5) + ((uint32_t)((int)r + kFarBias - 127) << kFarShift);
+}
+template <typename T>
+__device__ __noinline__ void write_far_emissions(const T* x, uint32_t* em, const int* targets, int len, int S, int blank,
+                                                 int V, float best, int lane) {
+  __syncwarp();                                    // behind the frame's other words
+  for (int i = lane; i <= len; i += 32) {
+    const int v = i < len ? __ldg(targets + i) : blank;
+    em[i < len ? i : S + 1] = v < 0 || v >= V ? 0u : far_emission_word(to_f32(x[v]), best);
+  }
+}
+
 __device__ __forceinline__ uint32_t emission_word(float a) {
   const float r = fmaf(a, kLog2e, 12582912.f);   // 1.5 * 2^23: the nearest integer of a / ln 2 in the low bits
   const float f = fmaf(a, kLog2e, 12582912.f - r);
@@ -200,7 +220,8 @@ __device__ __forceinline__ uint32_t emission_word(float a) {
 }
 
 // Emission words of F frames that follow one another (frame, x: of the first; count <= F of them are there): labels at
-// [0, len), a zero at S, the blank at S + 1, and at S + 2 how many octaves the least of them lies below the likeliest.
+// [0, len), a zero at S, the blank at S + 1, and at S + 2 how many octaves the least of them lies below the likeliest
+// (with kFarSpan where that takes the other words).
 // best[f]: the likeliest one's logit.  One warp; a label is looked up once for all its frames, and the first 32 KEEP
 // labels' logits stay in registers between the two passes.
 template <typename T, int F, int KEEP>
@@ -241,7 +262,7 @@ __device__ __forceinline__ void write_emissions(const CtcArgs& a, const T* x, in
     for (int f = 0; f < F; ++f) best[f] = fmaxf(best[f], __shfl_xor_sync(0xffffffffu, best[f], d));
   auto put = [&](int i, int f, float logit) {
     const float x = logit - best[f];
-    if (x >= kLowest) least[f] = fminf(least[f], x);
+    if (x >= kImpossible) least[f] = fminf(least[f], x);
     em[(int64_t)f * a.pitch + i] = emission_word(x);
   };
 #pragma unroll
@@ -265,7 +286,12 @@ __device__ __forceinline__ void write_emissions(const CtcArgs& a, const T* x, in
     for (int f = 0; f < F; ++f) least[f] = fminf(least[f], __shfl_xor_sync(0xffffffffu, least[f], d));
 #pragma unroll
   for (int f = 0; f < F; ++f)
-    if (lane == f && f < count) em[(int64_t)f * a.pitch + a.S + 2] = (uint32_t)(int)ceilf(-least[f] * kLog2e);
+    if (f < count) {
+      const bool far = least[f] < kLowest;
+      if (far) write_far_emissions<T>(x + f * a.ld_t, em + (int64_t)f * a.pitch, targets, len, a.S, a.blank, a.V, best[f], lane);
+      if (lane == f)
+        em[(int64_t)f * a.pitch + a.S + 2] = (uint32_t)(int)ceilf(-least[f] * kLog2e) | (far ? kFarSpan : 0u);
+    }
 }
 
 // what the frame adds to -log2 Z: its emissions are against `best` instead of the softmax's denominator
@@ -348,8 +374,9 @@ __host__ __device__ constexpr int lattice_warps(int pairs, int NP, int HL) {
 }
 
 // Four warps at most hold up to three pairs a lane; one more warp fetches the frames and adds up the blanks.
-// WIDE: every block on the exponents of its states, and every state stored with its own.  Otherwise true comes back, on
-// both sides, where the utterance has to be walked so for its posteriors: none is written yet, the loss is.
+// WIDE: every block on the exponents of its states, every state stored with its own, and frames of either emission words.
+// Otherwise true comes back, on both sides, where the utterance has to be walked so: no posterior is written yet, and the
+// loss where only the posteriors ask for it (again = 1), not the emissions (2).
 template <int NP, int H, int NBUF, bool GRAD, bool WIDE>
 __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
   constexpr int HL = halo_lanes<NP, H>(), NS = 2 * NP;
@@ -433,7 +460,8 @@ __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
 
   const int h = (n + 1) / 2, n1 = dir ? n - h : h;  // this side's frames before the meeting
   int issued = 0, waited = 0, blocks = 0, parity = 0;
-  bool fail = false, again = false;
+  bool fail = false;
+  int again = 0;
 
   // frames [k, k + cnt) of this side's order are rows lo, lo + 1, ...
   auto issue = [&](int k, int cnt, bool states) {
@@ -500,11 +528,24 @@ __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
       int pe[NS];
       fetch_below();
       gather(pm, pe);
+      if constexpr (WIDE) {
+        const bool far = em[a.S + 2] >= kFarSpan;
+        const int shift = far ? kFarShift : 20, bias = far ? kFarBias : 1023;
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const uint32_t x = em[s & 1 ? slot[s / 2] : a.S + 1];
-        m[s] = pm[s] * word_mantissa(x);
-        e[s] = max(pe[s] + (x < kWordOne ? kZeroExp : (int)(x >> 20) - 1023), kZeroExp);
+        for (int s = 0; s < NS; ++s) {
+          const uint32_t x = em[s & 1 ? slot[s / 2] : a.S + 1], field = x >> shift;
+          m[s] = pm[s] * __uint_as_float(((x << (23 - shift)) & 0x7FFFFFu) | 0x3F800000u);
+          e[s] = max(pe[s] + (field == 0 ? kZeroExp : (int)field - bias), kZeroExp);
+        }
+      } else {
+        if constexpr (!SECOND)
+          if (em[a.S + 2] >= kFarSpan) again = 2;  // this walk's numbers are void from here on
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          const uint32_t x = em[s & 1 ? slot[s / 2] : a.S + 1];
+          m[s] = pm[s] * word_mantissa(x);
+          e[s] = max(pe[s] + (x < kWordOne ? kZeroExp : (int)(x >> 20) - 1023), kZeroExp);
+        }
       }
       if constexpr (SECOND && WIDE) {
         auto joint = [&](int q, int s, float pm, int pe) {         // with state s (0 blank, 1 label) of the pair q
@@ -554,7 +595,8 @@ __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
 #pragma unroll
         for (int s = 1; s < NS; ++s) ref = max(ref, e[s]);
 #pragma unroll
-        for (int s = 0; s < NS; ++s) again |= own && e[s] >= kZeroBelow && e[s] < ref - kWordSpan;
+        for (int s = 0; s < NS; ++s)
+          if (own && e[s] >= kZeroBelow && e[s] < ref - kWordSpan) again = max(again, 1);
 #pragma unroll
         for (int j = 0; j < NP; ++j)
           if (j < blanks_here)
@@ -791,7 +833,7 @@ __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
       mine[2 * (i0 + j)] = make_float2(m[2 * j], __int_as_float(e[2 * j]));
       mine[2 * (i0 + j) + 1] = make_float2(m[2 * j + 1], __int_as_float(e[2 * j + 1]));
     }
-  if (again) a.again[b] = 1;                       // any lane's, either side's
+  if (again) atomicMax(a.again + b, again);        // any lane's, either side's
   // the states were stored by plain stores and are fetched by bulk copies of the other CTA
   asm volatile("fence.proxy.async;" ::: "memory");
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -800,7 +842,7 @@ __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
     drain();
     return false;
   }
-  if constexpr (!WIDE) again = __ldcg(a.again + b) != 0;
+  again = __ldcg(a.again + b);
   {
     int top = 2 * kZeroExp;
     float total = 0.f;
@@ -837,12 +879,13 @@ __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
       ze[w] = top;
     }
     __syncthreads();
+    if (!WIDE && again == 2) return true;
     top = ze[0];
     for (int i = 1; i < nw; ++i) top = max(top, ze[i]);
     total = 0.f;
     for (int i = 0; i < nw; ++i) total += zm[i] * pow2i(ze[i] - top);
     const bool exists = top > kZeroBelow;
-    if (!WIDE && dir == 0 && tid == 0) {
+    if ((!WIDE || again == 2) && dir == 0 && tid == 0) {
       norm = norms_sum;
       float raw = INFINITY;
       if (exists) raw = (float)((norm - (double)top - log2((double)total)) * 0.6931471805599453);

@@ -203,7 +203,7 @@ struct CtcArgs {
   float* loss = nullptr;         // [B] loss with zero_infinity applied
   int* bad = nullptr;            // workspace [B]: a length or label out of range
   float* norms = nullptr;        // workspace [B, T]: what each frame adds to -log2 Z
-  int* again = nullptr;          // workspace [B]: states too far apart for their words, to be walked again
+  int* again = nullptr;          // workspace [B]: states (1) or emissions (2) too far apart, to be walked again
   float2* exchange = nullptr;    // workspace [B, 2, 2, 2 pitch]: both sides' states where they meet, of either walk
   uint32_t* states = nullptr;    // workspace [B, T, state_pitch], or null: no posteriors wanted
   uint32_t* upper = nullptr;     // workspace [B, T, pitch] beside it: upper halves of the exponents of a second walk

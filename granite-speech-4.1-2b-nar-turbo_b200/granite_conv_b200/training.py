@@ -583,7 +583,9 @@ def ctc_loss(logits: torch.Tensor, targets: torch.Tensor, input_lengths: torch.T
              blank: int = 0, zero_infinity: bool = False) -> torch.Tensor:
     """CTC loss [B] (fp32, one value an utterance, no reduction) of logits [B, T, V], any strides with V innermost, for
     targets int [B, S] with input_lengths and target_lengths int [B]; the softmax is part of it.  Differentiable in the
-    logits.  An utterance without an alignment has the loss inf and a NaN gradient, or 0 and 0 with zero_infinity."""
+    logits.  An utterance without an alignment has the loss inf and a NaN gradient, or 0 and 0 with zero_infinity.  A
+    class of the transcript, the blank among them, counts as masked in a frame (impossible there, as with -inf) where its
+    logit lies more than 11000 below the largest of the transcript's classes; fp16's, bf16's and fp32's lowest values do."""
     if _dispatched(logits):
         return torch.ops.granite.ctc_loss(logits, targets, input_lengths, target_lengths, blank, zero_infinity)[0]
     if _recorded(logits):

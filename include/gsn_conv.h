@@ -402,7 +402,8 @@ int gsn_dropout_add_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* dh
  *   no alignment exists (0 with zero_infinity), NaN where a length lies outside [0, T] or [0, S], a label outside
  *   [0, V), or a valid frame holds NaN, +inf or nothing but -inf.  state: gsn_ctc_loss_state_bytes(B, T, S) bytes that
  *   the backward pass reads; it may be called after a forward pass with gradient != 0.  A class of the transcript, the
- *   blank among them, whose logit lies more than 690 below the largest of them counts as impossible in that frame.
+ *   blank among them, whose logit lies more than 11000 below the largest of them counts as masked: impossible in that
+ *   frame.
  *   workspace: gsn_ctc_loss_workspace_bytes(B, T, S, gradient) bytes.  Both 16-byte aligned.
  * gsn_ctc_loss_bwd: dlogits [B, T, V] dense, dloss[b] * d loss[b] / d logits; 0 in padding frames, for utterances
  *   without an alignment 0 with zero_infinity and NaN without, NaN for the others whose loss is NaN. */

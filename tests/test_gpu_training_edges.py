@@ -112,3 +112,39 @@ def test_ctc_utterances_far_apart_beside_others():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+# ---- CTC: emissions far apart ----------------------------------------------------------------------------------------
+def test_ctc_needed_class_far_below():
+    """A needed class far below the frame's likeliest has a finite loss by definition, no mask: one frame of 1000
+    against 0, single frames of thousands in an utterance, every frame of a long one, and the border at 11000."""
+    one = torch.tensor([[[1000.0, 0.0]]], device=DEV)
+    i = torch.ones(1, dtype=torch.int32, device=DEV)
+    assert tr.ctc_loss(one, i[None], i, i).item() == 1000.0
+    check_ctc(one, i[None], i, i)
+    check_ctc(one, i[None], i, i, zero_infinity=True)
+    g = np.random.default_rng(40)
+    for seed, T, V, S, share, gap in ((41, 40, 30, 9, 0.1, 900), (42, 90, 12, 30, 0.3, 5000), (43, 64, 8, 20, 1.0, 10900),
+                                      (44, 700, 40, 310, 0.05, 3000), (45, 1100, 40, 500, 0.02, 700)):
+        for dtype in (F32, BF, HF):
+            case = ctc_case(seed, 2, T, V, S, dtype, ([T, T - 7], [S, S // 2]))
+            at = torch.from_numpy(g.random((2, T, V)) < share).to(DEV)
+            low = torch.from_numpy(g.uniform(0.5, 1.0, (2, T, V)) * gap).to(DEV)
+            logits = (case[0].double() - torch.where(at, low, 0.0)).to(dtype)
+            check_ctc(logits, *case[1:])
+            check_ctc(logits, *case[1:], zero_infinity=True)
+    near, beyond = (torch.tensor([[[0.0, -v]]], device=DEV) for v in (10999.0, 11001.0))
+    assert tr.ctc_loss(near, i[None], i, i).item() == 10999.0
+    assert tr.ctc_loss(beyond, i[None], i, i).item() == math.inf
+
+
+def test_ctc_needed_class_far_below_over_the_longest_chain():
+    """Every frame of the longest utterance 10000 below: exponents of -2.3e8 in the states."""
+    T = tr.MAX_CTC_FRAMES
+    logits = torch.zeros(1, T, 3, device=DEV)
+    logits[:, :, 1:] = -10000.0
+    logits[:, :, 0] = -9000.0
+    logits[:, ::2, 0] = 0.0
+    logits[:, 1::2, 2] = 0.0                             # not of the transcript
+    targets = torch.ones(1, 5, dtype=torch.int32, device=DEV)
+    check_ctc(logits, targets, lens_of([T]), lens_of([5]))
