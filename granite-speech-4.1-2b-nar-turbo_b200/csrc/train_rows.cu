@@ -634,7 +634,8 @@ __global__ void __launch_bounds__(kRowThreads, NV < 4 ? 2 : 1) ln_bwd_kernel(Row
     sum[1] = q.x + q.y;
     row_sums(rg, sum);
     const float rstd = rsqrtf(fmaf(sum[0], inv_d, a.eps));
-    const float2 r2 = both(rstd), c1 = both(-rstd * mean_g), c2 = both(-rstd * rstd * rstd * (sum[1] * inv_d));
+    // rstd^3 alone would leave the range at spreads of 4e12 (and overflow for eps below 1e-26); rstd * S2 is of g's size
+    const float2 r2 = both(rstd), c1 = both(-rstd * mean_g), c2 = both(-rstd * (rstd * (rstd * (sum[1] * inv_d))));
     Kept<T, NV, VEC> kept;
     if (DROP && !a.drop_all) kept.draw(gen, (uint64_t)row * a.groups, base, lane, a.threshold << 16);
 #pragma unroll

@@ -7,7 +7,8 @@ import torch
 
 import train_ref as R
 from granite_conv_b200 import training as tr
-from test_gpu_training import BF, DEV, E, EPS, F32, HF, check_ctc, close, ctc_case, lens_of, rand, rng_of, rounded
+from test_gpu_training import (BF, DEV, E, EPS, F32, HF, check_ctc, close, ctc_case, grads_bound, lens_of, param_bounds,
+                               rand, rng_of, rounded)
 
 pytestmark = pytest.mark.gpu
 
@@ -148,3 +149,29 @@ def test_ctc_needed_class_far_below_over_the_longest_chain():
     logits[:, 1::2, 2] = 0.0                             # not of the transcript
     targets = torch.ones(1, 5, dtype=torch.int32, device=DEV)
     check_ctc(logits, targets, lens_of([T]), lens_of([5]))
+
+
+# ---- norms: spreads far from 1 ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("D", [40, 1001, 1024])
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("spread,eps", [(1e10, EPS), (1e13, EPS), (1e15, EPS), (1e17, EPS), (1e-14, 1e-30)])
+def test_layer_norm_gradient_at_far_spreads(spread, eps, dtype, D):
+    """Rows whose deviation is far from 1, up to where its square still fits fp32 and down to an eps of 1e-30: the
+    gradient is as near as at 1, and a constant row's is that of eps."""
+    x, dy = rand(50, (2, 5, D), dtype, spread), rand(51, (2, 5, D), dtype)
+    x[0, 1] = x[0, 1, 0]
+    w, b = rand(52, (D,), F32, 0.2, 1.0), rand(53, (D,), F32)
+    ref, rdw, rdb, r, xh = R.layer_norm_backward(dy, x, w, eps)
+    dx, dw, db = tr.layer_norm_backward(dy, x, w, eps)
+    even = [i for i in range(10) if i != 1]
+    # of the constant row the formula has r of eps alone, 1e15 here: x - m is exactly 0 in neither 64 bits nor fp32
+    bound = (grads_bound(dtype, ref, dy, x, w, r, None) - 1e-30 + torch.finfo(dtype).smallest_normal * 2.0 ** -8)
+    close(dx.view(10, D)[even], ref.view(10, D)[even], bound.view(10, D)[even], "dx")
+    assert torch.isfinite(dx).all()
+    fx, fres, fw, fb = tr.dropout_add_layer_norm_backward(dy, None, x, w, rng_of(), 0.0, eps=eps)
+    close(fres.view(10, D)[even], ref.view(10, D)[even], bound.view(10, D)[even], "dresidual")
+    assert torch.equal(fx, fres) and torch.equal(fw, dw) and torch.equal(fb, db)
+    bw, bb = param_bounds(F32, rdw, rdb, dy, x, r, xh, None)
+    if spread > 1:
+        close(dw, rdw, bw, "dw")
+    close(db, rdb, bb, "db")
