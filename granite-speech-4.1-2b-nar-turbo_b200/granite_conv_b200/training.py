@@ -184,18 +184,32 @@ def _(dy, x, weight, eps, lengths):
 
 
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
+_compiling = torch.compiler.is_compiling
+_tracing = torch._C._get_tracing_state
+_modes = torch._C._len_torch_dispatch_stack
+_early_modes = torch._ops._len_torch_dispatch_stack_pre_dispatch
 
 
 def _dispatched(*tensors: Optional[torch.Tensor]) -> bool:
-    """Whether a call has to go through the dispatcher: a graph being compiled, or a tensor subclass."""
-    return torch.compiler.is_compiling() or any(t is not None and type(t) not in _PLAIN for t in tensors)
+    """Whether a call has to go through the dispatcher: a graph being compiled or traced (whatever watches the ops that
+    are called would see an empty output and no kernel), another mode that takes them, or a tensor subclass."""
+    if _compiling() or _tracing() is not None or _modes() or _early_modes():
+        return True
+    for t in tensors:
+        if t is not None and type(t) not in _PLAIN:
+            return True
+    return False
 
 
 def _recorded(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether a call has a gradient to record.  It is then an autograd.Function around the direct launches: 95 to 127
     us of the CPU for a call and its gradient instead of 152 to 206 through the dispatcher's op (137 to 160 with
     setup_context as a function of its own; torch.func transforms, which want that, take neither form)."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 class _LayerNorm(torch.autograd.Function):

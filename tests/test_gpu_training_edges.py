@@ -175,3 +175,22 @@ def test_layer_norm_gradient_at_far_spreads(spread, eps, dtype, D):
     if spread > 1:
         close(dw, rdw, bw, "dw")
     close(db, rdb, bb, "db")
+
+
+# ---- tracers ---------------------------------------------------------------------------------------------------------
+def test_traced_calls_compute():
+    """make_fx and torch.jit.trace record the ops of every function, and their graphs compute on other inputs."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, y = (rand(s, (2, 5, 40), F32) for s in (60, 61))
+    w, b, rng = rand(62, (40,), F32, 0.2, 1.0), rand(63, (40,), F32), rng_of()
+    logits, targets, il, tl = ctc_case(64, 2, 9, 7, 3, F32)
+    other = rand(65, (2, 9, 7), F32)
+    rows = [lambda a: tr.layer_norm(a, w, b), lambda a: tr.layer_norm_backward(a, y, w)[0],
+            lambda a: tr.dropout_add(a, rng, 0.3, residual=y), lambda a: tr.dropout_add_backward(a, rng, 0.3),
+            lambda a: tr.dropout_add_layer_norm(a, y, w, b, rng, 0.3)[0],
+            lambda a: tr.dropout_add_layer_norm_backward(a, a, y, w, rng, 0.3)[1]]
+    for f, at, to in [(f, x, y) for f in rows] + [(lambda a: tr.ctc_loss(a, targets, il, tl), logits, other)]:
+        want = f(to)
+        graphs = [make_fx(f)(at), make_fx(f, pre_dispatch=True)(at), torch.jit.trace(f, at, check_trace=False)]
+        for g in graphs:
+            assert torch.equal(g(to), want)

@@ -177,3 +177,32 @@ def test_ctc_workspace_holds_every_lane_reference():
         frames = 1000
         states = lib.gsn_ctc_loss_workspace_bytes(1, frames, S, 1) - lib.gsn_ctc_loss_workspace_bytes(1, frames, S, 0)
         assert states >= frames * 4 * (2 * (S + 1) + 32 * nw), S
+
+
+# ---- who takes a call ------------------------------------------------------------------------------------------------
+def test_calls_under_a_tracer_go_through_the_dispatcher():
+    """A tracer or mode that watches ops has to see the op, not the empty output that the kernel would fill."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    x, seen = torch.randn(3), []
+
+    def f(a):
+        seen.append(training._dispatched(a))
+        return a * 1
+
+    f(x)
+    assert seen.pop() is False
+    with Mode():
+        f(x)
+    make_fx(f)(x)
+    make_fx(f, pre_dispatch=True)(x)
+    make_fx(f, tracing_mode="fake")(x)
+    torch.jit.trace(f, x, check_trace=False)
+    assert len(seen) == 5 and all(seen)
+    f(x)
+    assert seen.pop() is False
