@@ -13,9 +13,9 @@ directly.  Each is also a ``torch.library`` op, so ``torch.compile(fullgraph=Tru
   ``granite::ctc_loss_backward``
 
 Tensors are bf16, fp16 or fp32 on one CUDA device, parameters fp32 or of the activations' type; work runs on that
-device's current stream.  Results repeat bit for bit.  ``lengths`` (int [B], with x [B, T, D]) marks the frames
-t >= lengths[b] as padding: nothing of them is read, normed outputs and gradients there are zero, they join no weight
-gradient, and a residual passes through.
+device's current stream.  Results repeat bit for bit.  Tensors with a forward-mode tangent are refused.  ``lengths``
+(int [B], with x [B, T, D]) marks the frames t >= lengths[b] as padding: nothing of them is read, normed outputs and
+gradients there are zero, they join no weight gradient, and a residual passes through.
 
 ``rng`` is an int64 tensor of two on the device, (seed, offset), which the kernels read when they run: a captured graph
 draws new masks when it holds ``rng[1] += 1`` after its backward pass.  ``site`` tells apart the dropouts of one step.
@@ -26,6 +26,7 @@ import contextlib
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -62,6 +63,10 @@ def _int32(t: torch.Tensor) -> torch.Tensor:
 
 
 def _check_device(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    if forward_ad._current_level >= 0:             # inside a dual_level: a tangent would be lost without a word
+        for t in (first, *others):
+            if t is not None and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name}: no forward-mode derivative; use the backward pass")
     if not first.is_cuda:
         raise RuntimeError(f"{name}: every tensor must be on a CUDA device (got {first.device}); the kernels have no "
                            "CPU path")

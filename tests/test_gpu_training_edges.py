@@ -194,3 +194,15 @@ def test_traced_calls_compute():
         graphs = [make_fx(f)(at), make_fx(f, pre_dispatch=True)(at), torch.jit.trace(f, at, check_trace=False)]
         for g in graphs:
             assert torch.equal(g(to), want)
+
+
+def test_forward_mode_is_refused():
+    """Dual tensors are refused by the functions and by the ops behind them."""
+    from torch.autograd import forward_ad
+    x, w = rand(70, (2, 3, 16), F32), torch.ones(16, device=DEV)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, x)
+        for f in (tr.layer_norm, lambda *a: torch.ops.granite.layer_norm(*a, EPS)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f(dual, w, w)
+            assert torch.equal(f(x, w, w), tr.layer_norm(x, w, w))

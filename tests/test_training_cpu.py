@@ -206,3 +206,28 @@ def test_calls_under_a_tracer_go_through_the_dispatcher():
     assert len(seen) == 5 and all(seen)
     f(x)
     assert seen.pop() is False
+
+
+def test_functions_refuse_tangents():
+    """A forward-mode tangent is refused, by torch.func.jvp as by a dual tensor, not dropped."""
+    from torch.autograd import forward_ad
+    x, t = torch.randn(2, 3, 16), torch.ones(2, 3, 16)
+    w = torch.ones(16)
+    rng = torch.zeros(2, dtype=torch.int64)
+    i = torch.ones(2, dtype=torch.int32)
+    lab = torch.zeros(2, 4, dtype=torch.int32)
+    calls = [lambda a: training.layer_norm(a, w, w), lambda a: training.layer_norm(x, a[0, 0], w),
+             lambda a: training.layer_norm_backward(x, a, w), lambda a: training.dropout_add(x, rng, 0.1, residual=a),
+             lambda a: training.dropout_add_backward(a, rng, 0.1),
+             lambda a: training.dropout_add_layer_norm(x, a, w, w, rng, 0.1),
+             lambda a: training.dropout_add_layer_norm_backward(x, a, x, w, rng, 0.1),
+             lambda a: training.ctc_loss(a, lab, i, i)]
+    for f in calls:
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(f, (x,), (t,))
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(x, t)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f(dual)
+            with pytest.raises(RuntimeError, match="CUDA device"):     # other tensors of a dual level are welcome
+                f(x)
