@@ -16,7 +16,7 @@ int check_rows(const char* name, int64_t M, int D, int dtype, const int32_t* len
   if (M > 0x7fffffffLL) return fail(GSN_ERR_UNSUPPORTED, "%s: M=%lld rows, at most 2^31 - 1", name, (long long)M);
   if (dtype != GSN_BF16 && dtype != GSN_FP16 && dtype != GSN_FP32)
     return fail(GSN_ERR_UNSUPPORTED, "%s: dtype %d is none of bf16, fp16, fp32", name, dtype);
-  if (lengths && (T <= 0 || M % T != 0))
+  if (lengths && M > 0 && (T <= 0 || M % T != 0))
     return fail(GSN_ERR_UNSUPPORTED, "%s: with lengths, T=%d must divide M=%lld", name, T, (long long)M);
   return M == 0 ? -1 : 0;
 }

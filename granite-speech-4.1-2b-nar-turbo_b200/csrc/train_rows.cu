@@ -924,7 +924,7 @@ int launch_dropout(const RowArgs& a, bool vec, cudaStream_t stream) {
 template <typename T>
 int launch_typed(RowArgs a, int op, cudaStream_t stream) {
   const bool vec = vec_ok(a, sizeof(T));
-  if (a.lengths) {                                 // row / T = (umulhi(factor, row) + row) >> shift
+  if (a.lengths && a.M > 0) {                      // row / T = (umulhi(factor, row) + row) >> shift
     while (((uint64_t)1 << a.div_shift) < (uint64_t)a.T) ++a.div_shift;
     a.div_factor = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << a.div_shift) - a.T)) / a.T + 1);
   }
@@ -938,7 +938,7 @@ int launch_typed(RowArgs a, int op, cudaStream_t stream) {
   }
   if (bwd) {
     return launch_behind(ln_param_grad_kernel<T>, dim3((2 * a.D + 31) / 32), 1024, 0, stream, a.partials,
-                         (int)a.partial_rows, a.D, a.dweight, a.dbias, a.param_fp32);
+                         (int)a.partial_rows, a.D, a.dweight, a.dbias, a.param_fp32);     // zeros where there are no rows
   }
   return 0;
 }

@@ -349,10 +349,11 @@ int gsn_bpe_head_ctc_bf16(const void* pooled, const int32_t* pooled_lengths, con
 /* ---- fine-tuning: LayerNorm with its backward pass, dropout with a residual ------------------------------------
  * No counterpart in the reference, which only runs inference; the formulas are those of the block's norms
  * (models/granite_speech_nar/conformer.py:199, :209) and residual steps (:205-208).  Rows of D elements of `dtype`,
- * M of them (M < 2^31; with lengths, M / T utterances of T frames); inputs have row strides in elements, outputs are
- * dense and do not overlap inputs.  Rows aligned to 16 bytes with D % 8 == 0 move in 16-byte words, others element by
- * element.  weight, bias and their gradients are of `param_dtype`: GSN_FP32 or dtype.  D <= 8192 where a norm is
- * formed.  All arithmetic is fp32 and no sum depends on the order of arrival: results repeat bit for bit.
+ * M of them (M < 2^31; with lengths, M / T utterances of T frames, T of any value where M is 0); inputs have row
+ * strides in elements, outputs are dense and do not overlap inputs.  Rows aligned to 16 bytes with D % 8 == 0 move in
+ * 16-byte words, others element by element.  weight, bias and their gradients are of `param_dtype`: GSN_FP32 or dtype.
+ * D <= 8192 where a norm is formed.  All arithmetic is fp32 and no sum depends on the order of arrival: results repeat
+ * bit for bit.
  * Padding frames (t >= lengths[b]): x, h and dy are not read, y and dx are 0, nothing joins dweight and dbias, and
  * the residual path passes (h = residual, dresidual = dh; without a residual, out = 0).
  *

@@ -206,3 +206,21 @@ def test_forward_mode_is_refused():
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 f(dual, w, w)
             assert torch.equal(f(x, w, w), tr.layer_norm(x, w, w))
+
+
+# ---- empty batches ---------------------------------------------------------------------------------------------------
+def test_batches_without_frames_take_lengths():
+    w, rng = torch.ones(32, device=DEV), rng_of()
+    for shape, lengths in (((3, 0, 32), [0, 0, 0]), ((0, 5, 32), []), ((0, 0, 32), [])):
+        x, lens = torch.empty(shape, dtype=BF, device=DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV)
+        assert tr.layer_norm(x, w, w, lengths=lens).shape == shape
+        dx, dw, db = tr.layer_norm_backward(x, x, w, lengths=lens)
+        assert dx.shape == shape and not dw.any() and not db.any()
+        assert tr.dropout_add(x, rng, 0.1, residual=x, lengths=lens).shape == shape
+        y, h = tr.dropout_add_layer_norm(x, x, w, w, rng, 0.1, lengths=lens)
+        assert y.shape == h.shape == shape
+        dx, dres, dw, db = tr.dropout_add_layer_norm_backward(x, x, x, w, rng, 0.1, lengths=lens)
+        assert dres.shape == shape and not dw.any() and not db.any()
+        leaf = x.clone().requires_grad_()
+        tr.layer_norm(leaf, w, w, lengths=lens).sum().backward()
+        assert leaf.grad.shape == shape

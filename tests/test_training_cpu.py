@@ -231,3 +231,14 @@ def test_functions_refuse_tangents():
                 f(dual)
             with pytest.raises(RuntimeError, match="CUDA device"):     # other tensors of a dual level are welcome
                 f(x)
+
+
+def test_batches_without_frames_take_lengths():
+    """M = 0 with lengths, T = 0 among them, is a call with nothing to do and no error (the backward passes, which write
+    dweight and dbias, are launches: on the GPU)."""
+    L = _lib.lib()
+    for T in (0, 3):
+        assert L.gsn_layer_norm_fwd(P, 64, P, P, P, 0, 64, 1e-5, 0, 2, P, T, None) == 0
+        assert L.gsn_dropout_add(P, 64, P, 64, P, 0, 64, 0, P, 0, 0.1, 1.0, P, T, None) == 0
+        assert L.gsn_dropout_add_layer_norm_fwd(P, 64, P, 64, P, P, P, P, 0, 64, 1e-5, 0, 2, P, 0, 0.1, 1.0, P, T, None) == 0
+    assert L.gsn_layer_norm_fwd(P, 64, P, P, P, 4, 64, 1e-5, 0, 2, P, 0, None) == 2
