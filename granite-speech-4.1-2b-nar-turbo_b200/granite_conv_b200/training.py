@@ -142,9 +142,12 @@ def _layer_norm(x, weight, bias, eps, lengths):
     with _on(x.device):
         xr, ld = _rows(x)
         w, b = weight.contiguous(), bias.contiguous()
-        if (lens is None and x.dtype == w.dtype == torch.bfloat16 and D in INFERENCE_WIDTHS and ld % 8 == 0
-                and not (xr.data_ptr() | w.data_ptr() | b.data_ptr()) & 15):
-            # what the inference path's norm takes keeps its kernel, and its bits
+        if (lens is None and x.dtype == w.dtype == torch.bfloat16 and D in INFERENCE_WIDTHS
+                and not (w.data_ptr() | b.data_ptr()) & 15
+                and (not x.is_contiguous() or not xr.data_ptr() & 15)):
+            # what the inference path's norm takes keeps its kernel, and its bits: views off its 16-byte grid as a copy
+            if ld % 8 or xr.data_ptr() & 15:
+                xr, ld = x.contiguous(), D
             _lib.call("gsn_layernorm_bf16", xr.data_ptr(), ld, w.data_ptr(), b.data_ptr(), y.data_ptr(), D,
                       y.numel() // D, D, eps, None, 0, _stream(x.device))
             return y

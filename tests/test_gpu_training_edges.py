@@ -224,3 +224,17 @@ def test_batches_without_frames_take_lengths():
         leaf = x.clone().requires_grad_()
         tr.layer_norm(leaf, w, w, lengths=lens).sum().backward()
         assert leaf.grad.shape == shape
+
+
+# ---- what ran before -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("D", [256, 512, 1024, 2048])
+def test_views_keep_the_inference_kernel(D):
+    """Views of bf16 rows, off the 16-byte grid among them, have the inference kernel's bits."""
+    from granite_conv_b200 import ops
+    wide = rand(80, (64, 2 * D + 8), BF, 1.3, 0.7)
+    w, b = rand(81, (D,), BF, 0.1, 1.0), rand(82, (D,), BF)
+    for x in (wide[:, 3:3 + D], wide[:, 8:8 + D], wide[::2, :D], wide[1:3, 5:5 + D],
+              wide[:, 1:1 + D].t().contiguous().t(), wide.view(8, 8, -1)[:, 1:4, 7:7 + D]):
+        want = ops.layernorm(x.contiguous().view(-1, D), w, b, EPS).view(x.shape)
+        assert torch.equal(torch.ops.granite.layer_norm(x, w, b, EPS), want)
+        assert torch.equal(tr.layer_norm(x, w, b, EPS), want)
