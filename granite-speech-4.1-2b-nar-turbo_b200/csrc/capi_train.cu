@@ -14,6 +14,7 @@ int type_size(int dtype) { return dtype == GSN_FP32 ? 4 : 2; }
 int check_rows(const char* name, int64_t M, int D, int dtype, const int32_t* lengths, int T) {
   if (M < 0 || D <= 0) return fail(GSN_ERR_INVALID_ARG, "%s: bad sizes M=%lld D=%d", name, (long long)M, D);
   if (M > 0x7fffffffLL) return fail(GSN_ERR_UNSUPPORTED, "%s: M=%lld rows, at most 2^31 - 1", name, (long long)M);
+  if (D > kMaxRowElements) return fail(GSN_ERR_UNSUPPORTED, "%s: D=%d, at most %d", name, D, kMaxRowElements);
   if (dtype != GSN_BF16 && dtype != GSN_FP16 && dtype != GSN_FP32)
     return fail(GSN_ERR_UNSUPPORTED, "%s: dtype %d is none of bf16, fp16, fp32", name, dtype);
   if (lengths && M > 0 && (T <= 0 || M % T != 0))
@@ -91,6 +92,7 @@ int check_ctc(const char* name, int B, int T, int V, int S, int64_t ld_b, int64_
   if (dtype != GSN_BF16 && dtype != GSN_FP16 && dtype != GSN_FP32)
     return fail(GSN_ERR_UNSUPPORTED, "%s: dtype %d is none of bf16, fp16, fp32", name, dtype);
   if (blank < 0 || blank >= V) return fail(GSN_ERR_INVALID_ARG, "%s: blank=%d outside the %d classes", name, blank, V);
+  if (V > kMaxCtcClasses) return fail(GSN_ERR_UNSUPPORTED, "%s: V=%d classes, at most %d", name, V, kMaxCtcClasses);
   if (S > kMaxCtcLabels) return fail(GSN_ERR_UNSUPPORTED, "%s: S=%d labels, at most %d", name, S, kMaxCtcLabels);
   if (T > kMaxCtcFrames) return fail(GSN_ERR_UNSUPPORTED, "%s: T=%d frames, at most %d", name, T, kMaxCtcFrames);
   if (B * (int64_t)T > 0 && (ld_t < V || ld_b < 0))

@@ -151,7 +151,8 @@ int launch_ctc_collapse(const unsigned long long* keys, const int* plen, int* id
 //   kRowNormGrad      x, dy, weight -> dx, dweight, dbias
 //   kRowDropNormGrad  x (the stored h), dy, dh (or null), weight -> dx, dres, dweight, dbias
 enum RowOp { kRowNorm = 0, kRowDropout = 1, kRowDropNorm = 2, kRowNormGrad = 3, kRowDropNormGrad = 4 };
-constexpr int kMaxRowWidth = 8192;
+constexpr int kMaxRowWidth = 8192;              // where a norm is formed
+constexpr int kMaxRowElements = 0x7fffff00;     // a block of 256 columns past the end is still an int
 struct RowArgs {
   const void* x = nullptr;
   const void* dy = nullptr;
@@ -186,6 +187,7 @@ int launch_row_op(const RowArgs& args, int op, int dtype, cudaStream_t stream);
 // ---- CTC loss and its gradient (ctc_loss.cu) ---------------------------------------------------------------------
 constexpr int kMaxCtcLabels = 2000;
 constexpr int kMaxCtcFrames = 16384;
+constexpr int kMaxCtcClasses = 0x7ffffc00;      // a CTA's stride past the end is still an int
 struct CtcArgs {
   const void* logits = nullptr;  // [B, T, V], strides ld_b, ld_t, 1
   int64_t ld_b = 0, ld_t = 0;

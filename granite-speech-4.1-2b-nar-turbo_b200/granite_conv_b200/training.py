@@ -33,9 +33,11 @@ from . import _lib
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _HERE = contextlib.nullcontext()
 MAX_NORM_WIDTH = 8192
+MAX_ROW_ELEMENTS = 2 ** 31 - 256
 INFERENCE_WIDTHS = (256, 512, 1024, 2048)       # of gsn_layernorm_bf16
 MAX_CTC_LABELS = 2000
 MAX_CTC_FRAMES = 16384
+MAX_CTC_CLASSES = 2 ** 31 - 1024
 
 
 def _on(device: torch.device):
@@ -76,8 +78,8 @@ def _check_device(name: str, first: torch.Tensor, *others: Optional[torch.Tensor
 
 
 def _check_rows(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-    if first.dim() < 1 or first.shape[-1] == 0:
-        raise RuntimeError(f"{name}: rows of at least one element expected, got {tuple(first.shape)}")
+    if first.dim() < 1 or not 0 < first.shape[-1] <= MAX_ROW_ELEMENTS:
+        raise RuntimeError(f"{name}: rows of 1 to {MAX_ROW_ELEMENTS} elements expected, got {tuple(first.shape)}")
     if first.dtype not in _TYPES:
         raise RuntimeError(f"{name}: bf16, fp16 or fp32 tensors expected, got {first.dtype}")
     for t in others:
@@ -482,6 +484,8 @@ def _ctc_check(name, logits, targets, input_lengths, target_lengths, blank):
     for t in (input_lengths, target_lengths):
         if t.shape != (B,) or t.dtype not in ints:
             raise RuntimeError(f"{name}: lengths must be int [{B}], got {t.dtype} {tuple(t.shape)}")
+    if B >= 2 ** 31 or V > MAX_CTC_CLASSES:
+        raise RuntimeError(f"{name}: {B} utterances of {V} classes, at most 2^31 - 1 and {MAX_CTC_CLASSES}")
     if not 0 <= blank < V:
         raise RuntimeError(f"{name}: blank={blank} outside the {V} classes")
     if targets.shape[1] > MAX_CTC_LABELS or T > MAX_CTC_FRAMES:

@@ -352,7 +352,7 @@ int gsn_bpe_head_ctc_bf16(const void* pooled, const int32_t* pooled_lengths, con
  * M of them (M < 2^31; with lengths, M / T utterances of T frames, T of any value where M is 0); inputs have row
  * strides in elements, outputs are dense and do not overlap inputs.  Rows aligned to 16 bytes with D % 8 == 0 move in
  * 16-byte words, others element by element.  weight, bias and their gradients are of `param_dtype`: GSN_FP32 or dtype.
- * D <= 8192 where a norm is formed.  All arithmetic is fp32 and no sum depends on the order of arrival: results repeat
+ * D <= 8192 where a norm is formed, else 2^31 - 256.  All arithmetic is fp32 and no sum depends on the order of arrival: results repeat
  * bit for bit.
  * Padding frames (t >= lengths[b]): x, h and dy are not read, y and dx are 0, nothing joins dweight and dbias, and
  * the residual path passes (h = residual, dresidual = dh; without a residual, out = 0).
@@ -398,7 +398,7 @@ int gsn_dropout_add_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* dh
 /* ---- CTC loss with its gradient ---------------------------------------------------------------------------------
  * No counterpart in the reference (inference only): the loss that its CTC heads (conformer.py:240-252) are trained
  * with, from logits [B, T, V] of `dtype` with strides ld_b, ld_t, 1.  targets int32 [B, S], input_lengths and
- * target_lengths int32 [B] on the device; S <= 2000, T <= 16384.
+ * target_lengths int32 [B] on the device; S <= 2000, T <= 16384, V <= 2^31 - 1024.
  * gsn_ctc_loss_fwd: loss[b] = -log p(targets[b, :target_lengths[b]] | softmax(logits[b, :input_lengths[b]])), inf where
  *   no alignment exists (0 with zero_infinity), NaN where a length lies outside [0, T] or [0, S], a label outside
  *   [0, V), or a valid frame holds NaN, +inf or nothing but -inf.  state: gsn_ctc_loss_state_bytes(B, T, S) bytes that

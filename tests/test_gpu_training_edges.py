@@ -238,3 +238,15 @@ def test_views_keep_the_inference_kernel(D):
         want = ops.layernorm(x.contiguous().view(-1, D), w, b, EPS).view(x.shape)
         assert torch.equal(torch.ops.granite.layer_norm(x, w, b, EPS), want)
         assert torch.equal(tr.layer_norm(x, w, b, EPS), want)
+
+
+# ---- sizes that an int does not hold ---------------------------------------------------------------------------------
+def test_sizes_past_32_bits_are_refused():
+    """Refused before anything is allocated: the tensors are one element, expanded."""
+    one, i = torch.zeros(1, dtype=BF, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    with pytest.raises(RuntimeError, match="elements expected"):
+        tr.dropout_add(one.expand(2 ** 32 + 5), rng_of(), 0.1)
+    with pytest.raises(RuntimeError, match="classes"):
+        tr.ctc_loss(one.expand(1, 1, 2 ** 32 + 5), i[None], i, i)
+    with pytest.raises(RuntimeError, match="utterances"):
+        tr.ctc_loss(one.expand(2 ** 32 + 1, 0, 5), i.expand(2 ** 32 + 1, 0), i.expand(2 ** 32 + 1), i.expand(2 ** 32 + 1))

@@ -242,3 +242,17 @@ def test_batches_without_frames_take_lengths():
         assert L.gsn_dropout_add(P, 64, P, 64, P, 0, 64, 0, P, 0, 0.1, 1.0, P, T, None) == 0
         assert L.gsn_dropout_add_layer_norm_fwd(P, 64, P, 64, P, P, P, P, 0, 64, 1e-5, 0, 2, P, 0, 0.1, 1.0, P, T, None) == 0
     assert L.gsn_layer_norm_fwd(P, 64, P, P, P, 4, 64, 1e-5, 0, 2, P, 0, None) == 2
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Widths, classes and utterances that an int does not hold must not come down to their low halves."""
+    L = _lib.lib()
+    wide = 2 ** 31 - 255
+    assert L.gsn_dropout_add(P, wide, None, 0, P, 1, wide, 0, P, 0, 0.1, 1.0, None, 0, None) == 2
+    assert "at most" in _lib.last_error()
+    big = 2 ** 31 - 1023
+    assert L.gsn_ctc_loss_fwd(P, big, big, P, P, P, 1, 1, big, 1, 0, 0, 0, 0, P, P, 1 << 20, P, 1 << 20, None) == 2
+    one = torch.zeros(1)
+    with pytest.raises(RuntimeError, match="elements expected"):
+        training._check_rows("rows", one.expand(2 ** 32 + 5))
+    training._check_rows("rows", one.expand(2 ** 31 - 256))
