@@ -128,12 +128,43 @@ int set_state(const char* name, CtcArgs& a, void* state, size_t bytes) {
   char* p = static_cast<char*>(state);
   a.raw_loss = (float*)p;
   p += align256(a.B * sizeof(float));
+  a.again = (int*)p;
+  p += align256(a.B * sizeof(int));
   a.stats = (float2*)p;
   p += align256((size_t)a.B * a.T * sizeof(float2));
   a.order = (int2*)p;
   p += align256((size_t)a.B * a.pitch * sizeof(int2));
   a.post = (float*)p;
   return 0;
+}
+
+// gsn_ctc_loss_fwd, or with a copy withheld for the self-test
+int ctc_loss_fwd(const char* name, const void* logits, int64_t ld_b, int64_t ld_t, const int32_t* targets,
+                 const int32_t* input_lengths, const int32_t* target_lengths, int B, int T, int V, int S, int blank,
+                 int zero_infinity, int gradient, int dtype, float* loss, void* state, size_t state_bytes, void* workspace,
+                 size_t workspace_bytes, int withhold, gsn_stream_t stream) {
+  if (int rc = check_ctc(name, B, T, V, S, ld_b, ld_t, blank, dtype)) return rc < 0 ? ok() : rc;
+  if (!input_lengths || !target_lengths || !loss || (S > 0 && !targets) || (T > 0 && !logits))
+    return fail(GSN_ERR_INVALID_ARG, "%s: null pointer", name);
+  if (!aligned(logits, type_size(dtype))) return fail(GSN_ERR_UNSUPPORTED, "%s: logits are not aligned to their type", name);
+  CtcArgs a = ctc_args(logits, ld_b, ld_t, targets, input_lengths, target_lengths, B, T, V, S, blank, zero_infinity);
+  if (int rc = set_state(name, a, state, state_bytes)) return rc;
+  const size_t need = gsn_ctc_loss_workspace_bytes(B, T, S, gradient);
+  if (workspace_bytes < need) return fail(GSN_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", name, workspace_bytes, need);
+  if (!workspace || !aligned(workspace, 16)) return fail(GSN_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", name);
+  a.loss = loss;
+  a.withhold = withhold;
+  char* ws = static_cast<char*>(workspace);
+  a.bad = (int*)ws;
+  ws += align256((size_t)B * sizeof(int));
+  a.norms = (float*)ws;
+  ws += align256((size_t)B * T * sizeof(float));
+  a.exchange = (float2*)ws;
+  if (gradient) {
+    a.states = (uint32_t*)(ws + align256((size_t)B * 8 * a.pitch * sizeof(float2)));
+    a.upper = a.states + (size_t)B * T * a.state_pitch;
+  }
+  return finish(launch_ctc_loss(a, dtype, (cudaStream_t)stream), name);
 }
 
 }  // namespace
@@ -271,13 +302,13 @@ int gsn_dropout_add_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* dh
 size_t gsn_ctc_loss_state_bytes(int B, int T, int S) {
   if (B <= 0 || T < 0 || S < 0 || S > kMaxCtcLabels) return 0;
   const size_t frames = (size_t)B * T, pitch = ctc_pitch(S);
-  return align256(B * sizeof(float)) + align256(frames * sizeof(float2)) + align256(B * pitch * sizeof(int2)) +
+  return align256(B * sizeof(float)) + align256(B * sizeof(int)) + align256(frames * sizeof(float2)) + align256(B * pitch * sizeof(int2)) +
          align256(frames * pitch * sizeof(float));
 }
 
 size_t gsn_ctc_loss_workspace_bytes(int B, int T, int S, int gradient) {
   if (B <= 0 || T < 0 || S < 0 || S > kMaxCtcLabels) return 0;
-  size_t n = 2 * align256((size_t)B * sizeof(int)) + align256((size_t)B * T * sizeof(float)) +
+  size_t n = align256((size_t)B * sizeof(int)) + align256((size_t)B * T * sizeof(float)) +
              align256((size_t)B * 8 * ctc_pitch(S) * sizeof(float2));
   if (gradient) n += (size_t)B * T * (ctc_state_pitch(S) + ctc_pitch(S)) * sizeof(uint32_t);
   return n;
@@ -287,30 +318,19 @@ int gsn_ctc_loss_fwd(const void* logits, int64_t ld_b, int64_t ld_t, const int32
                      const int32_t* input_lengths, const int32_t* target_lengths, int B, int T, int V, int S, int blank,
                      int zero_infinity, int gradient, int dtype, float* loss, void* state, size_t state_bytes,
                      void* workspace, size_t workspace_bytes, gsn_stream_t stream) {
-  const char* name = "gsn_ctc_loss_fwd";
-  if (int rc = check_ctc(name, B, T, V, S, ld_b, ld_t, blank, dtype)) return rc < 0 ? ok() : rc;
-  if (!input_lengths || !target_lengths || !loss || (S > 0 && !targets) || (T > 0 && !logits))
-    return fail(GSN_ERR_INVALID_ARG, "%s: null pointer", name);
-  if (!aligned(logits, type_size(dtype))) return fail(GSN_ERR_UNSUPPORTED, "%s: logits are not aligned to their type", name);
-  CtcArgs a = ctc_args(logits, ld_b, ld_t, targets, input_lengths, target_lengths, B, T, V, S, blank, zero_infinity);
-  if (int rc = set_state(name, a, state, state_bytes)) return rc;
-  const size_t need = gsn_ctc_loss_workspace_bytes(B, T, S, gradient);
-  if (workspace_bytes < need) return fail(GSN_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", name, workspace_bytes, need);
-  if (!workspace || !aligned(workspace, 16)) return fail(GSN_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", name);
-  a.loss = loss;
-  char* ws = static_cast<char*>(workspace);
-  a.bad = (int*)ws;
-  ws += align256((size_t)B * sizeof(int));
-  a.again = (int*)ws;
-  ws += align256((size_t)B * sizeof(int));
-  a.norms = (float*)ws;
-  ws += align256((size_t)B * T * sizeof(float));
-  a.exchange = (float2*)ws;
-  if (gradient) {
-    a.states = (uint32_t*)(ws + align256((size_t)B * 8 * a.pitch * sizeof(float2)));
-    a.upper = a.states + (size_t)B * T * a.state_pitch;
-  }
-  return finish(launch_ctc_loss(a, dtype, (cudaStream_t)stream), name);
+  return ctc_loss_fwd("gsn_ctc_loss_fwd", logits, ld_b, ld_t, targets, input_lengths, target_lengths, B, T, V, S, blank,
+                      zero_infinity, gradient, dtype, loss, state, state_bytes, workspace, workspace_bytes, 0, stream);
+}
+
+int gsn_selftest_ctc_withheld(const void* logits, int64_t ld_b, int64_t ld_t, const int32_t* targets,
+                              const int32_t* input_lengths, const int32_t* target_lengths, int B, int T, int V, int S,
+                              int blank, int dtype, float* loss, void* state, size_t state_bytes, void* workspace,
+                              size_t workspace_bytes, int side, int half, gsn_stream_t stream) {
+  const char* name = "gsn_selftest_ctc_withheld";
+  if (side < 0 || side > 1 || half < 0 || half > 1) return fail(GSN_ERR_INVALID_ARG, "%s: side=%d half=%d", name, side, half);
+  if (S > kMaxCtcHeldLabels) return fail(GSN_ERR_UNSUPPORTED, "%s: S=%d labels, at most %d", name, S, kMaxCtcHeldLabels);
+  return ctc_loss_fwd(name, logits, ld_b, ld_t, targets, input_lengths, target_lengths, B, T, V, S, blank, 0, 1, dtype,
+                      loss, state, state_bytes, workspace, workspace_bytes, 1 + side + 2 * half, stream);
 }
 
 int gsn_ctc_loss_bwd(const float* dloss, const void* logits, int64_t ld_b, int64_t ld_t, const int32_t* targets,

@@ -187,6 +187,7 @@ __device__ __forceinline__ void plan_utterance(const CtcArgs& a, int b) {
   if (threadIdx.x == 0) {
     a.bad[b] = bad;
     a.again[b] = 0;
+    a.raw_loss[b] = a.loss[b] = NAN;               // what stays where a wait of the lattice runs out
   }
 }
 
@@ -376,8 +377,9 @@ __host__ __device__ constexpr int lattice_warps(int pairs, int NP, int HL) {
 // Four warps at most hold up to three pairs a lane; one more warp fetches the frames and adds up the blanks.
 // WIDE: every block on the exponents of its states, every state stored with its own, and frames of either emission words.
 // Otherwise true comes back, on both sides, where the utterance has to be walked so: no posterior is written yet, and the
-// loss where only the posteriors ask for it (again = 1), not the emissions (2).
-template <int NP, int H, int NBUF, bool GRAD, bool WIDE>
+// loss where only the posteriors ask for it (again = 1), not the emissions (2).  3 stands for a wait that has run out.
+// HOLD: the self-test's, which leaves a copy out.
+template <int NP, int H, int NBUF, bool GRAD, bool WIDE, bool HOLD>
 __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
   constexpr int HL = halo_lanes<NP, H>(), NS = 2 * NP;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -468,7 +470,8 @@ __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
     const int lo = dir ? n - k - cnt : k, buf = issued % NBUF;
     const uint32_t be = cnt * pitch * 4, bs = states ? cnt * spitch * 4 : 0;
     mbar_arrive_expect_tx(&full[buf], be + bs);
-    bulk_load(em_ring + buf * H * pitch, a.post + (frame0 + lo) * pitch, be, &full[buf]);
+    if (!HOLD || b > 0 || k > (states ? n1 : 0) || a.withhold != 1 + dir + 2 * states)
+      bulk_load(em_ring + buf * H * pitch, a.post + (frame0 + lo) * pitch, be, &full[buf]);
     if (states) bulk_load(st_ring + buf * H * spitch, a.states + (frame0 + lo) * spitch, bs, &full[buf]);
     ++issued;
   };
@@ -833,6 +836,7 @@ __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
       mine[2 * (i0 + j)] = make_float2(m[2 * j], __int_as_float(e[2 * j]));
       mine[2 * (i0 + j) + 1] = make_float2(m[2 * j + 1], __int_as_float(e[2 * j + 1]));
     }
+  if (fail) again = 3;
   if (again) atomicMax(a.again + b, again);        // any lane's, either side's
   // the states were stored by plain stores and are fetched by bulk copies of the other CTA
   asm volatile("fence.proxy.async;" ::: "memory");
@@ -879,7 +883,7 @@ __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
       ze[w] = top;
     }
     __syncthreads();
-    if (!WIDE && again == 2) return true;
+    if (again >= (WIDE ? 3 : 2)) return !WIDE;
     top = ze[0];
     for (int i = 1; i < nw; ++i) top = max(top, ze[i]);
     total = 0.f;
@@ -901,22 +905,28 @@ __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
   }
   if constexpr (GRAD) {
     walk(n1, n, std::true_type{});
-    if (fail) drain();
+    if (fail) {                                    // the gradient kernel makes NaN of the posteriors that are not there
+      uint32_t here;                               // b: kept to this place in a register, it cost the walk 30 us of 306
+      asm volatile("mov.u32 %0, %%ctaid.y;" : "=r"(here));
+      a.again[here] = 3;
+      drain();
+    }
   }
   return false;
 }
 
 // a function of its own: its code beside the other walk's took a fifth of that one's speed
-template <int NP, int H, int NBUF, bool GRAD>
+template <int NP, int H, int NBUF, bool GRAD, bool HOLD>
 __device__ __noinline__ void lattice_wide(const CtcArgs& a, int nw) {
+  if (__ldcg(a.again + blockIdx.y) == 3) return;   // the other side has given up
   __syncthreads();                                 // the first walk's shared memory is free
-  lattice_walk<NP, H, NBUF, GRAD, true>(a, nw);
+  lattice_walk<NP, H, NBUF, GRAD, true, HOLD>(a, nw);
 }
 
-template <int NP, int H, int NBUF, bool GRAD>
+template <int NP, int H, int NBUF, bool GRAD, bool HOLD>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NP < 4 ? 160 : H == 8 ? 288 : 576)
     ctc_lattice_kernel(const __grid_constant__ CtcArgs a, int nw) {
-  if (lattice_walk<NP, H, NBUF, GRAD, false>(a, nw)) lattice_wide<NP, H, NBUF, GRAD>(a, nw);
+  if (lattice_walk<NP, H, NBUF, GRAD, false, HOLD>(a, nw)) lattice_wide<NP, H, NBUF, GRAD, HOLD>(a, nw);
 }
 
 // ---- gradient --------------------------------------------------------------------------------------------------------
@@ -1029,9 +1039,9 @@ __global__ void __launch_bounds__(WARP_ROW ? kRowThreads : kCtaThreads) ctc_grad
   T* g = static_cast<T*>(a.dlogits) + frame * a.V;
   const int n = __ldg(a.input_lengths + b);
   const float raw = __ldg(a.raw_loss + b);
-  // frames of the utterance: a gradient where there is a finite loss, else zeros or NaN; behind it zeros.  A length out
-  // of range makes all its frames NaN.
-  const bool fits = n >= 0 && n <= a.T, finite = fabsf(raw) < INFINITY;
+  // frames of the utterance: a gradient where there is a finite loss and the lattice came to its end, else zeros or NaN;
+  // behind it zeros.  A length out of range makes all its frames NaN.
+  const bool fits = n >= 0 && n <= a.T, finite = fabsf(raw) < INFINITY && __ldg(a.again + b) != 3;
   const float other = raw == INFINITY && a.zero_infinity ? 0.f : NAN;
   const int count = fits ? min(n - t, F) : F;      // frames of the F that are not padding
   FrameGrad p[F];
@@ -1055,12 +1065,12 @@ __global__ void __launch_bounds__(WARP_ROW ? kRowThreads : kCtaThreads) ctc_grad
 
 constexpr size_t kMostSmem = 227 * 1024 - 1024;  // a CTA's, less the static part (of both walks)
 
-template <int NP, int H, int NBUF, bool GRAD>
+template <int NP, int H, int NBUF, bool GRAD, bool HOLD = false>
 int launch_lattice(const CtcArgs& a, int nw, cudaStream_t stream) {
   constexpr int HL = halo_lanes<NP, H>(), NS = 2 * NP;
   const size_t smem = (size_t)NBUF * H * a.pitch * 4 + (GRAD ? (size_t)NBUF * H * a.state_pitch * 4 : 0) +
                       (size_t)2 * nw * HL * NS * sizeof(float2) + (GRAD ? (size_t)2 * H * (nw * 32 + 4) * 4 : 0);
-  auto* kernel = ctc_lattice_kernel<NP, H, NBUF, GRAD>;
+  auto* kernel = ctc_lattice_kernel<NP, H, NBUF, GRAD, HOLD>;
   static std::atomic<uint64_t> allowed{0};
   if (int rc = allow_smem((const void*)kernel, kMostSmem, allowed)) return rc;
   return launch_behind(kernel, dim3(2, a.B), (nw + 1) * 32, smem, stream, a, nw);
@@ -1083,6 +1093,8 @@ LatticeShape lattice_shape(int pairs) {
 template <bool GRAD>
 int launch_lattice_for(const CtcArgs& a, cudaStream_t stream) {
   const LatticeShape s = lattice_shape(a.S + 1);
+  if constexpr (GRAD)
+    if (a.withhold) return launch_lattice<1, 16, 2, true, true>(a, s.nw, stream);
   if (s.NP == 1) return launch_lattice<1, 16, 2, GRAD>(a, s.nw, stream);
   if (s.NP == 2) return launch_lattice<2, 16, 2, GRAD>(a, s.nw, stream);
   if (s.NP == 3) return launch_lattice<3, 16, 2, GRAD>(a, s.nw, stream);

@@ -202,18 +202,20 @@ struct CtcArgs {
   float* post = nullptr;         // [B, T, pitch]: emission words, then posteriors, of the labels; blank's at S + 1
   int2* order = nullptr;         // [B, pitch] (place in post, class) in the order of the classes
   float* raw_loss = nullptr;     // [B] loss, inf where no path exists, NaN for bad input
+  int* again = nullptr;          // [B]: 1 states, 2 emissions too far apart, to be walked again; 3 a wait has run out
   float* loss = nullptr;         // [B] loss with zero_infinity applied
   int* bad = nullptr;            // workspace [B]: a length or label out of range
   float* norms = nullptr;        // workspace [B, T]: what each frame adds to -log2 Z
-  int* again = nullptr;          // workspace [B]: states (1) or emissions (2) too far apart, to be walked again
   float2* exchange = nullptr;    // workspace [B, 2, 2, 2 pitch]: both sides' states where they meet, of either walk
   uint32_t* states = nullptr;    // workspace [B, T, state_pitch], or null: no posteriors wanted
   uint32_t* upper = nullptr;     // workspace [B, T, pitch] beside it: upper halves of the exponents of a second walk
+  int withhold = 0;              // self-test: 1 + side + 2 * half, whose first copy of utterance 0 is armed, not issued
   const float* dloss = nullptr;  // [B]
   void* dlogits = nullptr;       // [B, T, V] dense
 };
 int ctc_pitch(int S);
 int ctc_state_pitch(int S);
+constexpr int kMaxCtcHeldLabels = 79;           // of the self-test's only form
 int launch_ctc_loss(const CtcArgs& args, int dtype, cudaStream_t stream);
 int launch_ctc_grad(const CtcArgs& args, int dtype, cudaStream_t stream);
 

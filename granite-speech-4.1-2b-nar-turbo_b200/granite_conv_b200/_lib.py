@@ -102,6 +102,8 @@ SIGNATURES = {
                                 _vp, _sz, _vp, _sz, _vp]),
     "gsn_ctc_loss_bwd": (_i32, [_fp, _vp, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp,
                                 _sz, _vp, _vp]),
+    "gsn_selftest_ctc_withheld": (_i32, [_vp, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _fp, _vp,
+                                         _sz, _vp, _sz, _i32, _i32, _vp]),
     "gsn_interleave_glu_rows": (_i32, [_vp, _vp, _i32, _i64, _vp]),
     "gsn_device_status": (_i32, [ctypes.POINTER(_i32), _i32, _vp]),
     "gsn_selftest_bounded_wait": (_i32, [_u64, _vp]),

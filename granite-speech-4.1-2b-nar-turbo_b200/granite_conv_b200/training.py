@@ -555,7 +555,7 @@ def _(logits, targets, input_lengths, target_lengths, blank, zero_infinity):
     B, T, _ = logits.shape
     S = targets.shape[1]
     pitch = (S + 6) // 4 * 4                       # as gsn_ctc_loss_state_bytes
-    sizes = (4 * B, 8 * B * T, 8 * B * pitch, 4 * B * T * pitch)
+    sizes = (4 * B, 4 * B, 8 * B * T, 8 * B * pitch, 4 * B * T * pitch)
     nbytes = sum((n + 255) // 256 * 256 for n in sizes)
     return logits.new_empty((B,), dtype=torch.float32), logits.new_empty((nbytes,), dtype=torch.uint8)
 

@@ -407,7 +407,8 @@ int gsn_dropout_add_layer_norm_bwd(const void* dy, int64_t ld_dy, const void* dh
  *   frame.
  *   workspace: gsn_ctc_loss_workspace_bytes(B, T, S, gradient) bytes.  Both 16-byte aligned.
  * gsn_ctc_loss_bwd: dlogits [B, T, V] dense, dloss[b] * d loss[b] / d logits; 0 in padding frames, for utterances
- *   without an alignment 0 with zero_infinity and NaN without, NaN for the others whose loss is NaN. */
+ *   without an alignment 0 with zero_infinity and NaN without, NaN for the others whose loss is NaN and where a bounded
+ *   wait of the forward pass ran out (gsn_device_status then reads 0x105). */
 size_t gsn_ctc_loss_state_bytes(int B, int T, int S);
 
 size_t gsn_ctc_loss_workspace_bytes(int B, int T, int S, int gradient);
@@ -464,14 +465,23 @@ int gsn_selftest_bounded_wait(uint64_t limit_ns, gsn_stream_t stream);
  *     TMEM accumulator when the MMA warp gives up;
  *   gsn_selftest_dwconv_withheld_bf16: the depthwise kernel (operands as gsn_dwconv_silu_bf16, without lengths),
  *     withholding each CTA's first tile; the layouts the TMA kernels take (channels-last rows, or T innermost with
- *     16-byte aligned rows and C % 64 == 0) exercise it.
+ *     16-byte aligned rows and C % 64 == 0) exercise it;
+ *   gsn_selftest_ctc_withheld: the CTC loss (operands as gsn_ctc_loss_fwd with a gradient, S <= 79), withholding the
+ *     first frames of utterance 0 on one side (0: the chain from the first frame, 1: from the last) in one half (0:
+ *     before the sides meet: its loss is NaN; 1: behind that: the loss is there, its gradient is NaN).
  * Every role then unwinds: copies in flight land, TMEM is freed, the kernel returns, and gsn_device_status reads a
- * timeout code (0x101-0x104).  The output is left partly written; the context stays usable. */
+ * timeout code (0x101-0x105; 0x105 is the CTC loss's).  What else it writes is left partly written; the context stays
+ * usable. */
 int gsn_selftest_gemm_withheld_bf16(const void* d, const void* w, const float* b, const void* residual, void* out,
                                     int M, int K, int N, gsn_stream_t stream);
 int gsn_selftest_dwconv_withheld_bf16(const void* x, const void* w, const void* b, void* y, int B, int C, int T,
                                       int64_t sxB, int64_t sxC, int64_t sxT, int64_t syB, int64_t syC, int64_t syT,
                                       gsn_stream_t stream);
+
+int gsn_selftest_ctc_withheld(const void* logits, int64_t ld_b, int64_t ld_t, const int32_t* targets,
+                              const int32_t* input_lengths, const int32_t* target_lengths, int B, int T, int V, int S,
+                              int blank, int dtype, float* loss, void* state, size_t state_bytes, void* workspace,
+                              size_t workspace_bytes, int side, int half, gsn_stream_t stream);
 
 #ifdef __cplusplus
 }

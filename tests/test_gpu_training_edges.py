@@ -250,3 +250,36 @@ def test_sizes_past_32_bits_are_refused():
         tr.ctc_loss(one.expand(1, 1, 2 ** 32 + 5), i[None], i, i)
     with pytest.raises(RuntimeError, match="utterances"):
         tr.ctc_loss(one.expand(2 ** 32 + 1, 0, 5), i.expand(2 ** 32 + 1, 0), i.expand(2 ** 32 + 1), i.expand(2 ** 32 + 1))
+
+
+# ---- a wait that runs out --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("far", [False, True])
+@pytest.mark.parametrize("side,half", [(0, 0), (1, 0), (0, 1), (1, 1)])
+def test_ctc_wait_that_runs_out_is_nan(side, half, far):
+    """A copy armed and never issued on one side: the status word reads 0x105, that utterance's gradient is NaN, its
+    loss too before the sides have met, the other utterance's are what they are, and the next call is as always.  far:
+    an utterance that is walked again for its posteriors."""
+    from granite_conv_b200 import _lib
+    if far:
+        case = run_case(60, 24, [("a", 80, 20.0), ("blank", 80, 20.0), ("a", 85, 20.0)])
+        logits, targets, il, tl = (torch.cat([t, t]).contiguous() for t in case)
+    else:
+        logits, targets, il, tl = ctc_case(90, 2, 150, 20, 40, F32, ([150, 141], [40, 39]))
+    _, T, V = logits.shape
+    S = targets.shape[1]
+    L, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    loss = torch.zeros(2, device=DEV)
+    state = torch.zeros(L.gsn_ctc_loss_state_bytes(2, T, S), dtype=torch.uint8, device=DEV)
+    ws = torch.zeros(L.gsn_ctc_loss_workspace_bytes(2, T, S, 1), dtype=torch.uint8, device=DEV)
+    _lib.device_status(stream, clear=True)
+    _lib.call("gsn_selftest_ctc_withheld", logits.data_ptr(), T * V, V, targets.data_ptr(), il.data_ptr(), tl.data_ptr(),
+              2, T, V, S, 0, 2, loss.data_ptr(), state.data_ptr(), state.numel(), ws.data_ptr(), ws.numel(), side, half,
+              stream)
+    assert _lib.device_status(stream, clear=True) == 0x105
+    want = tr.ctc_loss(logits, targets, il, tl)
+    assert loss[1] == want[1] and (torch.isnan(loss[0]) if half == 0 else loss[0] == want[0])
+    grad = tr._ctc_loss_backward(torch.ones(2, device=DEV), logits, targets, il, tl, state, 0, False)
+    assert torch.isnan(grad[0]).all() and torch.isfinite(grad[1]).all()
+    _, good = check_ctc(logits, targets, il, tl, dloss=torch.ones(2, device=DEV))
+    assert torch.equal(grad[1], good[1])
+    assert _lib.device_status(stream, clear=False) == 0

@@ -256,3 +256,13 @@ def test_sizes_past_32_bits_are_refused():
     with pytest.raises(RuntimeError, match="elements expected"):
         training._check_rows("rows", one.expand(2 ** 32 + 5))
     training._check_rows("rows", one.expand(2 ** 31 - 256))
+
+
+def test_ctc_selftest_refuses_bad_calls():
+    L = _lib.lib()
+
+    def call(side=0, half=0, B=2, nbytes=0, S=3):
+        return L.gsn_selftest_ctc_withheld(P, 35, 7, P, P, P, B, 5, 7, S, 0, 0, P, P, 1 << 20, P, nbytes, side, half, None)
+
+    assert call(side=2) == 1 and call(side=-1) == 1 and call(half=2) == 1 and call(B=-1) == 1 and call(S=80) == 2
+    assert call() == 5 and "gsn_selftest_ctc_withheld: workspace" in _lib.last_error() and call(B=0) == 0
