@@ -295,9 +295,10 @@ __device__ __forceinline__ void write_emissions(const CtcArgs& a, const T* x, in
     }
 }
 
-// what the frame adds to -log2 Z: its emissions are against `best` instead of the softmax's denominator
+// what the frame adds to -log Z: its emissions are against `best` instead of the softmax's denominator.  Natural, so that
+// a difference of the type's lowest value stays finite.
 __device__ __forceinline__ float frame_norm(const Online& o, float best) {
-  return log2f(o.sum) + (best == -INFINITY ? 0.f : (o.top - best) * kLog2e);
+  return logf(o.sum) + (best == -INFINITY ? 0.f : o.top - best);
 }
 
 constexpr int kRowThreads = 256;
@@ -892,7 +893,7 @@ __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
     if ((!WIDE || again == 2) && dir == 0 && tid == 0) {
       norm = norms_sum;
       float raw = INFINITY;
-      if (exists) raw = (float)((norm - (double)top - log2((double)total)) * 0.6931471805599453);
+      if (exists) raw = (float)(norm - ((double)top + log2((double)total)) * 0.6931471805599453);
       if (!(norm > -INFINITY)) raw = NAN;          // a frame of NaN, +inf or nothing but -inf
       a.raw_loss[b] = raw;
       a.loss[b] = a.zero_infinity && raw == INFINITY ? 0.f : raw;

@@ -205,7 +205,7 @@ struct CtcArgs {
   int* again = nullptr;          // [B]: 1 states, 2 emissions too far apart, to be walked again; 3 a wait has run out
   float* loss = nullptr;         // [B] loss with zero_infinity applied
   int* bad = nullptr;            // workspace [B]: a length or label out of range
-  float* norms = nullptr;        // workspace [B, T]: what each frame adds to -log2 Z
+  float* norms = nullptr;        // workspace [B, T]: what each frame adds to -log Z
   float2* exchange = nullptr;    // workspace [B, 2, 2, 2 pitch]: both sides' states where they meet, of either walk
   uint32_t* states = nullptr;    // workspace [B, T, state_pitch], or null: no posteriors wanted
   uint32_t* upper = nullptr;     // workspace [B, T, pitch] beside it: upper halves of the exponents of a second walk

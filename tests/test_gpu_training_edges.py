@@ -283,3 +283,31 @@ def test_ctc_wait_that_runs_out_is_nan(side, half, far):
     _, good = check_ctc(logits, targets, il, tl, dloss=torch.ones(2, device=DEV))
     assert torch.equal(grad[1], good[1])
     assert _lib.device_status(stream, clear=False) == 0
+
+
+def test_ctc_transcript_at_the_lowest_value():
+    """A frame whose classes of the transcript all have the type's lowest value beside others at 0: the loss is that
+    value, and the gradient finite; two such frames are beyond fp32.  Next to a log Z of 3.4e38 the posteriors of a
+    64-bit recursion are lost (an ulp of 2^76): they are taken from the same frame with the other classes impossible,
+    which scales Z and changes no path's share of it."""
+    for dtype in (F32, BF, HF):
+        low = torch.finfo(dtype).min
+        logits, targets, il, tl = ctc_case(46, 2, 12, 9, 3, dtype, labels=[[1, 2, 3]] * 2)
+        logits[:, 5, :4] = low
+        logits[1, 6, :4] = low
+        shares = logits[:1].clone()
+        shares[:, 5, :4], shares[:, 5, 4:] = 0.0, -math.inf
+        ref = R.ctc(shares, targets[:1], il[:1], tl[:1], 0, False)[1]
+        p, q = (torch.softmax(t.double().cpu(), -1) for t in (logits[:1], shares))
+        ref = p - (q - ref)
+        for zero_infinity in (False, True):
+            x = logits.clone().requires_grad_()
+            loss = tr.ctc_loss(x, targets, il, tl, zero_infinity=zero_infinity)
+            grad, = torch.autograd.grad(loss.sum(), x)
+            assert abs(loss[0].item() + low) <= 2.0 ** -24 * abs(low) + 100
+            bound = rounded(dtype, ref) + (9 / 256 + 100 + 12 * 64 + 164) * E        # as in check_ctc
+            close(grad[:1], ref, bound, (dtype, zero_infinity))
+            if dtype == HF:
+                assert abs(loss[1].item() + 2 * low) < 200
+            else:
+                assert loss[1].item() == (0.0 if zero_infinity else math.inf)
