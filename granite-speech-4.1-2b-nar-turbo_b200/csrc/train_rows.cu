@@ -897,10 +897,10 @@ int launch_rows(const RowArgs& a, bool bwd, cudaStream_t stream) {
 template <typename T, bool RES>
 int launch_dropout(const RowArgs& a, bool vec, cudaStream_t stream) {
   const bool flat = vec && !a.lengths && (a.ld_x == a.D || a.M == 1) && (!RES || a.ld_res == a.D || a.M == 1);
-  // Blocks where they are at least three fifths full.  30 M elements of bf16 without a residual: 53 us in full blocks,
-  // 77 us at D = 150, 113 us at 100, 169 us at 65; eight neighbours a lane 86 to 88 us at any width.
+  // Blocks where they are at least 11 twentieths full.  30 M elements of bf16 without a residual: 55 us at D = 1001, 80
+  // us at 150, 84 at 141, 86 at 137, 90 at 131, 96 at 121, 115 at 100; eight neighbours a lane 90 to 92 us at each.
   const int64_t blocks = (a.D + 255) / 256;
-  if (!vec && (int64_t)a.D * 5 >= blocks * 256 * 3) {
+  if (!vec && (int64_t)a.D * 20 >= blocks * 256 * 11) {
     const int64_t want = (a.M * blocks + 7) / 8, most = 8 * device_sm_count();
     dropout_block_kernel<T><<<(int)(want < most ? want : most), 256, 0, stream>>>(a);
     return (int)cudaGetLastError();

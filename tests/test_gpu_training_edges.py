@@ -311,3 +311,15 @@ def test_ctc_transcript_at_the_lowest_value():
                 assert abs(loss[1].item() + 2 * low) < 200
             else:
                 assert loss[1].item() == (0.0 if zero_infinity else math.inf)
+
+
+@pytest.mark.parametrize("D", [139, 141, 150, 281, 282])
+def test_dropout_on_either_side_of_its_rule(D):
+    """Off the 16-byte grid, around the width where blocks of 256 columns take over: the same mask and values."""
+    x, res = rand(95, (3, 7, D), BF), rand(96, (3, 7, D), BF)
+    keep = R.keep_mask(x.shape, 99, 1, 6, 0.4)
+    assert torch.equal(tr.dropout_add(torch.ones_like(x), rng_of(99, 1), 0.4, site=6).cpu() != 0, keep)
+    out = tr.dropout_add(x, rng_of(99, 1), 0.4, residual=res, site=6, lengths=lens_of([7, 0, 3]))
+    ref = R.dropout_add(x, res, 99, 1, 6, 0.4, 1.0, [7, 0, 3])
+    k = R.factor(0.4, 1.0)
+    close(out, ref, rounded(BF, ref) + 2 * E * (k * x.double().cpu().abs() + res.double().cpu().abs()))
