@@ -302,7 +302,10 @@ __device__ __forceinline__ float frame_norm(const Online& o, float best) {
 }
 
 constexpr int kRowThreads = 256;
-constexpr int kWarpRowV = 2048;                  // up to it a warp takes a row, beyond it a CTA
+// Up to it a warp takes a row, beyond it a CTA.  Loss and gradient in a warp | in a CTA, bf16: 48 x 384 x 2048 61 + 47 |
+// 89 + 94 us, 48 x 384 x 4096 78 + 88 | 100 + 109, 48 x 128 x 8192 51 + 66 | 51 + 53; but one utterance of 60 frames
+// waits for its rows: 22.5 + 10.2 | 20.5 + 8.2 at 2048 classes, 24.6 + 14.3 | 20.5 + 8.2 at 4096.
+constexpr int kWarpRowV = 2048;
 
 // Frames of one utterance that a warp takes: two, which share what is looked up of the transcript, where that leaves
 // 16 warps an SM; a CTA takes one.  48 x 1536 x 348 with 300 labels: rows and gradient 47 and 59 us, with three frames
@@ -359,8 +362,9 @@ __global__ void __launch_bounds__(kRowThreads) ctc_rows_kernel(CtcArgs a) {
 // Within a block of H frames a lane may hold its states as fp64 against one exponent, the largest of the states that
 // can reach it: a step is then two products and three multiply-adds a pair (behind the meeting, which wants the sums
 // before the emission: two additions, a multiply-add, two products), and the stored words are used as they are.  A warp takes this form where its states (else the states of each lane's reach) and the block's emissions
-// together span no more than kFastSpan octaves, which keeps every state of weight a normal number; any other block,
-// and one that is not whole, runs on the exponent of every state, at three times the instructions.
+// together span no more than kFastSpan octaves, which keeps every state of weight a normal number, and no lane's states
+// lie out of the factor's reach from the lane above; any other block, and one that is not whole, runs on the exponent
+// of every state, at three times the instructions.
 //
 // Bound by the instructions of one warp a scheduler: at 48 utterances of 1536 frames with 300 labels (195 us) a step
 // takes 171 cycles before the meeting and 357 behind it, 60 of them a block's begin and end; HBM and the fp64 pipe wait.
@@ -1079,7 +1083,9 @@ int launch_lattice(const CtcArgs& a, int nw, cudaStream_t stream) {
 
 // Pairs a lane: as few as four warps hold (one a scheduler of the SM, so that a step issues in the least time), then
 // four pairs and more warps.  Frames a block: 16 where they fit (48 utterances of 1536 frames with 300 labels: 195 us,
-// with 8 frames 252 us: about 500 cycles go into a block's begin and end), fewer where the rows get long.
+// with 8 frames 252 us: about 500 cycles go into a block's begin and end), fewer where the rows get long: beyond 967
+// labels two buffers of eight frames, their states and nine warps' blanks come near a CTA's shared memory and at 1000
+// past it.  48 utterances, a frame with its gradient: 0.74 us at 967 labels, 0.93 at 968.
 struct LatticeShape {
   int NP, H, nw;
 };

@@ -828,7 +828,8 @@ __global__ void __launch_bounds__(256) dropout_block_kernel(RowArgs a) {
 
 // A row's warps and blocks of 256 columns a warp.  Two blocks, 16 columns a lane, leave 16 warps an SM beside the
 // weights and the sums of their gradients in registers; the widest rows take four.  At 73728 x 1024 bf16 backward, fused
-// with dropout, two blocks take 123 us and four 122, one block 158; of the odd 11376 x 1001, 36, 51 and 32 us.
+// with dropout, two blocks take 123 us and four 122, one block 158; of the odd 11376 x 1001, 36, 51 and 32 us.  One shape
+// a width: the partial rows of the weights' gradients are counted before anything is known of the rows' alignment.
 struct RowShape {
   int W, NV, warps;
 };

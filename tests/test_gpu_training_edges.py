@@ -1,4 +1,4 @@
-"""The fine-tuning operators at the edges of their ranges: each test here failed before what it names was put right."""
+"""The fine-tuning operators at the edges of their ranges: where they once were wrong, and where a rule changes sides."""
 import math
 
 import numpy as np
