@@ -233,7 +233,7 @@ class _LayerNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, lengths = ctx.saved_tensors
-        return (*_layer_norm_backward(dy, x, weight, ctx.eps, lengths), None, None)
+        return (*layer_norm_backward(dy, x, weight, ctx.eps, lengths), None, None)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, eps: float = 1e-5,
@@ -445,8 +445,8 @@ class _DropoutAddLayerNorm(torch.autograd.Function):
         if dy is None and dh is None:
             return (None,) * 10
         if dy is None:
-            return (_dropout_add(dh, None, rng, ctx.p, ctx.scale, ctx.site, lengths), dh, None, None, *rest)
-        return (*_dropout_add_layer_norm_backward(dy, dh, h, weight, rng, ctx.p, ctx.scale, ctx.site, ctx.eps, lengths),
+            return (dropout_add_backward(dh, rng, ctx.p, ctx.scale, ctx.site, lengths), dh, None, None, *rest)
+        return (*dropout_add_layer_norm_backward(dy, dh, h, weight, rng, ctx.p, ctx.scale, ctx.site, ctx.eps, lengths),
                 *rest)
 
 
@@ -601,7 +601,8 @@ class _CtcLoss(torch.autograd.Function):
     def backward(ctx, dloss, _):
         dx = None
         if dloss is not None:
-            dx = _ctc_loss_backward(dloss, *ctx.saved_tensors, ctx.blank, ctx.zero_infinity)
+            backward = torch.ops.granite.ctc_loss_backward if _dispatched(dloss) else _ctc_loss_backward
+            dx = backward(dloss, *ctx.saved_tensors, ctx.blank, ctx.zero_infinity)
         return dx, None, None, None, None, None
 
 

@@ -196,6 +196,24 @@ def test_traced_calls_compute():
             assert torch.equal(g(to), want)
 
 
+def test_traced_gradients_compute():
+    """A tracer that sees only the backward pass of a call made before it records the ops of that."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, y = (rand(s, (2, 5, 40), F32) for s in (66, 67))
+    w, b, rng = rand(68, (40,), F32, 0.2, 1.0), rand(69, (40,), F32), rng_of()
+    logits, targets, il, tl = ctc_case(70, 2, 9, 7, 3, F32)
+    calls = [(lambda a: tr.layer_norm(a, w, b), x), (lambda a: tr.dropout_add(a, rng, 0.3, residual=y), x),
+             (lambda a: tr.dropout_add_layer_norm(a, y, w, b, rng, 0.3)[0], x),
+             (lambda a: tr.dropout_add_layer_norm(a, y, w, b, rng, 0.3)[1], x),
+             (lambda a: tr.ctc_loss(a, targets, il, tl), logits)]
+    for f, at in calls:
+        leaf = at.clone().requires_grad_()
+        out = f(leaf)
+        first, second = (torch.linspace(a, 2.0, out.numel(), device=DEV).reshape(out.shape) for a in (-1.0, 0.5))
+        graph = make_fx(lambda d: torch.autograd.grad(out, leaf, d, retain_graph=True)[0])(first)
+        assert torch.equal(graph(second), torch.autograd.grad(out, leaf, second, retain_graph=True)[0])
+
+
 def test_forward_mode_is_refused():
     """Dual tensors are refused by the functions and by the ops behind them."""
     from torch.autograd import forward_ad
