@@ -2,8 +2,9 @@
 regenerated from a counter, never stored), the residual step fused with the norm behind it (a Conformer block's tail,
 ``models/granite_speech_nar/conformer.py:208-209``), and the CTC loss of the heads (``:240-252``) with its gradient.
 
-The functions here take plain tensors and are differentiable; without a gradient to record they launch the kernel
-directly.  Each is also a ``torch.library`` op, so ``torch.compile(fullgraph=True)`` sees one node:
+The functions here take plain tensors and are differentiable (the ``*_backward`` ones, for gradients by hand, record
+nothing); without a gradient to record they launch the kernel directly.  Each is also a ``torch.library`` op, so
+``torch.compile(fullgraph=True)`` and other tracers see one node:
 
 * ``granite::layer_norm(x, weight, bias, eps, lengths?)``, ``granite::layer_norm_backward``
 * ``granite::dropout_add(x, residual?, rng, p, scale, site, lengths?)``
@@ -13,9 +14,10 @@ directly.  Each is also a ``torch.library`` op, so ``torch.compile(fullgraph=Tru
   ``granite::ctc_loss_backward``
 
 Tensors are bf16, fp16 or fp32 on one CUDA device, parameters fp32 or of the activations' type; work runs on that
-device's current stream.  Results repeat bit for bit.  Tensors with a forward-mode tangent are refused.  ``lengths``
-(int [B], with x [B, T, D]) marks the frames t >= lengths[b] as padding: nothing of them is read, normed outputs and
-gradients there are zero, they join no weight gradient, and a residual passes through.
+device's current stream.  Results repeat bit for bit.  Tensors with a forward-mode tangent are refused (by the bare
+ops as dual tensors only: under ``torch.func.jvp`` torch hands a custom op the values alone).  ``lengths`` (int [B], with
+x [B, T, D]) marks the frames t >= lengths[b] as padding: nothing of them is read, normed outputs and gradients there are
+zero, they join no weight gradient, and a residual passes through.
 
 ``rng`` is an int64 tensor of two on the device, (seed, offset), which the kernels read when they run: a captured graph
 draws new masks when it holds ``rng[1] += 1`` after its backward pass.  ``site`` tells apart the dropouts of one step.
@@ -195,15 +197,15 @@ def _(dy, x, weight, eps, lengths):
 
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 _compiling = torch.compiler.is_compiling
-_tracing = torch._C._get_tracing_state
+_tracing = torch._C._is_tracing
 _modes = torch._C._len_torch_dispatch_stack
-_early_modes = torch._ops._len_torch_dispatch_stack_pre_dispatch
+_early_modes = torch._ops.mode_stack_state_for_pre_dispatch().count
 
 
 def _dispatched(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether a call has to go through the dispatcher: a graph being compiled or traced (whatever watches the ops that
     are called would see an empty output and no kernel), another mode that takes them, or a tensor subclass."""
-    if _compiling() or _tracing() is not None or _modes() or _early_modes():
+    if _compiling() or _tracing() or _modes() or _early_modes():
         return True
     for t in tensors:
         if t is not None and type(t) not in _PLAIN:
