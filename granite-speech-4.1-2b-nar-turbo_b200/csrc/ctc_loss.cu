@@ -531,6 +531,13 @@ __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
     [[maybe_unused]] uint32_t* dst = a.states + frame * spitch;
     [[maybe_unused]] uint32_t* upper = a.upper + frame * pitch;
     [[maybe_unused]] float* bl = blanks + parity * H * brow + tid;
+    [[maybe_unused]] uint32_t ahead[NP + 1];       // the next frame's upper halves, of pairs q0 - j
+    auto load_upper = [&]() {
+      if constexpr (SECOND && WIDE)
+#pragma unroll
+        for (int j = 0; j <= NP; ++j) ahead[j] = __ldcg(upper + max(q0 - j, 0));
+    };
+    load_upper();
     for (int f = 0; f < cnt; ++f) {
       float pm[NS];
       int pe[NS];
@@ -556,20 +563,23 @@ __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
         }
       }
       if constexpr (SECOND && WIDE) {
-        auto joint = [&](int q, int s, float pm, int pe) {         // with state s (0 blank, 1 label) of the pair q
-          q = max(q, 0);
-          const uint32_t v = st[2 * q + s], u = __ldcg(upper + q) >> (16 * s) & 0xFFFFu;
+        uint32_t up[NP + 1];
+#pragma unroll
+        for (int j = 0; j <= NP; ++j) up[j] = ahead[j];
+        upper += step * pitch;
+        if (f + 1 < cnt) load_upper();
+        auto joint = [&](int j, int s, float pm, int pe) {         // with state s (0 blank, 1 label) of the pair q0 - j
+          const uint32_t v = st[2 * max(q0 - j, 0) + s], u = up[j] >> (16 * s) & 0xFFFFu;
           return u == 0 ? 0.f : pm * (wide_mantissa(v) * zinv) * pow2i(wide_exponent(v, u) - zexp + pe);
         };
         float blank = 0.f;
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
-          if (j < blanks_here) blank += joint(q0 - j, 0, pm[2 * j], pe[2 * j]);
-          if (j < labels_here) post[slot[j]] = joint(q0 - j - 1, 1, pm[2 * j + 1], pe[2 * j + 1]);
+          if (j < blanks_here) blank += joint(j, 0, pm[2 * j], pe[2 * j]);
+          if (j < labels_here) post[slot[j]] = joint(j + 1, 1, pm[2 * j + 1], pe[2 * j + 1]);
         }
         bl[f * brow] = blank;
         post += step * pitch;
-        upper += step * pitch;
         st += step * spitch;
       } else if constexpr (SECOND) {
         const int rh = (int)st[ref_hi] - zexp, rl = (int)st[ref_lo] - zexp;
@@ -832,7 +842,7 @@ __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
   walk(0, n1, std::false_type{});
 
   // the meeting: Z = sum over the states of this side's sum into them times the other side's value
-  // (one place for either walk: the other side may still be at the first one's meeting)
+  // (a place of its own for either walk: the other side may still be at the first one's meeting)
   float2* mine = a.exchange + (((int64_t)b * 2 + WIDE) * 2 + dir) * 2 * pitch;
   const float2* theirs = a.exchange + (((int64_t)b * 2 + WIDE) * 2 + (dir ^ 1)) * 2 * pitch;
 #pragma unroll
@@ -920,7 +930,8 @@ __device__ __forceinline__ bool lattice_walk(const CtcArgs& a, int nw) {
   return false;
 }
 
-// a function of its own: its code beside the other walk's took a fifth of that one's speed
+// A function of its own: its code beside the other walk's took a fifth of that one's speed.  48 utterances of 799 frames
+// with 300 labels, all of them walked again: 530 us with the gradient, 178 where none is.
 template <int NP, int H, int NBUF, bool GRAD, bool HOLD>
 __device__ __noinline__ void lattice_wide(const CtcArgs& a, int nw) {
   if (__ldcg(a.again + blockIdx.y) == 3) return;   // the other side has given up
